@@ -1,13 +1,12 @@
 // Bandwidth-bound elementwise kernels of the transformer block, all on 16-byte
 // bf16 vectors: GELU(tanh) and SwiGLU forward/backward, bias-dropout-add, rotary
-// embedding on packed qkv, embedding lookup / scatter, bias-gradient column sums,
+// embedding on packed qkv, bias-gradient column sums,
 // dtype casts and gradient accumulation.
 //
 // Reference counterparts: jiterator swiglu (mist/modules/activations.py:115-149),
 // TorchScript bias_gelu / bias_dropout_add (mist/modules/activations.py:16-112,
 // mist/model/transformer.py:535-546), Triton rotary kernel
-// (mist/modules/triton/rotary.py:20-51), csrc/rotary/rotary_cuda.cu:9-44,
-// embedding modules (mist/modules/embedding.py:207-281).
+// (mist/modules/triton/rotary.py:20-51), csrc/rotary/rotary_cuda.cu:9-44.
 #include "common.cuh"
 
 namespace {
@@ -213,85 +212,6 @@ __global__ void rope_kernel(__nv_bfloat16* __restrict__ qkv, const float* __rest
   }
 }
 
-// --------------------------------------------------------------- embedding
-// out[t] = wte[ids[t] - v0] (zero when the id is outside [v0, v1)) + wpe[t % seq]
-__global__ void embedding_fwd_kernel(const int64_t* __restrict__ ids,
-                                     const __nv_bfloat16* __restrict__ wte,
-                                     const __nv_bfloat16* __restrict__ wpe,
-                                     __nv_bfloat16* __restrict__ out, size_t tokens, int seq, int h,
-                                     int v0, int v1) {
-  const int vpr = h >> 3;
-  const size_t nvec = tokens * vpr;
-  for (size_t i = blockIdx.x * static_cast<size_t>(kBlock) + threadIdx.x; i < nvec;
-       i += static_cast<size_t>(gridDim.x) * kBlock) {
-    size_t t = i / vpr;
-    int c = static_cast<int>(i - t * vpr) * 8;
-    int64_t id = ids[t];
-    float f[8];
-    if (id >= v0 && id < v1)
-      mb::unpack8(*reinterpret_cast<const mb::bf16x8*>(wte + (id - v0) * h + c), f);
-    else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = 0.f;
-    }
-    if (wpe) {
-      float p[8];
-      mb::unpack8(*reinterpret_cast<const mb::bf16x8*>(wpe + (t % seq) * h + c), p);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] += p[k];
-    }
-    *reinterpret_cast<mb::bf16x8*>(out + t * h + c) = mb::pack8(f);
-  }
-}
-// dwte[ids[t] - v0] += dout[t]   (fp32 accumulation buffer, atomics: of 16 bytes where the buffer is aligned for them,
-// since the rate is one of requests, not of bytes: 16384 tokens of 2560 values 254 -> 87 us)
-template <bool VEC>
-__global__ void embedding_bwd_kernel(const int64_t* __restrict__ ids,
-                                     const __nv_bfloat16* __restrict__ dout,
-                                     float* __restrict__ dwte, size_t tokens, int h, int v0,
-                                     int v1) {
-  const int vpr = h >> 3;
-  const size_t nvec = tokens * vpr;
-  for (size_t i = blockIdx.x * static_cast<size_t>(kBlock) + threadIdx.x; i < nvec;
-       i += static_cast<size_t>(gridDim.x) * kBlock) {
-    size_t t = i / vpr;
-    int c = static_cast<int>(i - t * vpr) * 8;
-    int64_t id = ids[t];
-    if (id < v0 || id >= v1) continue;
-    float f[8];
-    mb::unpack8(*reinterpret_cast<const mb::bf16x8*>(dout + t * h + c), f);
-    float* dst = dwte + (id - v0) * h + c;
-    if (VEC) {
-      atomicAdd(reinterpret_cast<float4*>(dst), make_float4(f[0], f[1], f[2], f[3]));
-      atomicAdd(reinterpret_cast<float4*>(dst) + 1, make_float4(f[4], f[5], f[6], f[7]));
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) atomicAdd(dst + k, f[k]);
-    }
-  }
-}
-// dwpe[s] = sum_b dout[b*seq + s]
-__global__ void pos_embedding_bwd_kernel(const __nv_bfloat16* __restrict__ dout,
-                                         float* __restrict__ dwpe, int batch, int seq, int h) {
-  const int vpr = h >> 3;
-  const size_t nvec = static_cast<size_t>(seq) * vpr;
-  for (size_t i = blockIdx.x * static_cast<size_t>(kBlock) + threadIdx.x; i < nvec;
-       i += static_cast<size_t>(gridDim.x) * kBlock) {
-    size_t s = i / vpr;
-    int c = static_cast<int>(i - s * vpr) * 8;
-    float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int b = 0; b < batch; ++b) {
-      float f[8];
-      mb::unpack8(*reinterpret_cast<const mb::bf16x8*>(
-                      dout + (static_cast<size_t>(b) * seq + s) * h + c), f);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) acc[k] += f[k];
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) dwpe[s * h + c + k] += acc[k];
-  }
-}
-
 // --------------------------------------------------------- column reduction
 // out[c] (+)= sum_r x[r][c]; used for bias gradients.  Two stages through scratch:
 // stage 1 writes [parts][cols] partial sums, stage 2 adds them up.
@@ -323,23 +243,6 @@ __global__ void colsum_stage2(const float* __restrict__ part, OutT* __restrict__
 }
 
 // ------------------------------------------------------------------- casts
-// dst = bf16(dst + src): the sum is rounded once
-__global__ void add_f32_to_bf16_kernel(const float* __restrict__ src, __nv_bfloat16* __restrict__ dst, size_t n) {
-  const size_t nvec = n >> 3;
-  for (size_t i = blockIdx.x * static_cast<size_t>(kBlock) + threadIdx.x; i < nvec;
-       i += static_cast<size_t>(gridDim.x) * kBlock) {
-    const float4 a = reinterpret_cast<const float4*>(src)[2 * i], b = reinterpret_cast<const float4*>(src)[2 * i + 1];
-    float f[8];
-    mb::unpack8(reinterpret_cast<const mb::bf16x8*>(dst)[i], f);
-    f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w;
-    f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
-    reinterpret_cast<mb::bf16x8*>(dst)[i] = mb::pack8(f);
-  }
-  if (blockIdx.x == 0 && threadIdx.x < (n & 7)) {
-    const size_t j = (nvec << 3) + threadIdx.x;
-    dst[j] = __float2bfloat16(__bfloat162float(dst[j]) + src[j]);
-  }
-}
 __global__ void cast_f32_to_bf16_kernel(const float* __restrict__ in, __nv_bfloat16* __restrict__ out,
                                         size_t n, float scale) {
   const size_t nvec = n >> 3;
@@ -463,28 +366,6 @@ MB_API int mb_rope(void* qkv, const float* cosv, const float* sinv, size_t token
                                                 conj, n_rotated, row_stride);
   return LAUNCH_OK();
 }
-MB_API int mb_embedding_fwd(const int64_t* ids, const void* wte, const void* wpe, void* out,
-                            size_t tokens, int seq, int h, int v0, int v1, cudaStream_t s) {
-  if (h % 8) return -1;
-  if (!tokens) return 0;
-  embedding_fwd_kernel<<<grid_for(tokens * h / 8), kBlock, 0, s>>>(ids, BF(wte), BF(wpe), BFM(out),
-                                                                  tokens, seq, h, v0, v1);
-  return LAUNCH_OK();
-}
-MB_API int mb_embedding_bwd(const int64_t* ids, const void* dout, float* dwte, float* dwpe,
-                            int batch, int seq, int h, int v0, int v1, cudaStream_t s) {
-  if (h % 8) return -1;
-  size_t tokens = static_cast<size_t>(batch) * seq;
-  if (!tokens) return 0;
-  if ((reinterpret_cast<uintptr_t>(dwte) & 15) == 0)
-    embedding_bwd_kernel<true><<<grid_for(tokens * h / 8), kBlock, 0, s>>>(ids, BF(dout), dwte, tokens, h, v0, v1);
-  else
-    embedding_bwd_kernel<false><<<grid_for(tokens * h / 8), kBlock, 0, s>>>(ids, BF(dout), dwte, tokens, h, v0, v1);
-  if (dwpe)
-    pos_embedding_bwd_kernel<<<grid_for(static_cast<size_t>(seq) * h / 8), kBlock, 0, s>>>(
-        BF(dout), dwpe, batch, seq, h);
-  return LAUNCH_OK();
-}
 // scratch: ceil(rows / 256) * cols floats.
 MB_API int mb_colsum(const void* x, void* out, float* scratch, int rows, int cols, int out_fp32,
                      int accumulate, cudaStream_t s) {
@@ -505,12 +386,6 @@ MB_API int mb_colsum(const void* x, void* out, float* scratch, int rows, int col
 MB_API int mb_cast_f32_to_bf16(const float* in, void* out, size_t n, float scale, cudaStream_t s) {
   if (!n) return 0;
   cast_f32_to_bf16_kernel<<<grid_for((n + 7) / 8), kBlock, 0, s>>>(in, BFM(out), n, scale);
-  return LAUNCH_OK();
-}
-MB_API int mb_add_f32_to_bf16(const float* src, void* dst, size_t n, cudaStream_t s) {
-  if (!n) return 0;
-  if ((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst)) & 15) return -1;
-  add_f32_to_bf16_kernel<<<grid_for((n + 7) / 8), kBlock, 0, s>>>(src, BFM(dst), n);
   return LAUNCH_OK();
 }
 MB_API int mb_axpy_bf16_to_f32(const void* src, float* dst, size_t n, float scale, int accumulate,

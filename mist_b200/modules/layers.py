@@ -209,14 +209,9 @@ class VocabParallelEmbedding(nn.Module):
     def forward(self, input_ids, position_ids=None, tokentype_ids=None):
         ws = group_size(self.process_group)
         wpe = self.position_embeddings.weight if self.position_embeddings is not None else None
-        if position_ids is not None and wpe is not None:
-            # explicit position ids: gather rows, the fused kernel handles the arange case
-            x = F.embedding(input_ids, self.word_embeddings.weight, None, self.vocab_start)
-            pos = wpe[position_ids]
-            x = x + (pos if ws == 1 or group_rank(self.process_group) == 0 else 0)
-        else:
-            use_pos = wpe is not None and (ws == 1 or group_rank(self.process_group) == 0)
-            x = F.embedding(input_ids, self.word_embeddings.weight, wpe if use_pos else None, self.vocab_start)
+        use_pos = wpe is not None and (ws == 1 or group_rank(self.process_group) == 0)
+        x = F.embedding(input_ids, self.word_embeddings.weight, wpe if use_pos else None, self.vocab_start,
+                        position_ids=position_ids)
         if tokentype_ids is not None and self.tokentype_embeddings is not None:
             tt = self.tokentype_embeddings(tokentype_ids)
             x = x + (tt if ws == 1 or group_rank(self.process_group) == 0 else 0)

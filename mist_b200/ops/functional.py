@@ -1111,72 +1111,115 @@ def cross_entropy(logits, labels, vocab_start: int = 0, group=None, ignore_index
 
 
 # --------------------------------------------------------------------------- embedding
+def _elsewhere(t) -> bool:
+    """Whether ``t`` is on a GPU that is not the current one; kernels are launched on the current device."""
+    return t.is_cuda and t.get_device() != torch._C._cuda_getDevice()
+
+
+def _flat_positions(position_ids, ids):
+    """Explicit positions in the shape of ``ids``, or ``None``."""
+    if position_ids is None:
+        return None
+    if position_ids.is_floating_point() or position_ids.device != ids.device:
+        raise ValueError("position_ids: integers on the device of the ids expected")
+    return position_ids.expand(ids.shape).long().contiguous()
+
+
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ids, wte, wpe, v0):
+    def forward(ctx, ids, wte, wpe, v0, scale, pos):
         b, s = ids.shape
         h = wte.shape[1]
-        ctx.v0 = v0
+        ctx.v0, ctx.scale = v0, scale
         ctx.has_pos = wpe is not None
         ctx.param = _bucket_owner(wte)
-        ctx.save_for_backward(ids, wte, wpe)
-        v1 = v0 + wte.shape[0]
+        ctx.save_for_backward(ids, wte, wpe, pos)
         if not use_native(wte):
             loc = ids - v0
             inr = (loc >= 0) & (loc < wte.shape[0])
-            out = wte[loc.clamp(0, wte.shape[0] - 1)].float() * inr[..., None].float()
-            if wpe is not None:
+            out = wte[loc.clamp(0, wte.shape[0] - 1)].float() * (inr[..., None].float() * scale)
+            if wpe is not None and pos is None:
                 out = out + wpe[:s].float()[None]
+            elif wpe is not None:
+                known = (pos >= 0) & (pos < wpe.shape[0])
+                out = out + wpe[pos.clamp(0, wpe.shape[0] - 1)].float() * known[..., None].float()
             return out.to(wte.dtype)
-        ids = ids.contiguous()
         out = torch.empty(b, s, h, dtype=wte.dtype, device=wte.device)
-        call("mb_embedding_fwd", ptr(ids), ptr(wte), ptr(wpe), ptr(out), b * s, s, h, v0, v1, stream())
+        call("mb_embed_fwd", ptr(ids), ptr(pos), ptr(wte), ptr(wpe), ptr(out), b * s, s, h, v0, wte.shape[0],
+             0 if wpe is None else wpe.shape[0], scale, stream())
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        ids, wte, wpe = ctx.saved_tensors
+        ids, wte, wpe, pos = ctx.saved_tensors
         b, s = ids.shape
         h = wte.shape[1]
-        v0, v1 = ctx.v0, ctx.v0 + wte.shape[0]
-        bucket = getattr(ctx.param, "grad_bucket", None) if use_native(wte) and ctx.needs_input_grad[1] else None
-        accumulate = bool(getattr(ctx.param, "grad_accumulate", False))
-        if bucket is not None and bucket.dtype == torch.float32 and bucket.is_contiguous():      # summed in place
-            dwte = bucket if accumulate else bucket.zero_()
-        else:
-            dwte = torch.zeros(wte.shape, dtype=torch.float32, device=wte.device)
-        dwpe = torch.zeros(wpe.shape, dtype=torch.float32, device=wte.device) if ctx.has_pos else None
+        want_wte, want_wpe = ctx.needs_input_grad[1], ctx.has_pos and ctx.needs_input_grad[2]
         if not use_native(wte):
-            loc = ids - v0
+            dwte = torch.zeros(wte.shape, dtype=torch.float32, device=wte.device)
+            dwpe = torch.zeros(wpe.shape, dtype=torch.float32, device=wte.device) if ctx.has_pos else None
+            loc = ids - ctx.v0
             inr = (loc >= 0) & (loc < wte.shape[0])
             d2 = dout.float().reshape(-1, h)
             sel = inr.reshape(-1)
-            dwte.index_add_(0, loc.reshape(-1)[sel], d2[sel])
-            if dwpe is not None:
+            dwte.index_add_(0, loc.reshape(-1)[sel], d2[sel] * ctx.scale)
+            if dwpe is not None and pos is None:
                 dwpe[:s] += dout.float().sum(0)
-        else:
-            dout = dout.contiguous()
-            call("mb_embedding_bwd", ptr(ids.contiguous()), ptr(dout), ptr(dwte), ptr(dwpe), b, s, h, v0,
-                 v1, stream())
-        dwpe = None if dwpe is None else dwpe.to(wpe.dtype)
+            elif dwpe is not None:
+                known = ((pos >= 0) & (pos < wpe.shape[0])).reshape(-1)
+                dwpe.index_add_(0, pos.reshape(-1)[known], d2[known])
+            return None, dwte.to(wte.dtype), None if dwpe is None else dwpe.to(wpe.dtype), None, None, None
+        bucket = getattr(ctx.param, "grad_bucket", None) if want_wte else None
+        accumulate = bucket is not None and bool(getattr(ctx.param, "grad_accumulate", False))
+        direct = (bucket is not None and bucket.dtype in (torch.float32, torch.bfloat16) and bucket.is_contiguous()
+                  and ptr(bucket) % 16 == 0)
+        dwte = None
+        if direct:
+            dwte = bucket
+        elif want_wte:
+            dwte = torch.empty(wte.shape, dtype=wte.dtype if bucket is None else torch.float32, device=wte.device)
+        dwpe = torch.empty_like(wpe) if want_wpe else None
+        dout = dout.contiguous()
+        if ptr(dout) % 16:
+            dout = dout.clone()
+        area = native.kernels().mb_embed_bwd_workspace(b * s, h, int(want_wpe and pos is not None))
+        workspace = torch.empty(area, dtype=torch.uint8, device=wte.device)
+        call("mb_embed_bwd", ptr(ids), ptr(pos), ptr(dout), ptr(dwte), ptr(dwpe), b * s, s, h, ctx.v0, wte.shape[0],
+             wpe.shape[0] if want_wpe else 0, ctx.scale, int(dwte is not None and dwte.dtype == torch.float32),
+             int(direct and accumulate), ptr(workspace), stream())
         if bucket is None:
-            return None, dwte.to(wte.dtype), dwpe, None
-        if dwte is not bucket:
-            if bucket.dtype != torch.bfloat16 or not bucket.is_contiguous() or ptr(bucket) % 16:
-                bucket.add_(dwte) if accumulate else bucket.copy_(dwte)      # any type, order and start
-            elif accumulate:
-                call("mb_add_f32_to_bf16", ptr(dwte), ptr(bucket), dwte.numel(), stream())
-            else:
-                cast_to_bf16(dwte, bucket)
+            return None, dwte, dwpe, None, None, None
+        if not direct:
+            bucket.add_(dwte) if accumulate else bucket.copy_(dwte)      # any type, order and start
         ctx.param.grad_accumulate = True
-        return None, None, dwpe, None
+        return None, None, dwpe, None, None, None
 
 
-def embedding(ids, wte, wpe=None, vocab_start: int = 0):
-    """``wte[ids - vocab_start]`` (zero outside this rank's slice) ``+ wpe[position]``."""
+def embedding(ids, wte, wpe=None, vocab_start: int = 0, scale: float = 1.0, position_ids=None):
+    """``scale * wte[ids - vocab_start]`` (zero outside this rank's slice) ``+ wpe[position]``.
+
+    ``ids``: ``[batch, seq]``; the position of a token is its place in its row, or, with ``position_ids`` (integers
+    that broadcast to the shape of ``ids``), what stands there -- documents packed into one row start again at 0.
+    Positions outside ``wpe`` add nothing.  The sum is in fp32, rounded once.  The gradients of both tables are summed
+    over tokens sorted by row, in fp32 and always in the same order; the one of ``wte`` goes straight into its gradient
+    bucket where it has one."""
     if _sym(ids):
         return _rules().embedding(ids, wte, wpe, vocab_start)
-    return _EmbeddingFn.apply(ids, wte, wpe, int(vocab_start))
+    if _elsewhere(wte):
+        with torch.cuda.device(wte.device):
+            return embedding(ids, wte, wpe, vocab_start, scale, position_ids)
+    if ids.dim() != 2 or ids.is_floating_point():
+        raise ValueError(f"ids: [batch, seq] integers expected, got {tuple(ids.shape)} of {ids.dtype}")
+    if wpe is not None and position_ids is None and ids.shape[1] > wpe.shape[0]:
+        raise ValueError(f"{ids.shape[1]} positions, but the table has {wpe.shape[0]}")
+    pos = _flat_positions(position_ids, ids) if wpe is not None else None
+    if use_native(wte):
+        for name, t in (("wte", wte), ("wpe", wpe)):
+            if t is not None and (t.dtype != torch.bfloat16 or not t.is_contiguous() or t.shape[1] != wte.shape[1]
+                                  or t.shape[1] % 8 or t.device != ids.device):
+                raise ValueError(f"{name}: contiguous bf16 rows of a multiple of 8 values on the device of the ids expected")
+        ids = ids.long().contiguous()
+    return _EmbeddingFn.apply(ids, wte, wpe, int(vocab_start), float(scale), pos)
 
 
 # --------------------------------------------------------------------- optimizer / casts

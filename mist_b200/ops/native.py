@@ -55,12 +55,12 @@ _SIGNATURES = {
     "mb_bias_dropout_add": ([_p, _p, _p, _p, _z, _i, _f, _u64, _p], _i),
     "mb_dropout_bwd": ([_p, _p, _z, _f, _u64, _p], _i),
     "mb_rope": ([_p, _p, _p, _z, _i, _i, _i, _i, _i, _i, _i, _p], _i),
-    "mb_embedding_fwd": ([_p, _p, _p, _p, _z, _i, _i, _i, _i, _p], _i),
-    "mb_embedding_bwd": ([_p, _p, _p, _p, _i, _i, _i, _i, _i, _p], _i),
+    "mb_embed_fwd": ([_p, _p, _p, _p, _p, _i, _i, _i, _l, _i, _i, _f, _p], _i),
+    "mb_embed_bwd_workspace": ([_i, _i, _i], _z),
+    "mb_embed_bwd": ([_p, _p, _p, _p, _p, _i, _i, _i, _l, _i, _i, _f, _i, _i, _p, _p], _i),
     "mb_colsum": ([_p, _p, _p, _i, _i, _i, _i, _p], _i),
     "mb_cast_f32_to_bf16": ([_p, _p, _z, _f, _p], _i),
     "mb_axpy_bf16_to_f32": ([_p, _p, _z, _f, _i, _p], _i),
-    "mb_add_f32_to_bf16": ([_p, _p, _z, _p], _i),
     "mb_add_bf16": ([_p, _p, _z, _p], _i),
     "mb_xent_stats": ([_p, _p, _p, _i, _i, _i, _i, _p], _i),
     "mb_xent_loss": ([_p, _p, _p, _p, _i, _i, _p], _i),
