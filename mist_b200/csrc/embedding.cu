@@ -18,18 +18,15 @@ namespace cg = cooperative_groups;
 namespace {
 
 // ------------------------------------------------------------------------------------------------ lookup
-constexpr int kSlice = 128;      // vectors of 8 values that a warp copies: four loads in flight per lane
-
-// One warp per token and slice of its row. 
-__global__ void __launch_bounds__(256)
+// One warp per token and slice of its row, `per_warp` vectors of 8 values, four rounds of loads in flight per lane.
+__global__ void __launch_bounds__(256, 6)
 embed_fwd_kernel(const int64_t* __restrict__ ids, const int64_t* __restrict__ pos, const __nv_bfloat16* __restrict__ wte,
                  const __nv_bfloat16* __restrict__ wpe, __nv_bfloat16* __restrict__ out, int tokens, int seq, int h, int64_t v0,
-                 int rows, int positions, float scale, int slices) {
+                 int rows, int positions, float scale, int per_warp) {
   const int lane = threadIdx.x & 31;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int64_t t = item / slices;
+  const int t = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (t >= tokens) return;
-  const int vpr = h >> 3, first = static_cast<int>(item - t * slices) * kSlice + lane;
+  const int vpr = h >> 3, from = blockIdx.y * per_warp, to = min(vpr, from + per_warp);
   const int64_t row = ids[t] - v0;
   const bool in = row >= 0 && row < rows;
   int64_t p = -1;
@@ -39,25 +36,31 @@ embed_fwd_kernel(const int64_t* __restrict__ ids, const int64_t* __restrict__ po
   }
   const mb::bf16x8* we = reinterpret_cast<const mb::bf16x8*>(wte + (in ? row : 0) * h);
   const mb::bf16x8* pe = reinterpret_cast<const mb::bf16x8*>(wpe + (p >= 0 ? p : 0) * h);
-  mb::bf16x8 zero;
-  memset(&zero, 0, sizeof(zero));
-  mb::bf16x8 a[4], b[4];
+  mb::bf16x8* dst = reinterpret_cast<mb::bf16x8*>(out + static_cast<int64_t>(t) * h);
+  for (int c0 = from + lane; c0 < to; c0 += 128) {
+    mb::bf16x8 a[4];
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int c = first + 32 * u;
-    a[u] = (in && c < vpr) ? we[c] : zero;
-    b[u] = (p >= 0 && c < vpr) ? pe[c] : zero;
-  }
+    for (int u = 0; u < 4; ++u) {
+      memset(&a[u], 0, sizeof(a[u]));
+      if (in && c0 + 32 * u < to) a[u] = we[c0 + 32 * u];
+    }
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int c = first + 32 * u;
-    if (c >= vpr) break;
-    float f[8], g[8];
-    mb::unpack8(a[u], f);
-    mb::unpack8(b[u], g);
+    for (int u = 0; u < 4; ++u) {
+      const int c = c0 + 32 * u;
+      if (c >= to) break;
+      float f[8];
+      mb::unpack8(a[u], f);
+      if (p >= 0) {
+        float g[8];
+        mb::unpack8(pe[c], g);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = in ? (p >= 0 ? fmaf(f[k], scale, g[k]) : f[k] * scale) : g[k];
-    reinterpret_cast<mb::bf16x8*>(out + t * h)[c] = mb::pack8(f);
+        for (int k = 0; k < 8; ++k) f[k] = in ? fmaf(f[k], scale, g[k]) : g[k];
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] = in ? f[k] * scale : 0.f;
+      }
+      dst[c] = mb::pack8(f);
+    }
   }
 }
 
@@ -84,15 +87,17 @@ struct Sort {
 
 constexpr int kSortThreads = 1024;
 constexpr int kSortCluster = 8;
+constexpr int kHeld = 4;         // tokens that a lane keeps in registers over a pass
 
 // One cluster (or, for few tokens, one CTA) sorts one table's tokens, 8 bits of the key a pass.  A warp owns a stretch
 // of consecutive tokens; __match_any_sync ranks equal digits inside 32 of them, a histogram per warp counts those before.
 // The CTAs exchange their digit counts through distributed shared memory.  Latency is what it costs: about 2 us a pass
 //.
+template <bool HELD>
 __global__ void __launch_bounds__(kSortThreads)
-embed_sort_kernel(const Sort s0, const Sort s1, int tokens, int counters) {
+embed_sort_kernel(const __grid_constant__ Sort s0, const __grid_constant__ Sort s1, int tokens, int counters) {
   __shared__ int hist[32][256];
-  __shared__ int totals[256], base[256], warp_part[8];
+  __shared__ int totals[256], base[256], warp_part[8], quarter[4][256];
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
   const Sort& s = (blockIdx.x / ctas) ? s1 : s0;
@@ -111,32 +116,54 @@ embed_sort_kernel(const Sort s0, const Sort s1, int tokens, int counters) {
     const int shift = 8 * pass;
     const uint32_t* src_key = s.area.key[(pass + 1) & 1];
     const int* src_tok = s.area.tok[(pass + 1) & 1];
+    uint32_t* dst_key = s.area.key[pass & 1];
+    int* dst_tok = s.area.tok[pass & 1];
     auto key_at = [&](int i) -> uint32_t {
       if (pass > 0) return __ldcg(src_key + i);
       const int64_t r = s.ids[i] - s.v0;
       return (r >= 0 && r < s.rows) ? static_cast<uint32_t>(r) : static_cast<uint32_t>(s.rows);
     };
+    uint32_t key[kHeld];
+    int tok[kHeld];
+    if (HELD) {
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u) {
+        const int i = begin + 32 * u + lane;
+        if (i < end) {
+          key[u] = key_at(i);
+          tok[u] = pass > 0 ? __ldcg(src_tok + i) : i;
+        }
+      }
+    }
 #pragma unroll
     for (int d = lane; d < 256; d += 32) hist[warp][d] = 0;
     __syncwarp();
-    for (int i0 = begin; i0 < end; i0 += 32) {
-      const int i = i0 + lane;
-      const unsigned digit = i < end ? (key_at(i) >> shift) & 255u : 256u;
+    auto count = [&](int i, uint32_t k) {
+      const unsigned digit = i < end ? (k >> shift) & 255u : 256u;
       const unsigned same = __match_any_sync(0xffffffffu, digit);
       if (digit < 256 && (same & below) == 0) hist[warp][digit] += __popc(same);
       __syncwarp();
+    };
+    if (HELD) {
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u)
+        if (begin + 32 * u < end) count(begin + 32 * u + lane, key[u]);
+    } else {
+      for (int i = begin + lane; i - lane < end; i += 32) count(i, i < end ? key_at(i) : 0u);
     }
     __syncthreads();
-    if (tid < 256) {
-      int sum = 0;
+    // exclusive sum of a digit over the warps, a quarter of them per thread
+    int* column = &hist[8 * (tid >> 8)][tid & 255];
+    int sum = 0;
 #pragma unroll
-      for (int w = 0; w < 32; ++w) {
-        const int n = hist[w][tid];
-        hist[w][tid] = sum;
-        sum += n;
-      }
-      totals[tid] = sum;
+    for (int w = 0; w < 8; ++w) {
+      const int n = column[256 * w];
+      column[256 * w] = sum;
+      sum += n;
     }
+    quarter[tid >> 8][tid & 255] = sum;
+    __syncthreads();
+    if (tid < 256) totals[tid] = quarter[0][tid] + quarter[1][tid] + quarter[2][tid] + quarter[3][tid];
     cluster.sync();
     int before = 0, all = 0;
     if (tid < 256) {
@@ -161,21 +188,26 @@ embed_sort_kernel(const Sort s0, const Sort s1, int tokens, int counters) {
       base[tid] = start + before;
     }
     __syncthreads();
-    uint32_t* dst_key = s.area.key[pass & 1];
-    int* dst_tok = s.area.tok[pass & 1];
-    for (int i0 = begin; i0 < end; i0 += 32) {
-      const int i = i0 + lane;
-      const uint32_t key = i < end ? key_at(i) : 0u;
-      const unsigned digit = i < end ? (key >> shift) & 255u : 256u;
+    auto place = [&](int i, uint32_t k, int t) {
+      const unsigned digit = i < end ? (k >> shift) & 255u : 256u;
       const unsigned same = __match_any_sync(0xffffffffu, digit);
       if (digit < 256) {
-        const int at = base[digit] + hist[warp][digit] + __popc(same & below);
-        dst_key[at] = key;
-        dst_tok[at] = pass > 0 ? __ldcg(src_tok + i) : i;
+        int at = base[digit] + hist[warp][digit] + __popc(same & below);
+        for (int q = 0; q < (warp >> 3); ++q) at += quarter[q][digit];
+        dst_key[at] = k;
+        dst_tok[at] = t;
       }
       __syncwarp();
       if (digit < 256 && (same & below) == 0) hist[warp][digit] += __popc(same);
       __syncwarp();
+    };
+    if (HELD) {
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u)
+        if (begin + 32 * u < end) place(begin + 32 * u + lane, key[u], tok[u]);
+    } else {
+      for (int i = begin + lane; i - lane < end; i += 32)
+        place(i, i < end ? key_at(i) : 0u, (pass > 0 && i < end) ? __ldcg(src_tok + i) : i);
     }
     cluster.sync();      // the next pass reads what other CTAs wrote; nobody reads totals any more
   }
@@ -377,8 +409,8 @@ __device__ void sum_long(const Table& t, const __nv_bfloat16* dout, int tokens, 
 }
 
 // blocks: [long rows of table 0][of table 1][rows of table 0][of table 1]
-__global__ void __launch_bounds__(kSumThreads)
-embed_sum_kernel(const Table t0, const Table t1, const __nv_bfloat16* dout, int tokens, int h, int long0, int long1,
+__global__ void __launch_bounds__(kSumThreads, 6)
+embed_sum_kernel(const __grid_constant__ Table t0, const __grid_constant__ Table t1, const __nv_bfloat16* dout, int tokens, int h, int long0, int long1,
                  int rows0, int slices) {
   mb::wait_for_previous_kernel();
   int b = blockIdx.x;
@@ -447,12 +479,11 @@ MB_API int mb_embed_fwd(const int64_t* ids, const int64_t* pos, const void* wte,
   if (tokens < 0 || h <= 0 || h % 8 || rows < 0 || (wpe && !pos && seq <= 0)) return -1;
   if (!aligned16(wte) || !aligned16(wpe) || !aligned16(out)) return -1;
   if (tokens == 0) return 0;
-  const int slices = (h / 8 + kSlice - 1) / kSlice;
-  const int64_t items = static_cast<int64_t>(tokens) * slices;
-  if (items > (1ll << 33)) return -1;
-  embed_fwd_kernel<<<static_cast<unsigned>((items + 7) / 8), 256, 0, stream>>>(
+  // whole rows once they fill the chip (48 warps on each of 148 SMs); before that a row is cut into slices of 128 vectors
+  const int per_warp = tokens >= 7104 ? h / 8 : 128;
+  embed_fwd_kernel<<<dim3((tokens + 7) / 8, (h / 8 + per_warp - 1) / per_warp), 256, 0, stream>>>(
       ids, pos, static_cast<const __nv_bfloat16*>(wte), static_cast<const __nv_bfloat16*>(wpe),
-      static_cast<__nv_bfloat16*>(out), tokens, seq, h, v0, rows, positions, scale, slices);
+      static_cast<__nv_bfloat16*>(out), tokens, seq, h, v0, rows, positions, scale, per_warp);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
@@ -505,7 +536,8 @@ MB_API int mb_embed_bwd(const int64_t* ids, const int64_t* pos, const void* dout
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, embed_sort_kernel, s[0], s[1], tokens, 2 * tiles * slices) != cudaSuccess) return -4;
+    const bool held = tokens <= ctas * kSortThreads * kHeld;
+    if (cudaLaunchKernelEx(&cfg, held ? embed_sort_kernel<true> : embed_sort_kernel<false>, s[0], s[1], tokens, 2 * tiles * slices) != cudaSuccess) return -4;
   }
   const long rows0 = sort0 ? (rows + kRows - 1) / kRows : 0, rows1 = dwpe ? (positions + kRows - 1) / kRows : 0;
   const long long0 = sort0 ? static_cast<long>(tiles) * slices : 0, long1 = sort1 ? static_cast<long>(tiles) * slices : 0;

@@ -70,15 +70,74 @@ __device__ __forceinline__ void report(int* status, int code) {
 
 // What a kernel's epilogue does beside the common part.  The split form is a kernel of its own: its second source of the
 // products cost the others 4 - 9 % where the epilogue is the bound (13760 x 6664 x 128: 81.7 us against 87.4).
-enum Kind : int { kPlain = 0, kAux = 1, kSplit = 2 };
+enum Kind : int { kPlain = 0, kAux = 1, kSplit = 2, kXentStats = 3, kXentGrad = 4 };
+
+// Vocabulary projection with cross entropy: C, the logits, is never stored.  A struct of its own, because a parameter
+// more changes the code of the other kinds (registers of the split one 238 -> 164).
+struct XentParams : PairParams {
+  const int64_t* labels;      // [M]; the label's column is labels[m] - v0
+  int64_t v0, ignore;
+  int segments;               // parts of K whose sums are added in registers
+  float2* stats;              // kXentStats: [column tile][M] {maximum * log2(e), sum of 2^(x * log2(e) - that)}
+  float* target;              // kXentStats: [M], written where the label's column is among these
+  const float *lse, *gloss;   // kXentGrad: [M]
+  float* col_sums;            // kXentGrad: [32 rows][N], column sums of what is stored, or null
+};
+template <int KIND> struct ParamsOf { using type = PairParams; };
+template <> struct ParamsOf<kXentStats> { using type = XentParams; };
+template <> struct ParamsOf<kXentGrad> { using type = XentParams; };
+
+// The bias of N columns, what the sums of their logits start from.
+template <int N>
+__device__ __forceinline__ void xent_start(const XentParams& p, float* v, int col0) {
+  if (!(p.flags & EPI_BIAS)) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = 0.f;
+  } else if (col0 + N <= p.N && (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 8) mb::unpack8(*reinterpret_cast<const mb::bf16x8*>(p.bias + col0 + i), v + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __bfloat162float(p.bias[min(col0 + i, p.N - 1)]);
+  }
+}
+
+// Statistics of the logits of one row over half a tile.  The maximum is kept in units of log2(e),
+// so that an exponential is one FFMA and one ex2: 128 of them per thread, 2048 cycles of the special-function units per
+// tile, against 8 cycles per unit of K of the products.
+__device__ __forceinline__ float2 xent_row_stats(const XentParams& p, float* v, int col0, int lab, float& target) {
+  constexpr float kLog2e = 1.4426950408889634f;
+  if (col0 + 128 > p.N) {
+#pragma unroll
+    for (int i = 0; i < 128; ++i) v[i] = col0 + i < p.N ? v[i] : -INFINITY;
+  }
+  if (lab >= 0) {
+#pragma unroll
+    for (int i = 0; i < 128; ++i) target = lab == i ? v[i] : target;
+  }
+  float mx[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+  for (int i = 4; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
+  const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kLog2e;
+  const float m_use = m == -INFINITY ? 0.f : m;       // nothing but -inf: the exponentials are 0
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 128; ++i) s[i & 3] += mb::fast_exp2(fmaf(v[i], kLog2e, -m_use));
+  return make_float2(m, (s[0] + s[1]) + (s[2] + s[3]));
+}
+
+// Threads of a kind's CTA: the epilogues of cross entropy have two warps for each 32 rows.
+__host__ __device__ constexpr bool is_xent(int kind) { return kind == kXentStats || kind == kXentGrad; }
+__host__ __device__ constexpr int threads_of(int kind) { return is_xent(kind) ? 320 : kThreads; }
+__host__ __device__ constexpr int staged_tiles(int kind) { return kind == kAux || kind == kXentGrad ? 4 : 2; }
 
 template <bool A_MN, bool B_MN, int KIND>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(threads_of(KIND), 1)
 gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                  const __grid_constant__ CUtensorMap tma_c, const __grid_constant__ CUtensorMap tma_aux,
-                 const PairParams p) {
-  constexpr bool AUX = KIND == kAux, SPLIT = KIND == kSplit;
-  using L = Layout<AUX>;
+                 const typename ParamsOf<KIND>::type p) {
+  constexpr bool AUX = KIND == kAux, SPLIT = KIND == kSplit, XENT = is_xent(KIND), STATS = KIND == kXentStats;
+  using L = Layout<staged_tiles(KIND) == 4>;
   constexpr int STAGES = L::kStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // Both CTAs of the pair must use the same offsets: the dynamic segment starts at the same
@@ -103,7 +162,9 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
   const int num_n = (p.N + BN - 1) / BN;
   const int num_kb = (p.K + BK - 1) / BK;
   const int full_tiles = num_m * num_n - (SPLIT ? p.tail_tiles : 0);
-  const int num_items = full_tiles + (SPLIT ? p.tail_tiles * p.splits : 0);
+  int num_items = full_tiles + (SPLIT ? p.tail_tiles * p.splits : 0);
+  if constexpr (XENT)       // a pair's tiles, each as many items in a row as K has segments
+    num_items = pair + num_pairs * p.segments * ((full_tiles - pair + num_pairs - 1) / num_pairs);
   constexpr int GM = 4;  // 256-row tiles per raster group: neighbours share B panels in L2
 
   auto tile_coords = [&](int t, int& m0, int& n0) {
@@ -122,6 +183,12 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
     kb0 = 0;
     kb1 = num_kb;
     split = -1;
+    if constexpr (XENT) {
+      const int q = (w - pair) / num_pairs, seg = q % p.segments;
+      t = pair + q / p.segments * num_pairs;
+      kb0 = seg * num_kb / p.segments;
+      kb1 = (seg + 1) * num_kb / p.segments;
+    }
     if (SPLIT && w >= full_tiles) {
       const int u = w - full_tiles;
       split = u / p.tail_tiles;
@@ -138,7 +205,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull_bar[a], 1);   // one MMA commit, broadcast to both CTAs
-      mbar_init(&tempty_bar[a], 8);  // leader's: 4 epilogue warps of each CTA
+      mbar_init(&tempty_bar[a], XENT ? 16 : 8);  // leader's: the epilogue warps of both CTAs, 4 (8) each
       mbar_init(&aux_full[a], 1);    // second epilogue operand staged by TMA (AUX kernels)
     }
     fence_barrier_init();
@@ -248,6 +315,127 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
         __syncwarp();
       }
     }
+  } else if constexpr (XENT) {
+    // --------------------------------------------- cross entropy of the logits (both CTAs)
+    // Two warps for 32 rows, 128 columns each.  A tensor-core sum truncates, which makes logits of a long K too small by
+    // some 2^-24 of themselves per 16 products (hidden size 4096: a loss 1.5e-6 off); so for the statistics K is cut into
+    // segments of 1024 at most, whose sums are added here.  The accumulator goes back before the exponentials.
+    const int q = warp & 3, half = (warp - 2) >> 2, r = q * 32 + lane;
+    const bool leader = (warp & 3) == 2 && lane == 0;                        // of this half's 128 threads
+    float2* meet = reinterpret_cast<float2*>(smem + L::kStagingOffset);      // [parity of the tile][row]
+    uint32_t count = 0, stored = 0;
+    int parity = 0;
+    bool ok = true;
+    auto wait_sum = [&](uint32_t n) -> bool {
+      if (mbar_wait(&tfull_bar[n & 1], (n >> 1) & 1)) return true;
+      report(p.status, MB_ERR_TIMEOUT_TMEM);
+      return false;
+    };
+    auto add32 = [&](float* v, uint32_t n, int c) {      // columns c ... of this half
+      uint32_t rr[32];
+      tmem_ld32(tmem_base + (n & 1) * BN + half * 128 + c + (static_cast<uint32_t>(q * 32) << 16), rr);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] += __uint_as_float(rr[i]);
+    };
+    auto give_back = [&](uint32_t n) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tempty_bar[n & 1]), 0));
+    };
+    auto label_at = [&](bool live, int row, int col, int width) -> int {      // the label's place among these, or -1
+      if (!live) return -1;
+      const int64_t at = p.labels[row] - p.v0 - col;
+      return at >= 0 && at < min(width, p.N - col) ? static_cast<int>(at) : -1;
+    };
+    for (int t = pair; t < full_tiles && ok; t += num_pairs, parity ^= 1) {
+      int m0, n0;
+      tile_coords(t, m0, n0);
+      const int row = m0 + r, col0 = n0 + half * 128;
+      const bool live = row < p.M;
+      if constexpr (STATS) {
+        float v[128];
+        xent_start<128>(p, v, col0);
+#pragma unroll 1
+        for (int seg = 0; seg < p.segments && ok; ++seg, ++count) {
+          ok = wait_sum(count);
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < 128; c += 32) add32(v + c, count, c);
+          give_back(count);
+        }
+        if (!ok || m0 >= p.M) continue;
+        const int lab = label_at(live, row, col0, 128);
+        float target = 0.f;
+        float2 mine = xent_row_stats(p, v, col0, lab, target);
+        if (half) meet[parity * BM + r] = mine;
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
+        if (!half) {
+          const float2 other = meet[parity * BM + r];
+          const float m = fmaxf(mine.x, other.x), use = m == -INFINITY ? 0.f : m;
+          mine = make_float2(m, mine.y * mb::fast_exp2(mine.x - use) + other.y * mb::fast_exp2(other.x - use));
+          if (live) p.stats[static_cast<size_t>(n0 / BN) * p.M + row] = mine;
+        }
+        if (lab >= 0) p.target[row] = target;
+      } else {
+        // (softmax - [label]) * gradient of the loss, 0 in an ignored row; 64 columns at a time through staging
+        const bool skipped = !live || p.labels[row] == p.ignore;
+        const float lse2 = live ? p.lse[row] * 1.4426950408889634f : 0.f, gloss = live ? p.gloss[row] : 0.f;
+        ok = wait_sum(count);
+        tc_fence_after();
+#pragma unroll 1
+        for (int u = 0; u < 2 && ok; ++u) {
+          const int ucol0 = col0 + 64 * u;
+          float v[64];
+          xent_start<64>(p, v, ucol0);
+          add32(v, count, 64 * u);
+          add32(v + 32, count, 64 * u + 32);
+          if (u == 1) give_back(count);
+          if (m0 >= p.M || ucol0 >= p.N) continue;
+#pragma unroll
+          for (int i = 0; i < 64; ++i) v[i] = mb::fast_exp2(fmaf(v[i], 1.4426950408889634f, -lse2));
+          const int lab = label_at(live, row, ucol0, 64);
+          if (lab >= 0) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) v[i] = i == lab ? v[i] - 1.f : v[i];
+          }
+          uint8_t* stg = smem + L::kStagingOffset + (2 * half + (stored & 1)) * L::kStagingBytes;
+          if (leader) tma_wait_read<1>();
+          asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = skipped ? 0.f : v[8 * g + i] * gloss;
+            *reinterpret_cast<mb::bf16x8*>(stg + r * 128 + ((g ^ (r & 7)) << 4)) = mb::pack8(f);
+          }
+          if (p.col_sums && m0 + q * 32 < p.M) {
+            // column sums of what is stored (the bias' gradient): a lane adds two columns of its warp's 32 rows
+            __syncwarp();
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll 8
+            for (int i = 0; i < 32; ++i) {
+              const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(
+                  stg + (q * 32 + i) * 128 + (((lane >> 2) ^ (i & 7)) << 4) + (lane & 3) * 4));
+              s0 += x.x;
+              s1 += x.y;
+            }
+            float* dst = p.col_sums + static_cast<size_t>((m0 >> 5) + q) * p.N + ucol0 + 2 * lane;
+            if (ucol0 + 2 * lane < p.N) dst[0] = s0;
+            if (ucol0 + 2 * lane + 1 < p.N) dst[1] = s1;
+          }
+          fence_async_smem();
+          asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+          if (leader) {
+            tma_store_2d(&tma_c, stg, ucol0, m0);
+            tma_commit();
+          }
+          ++stored;
+        }
+        ++count;
+      }
+    }
+    if (leader) tma_wait_all<0>();
   } else {
     // ----------------------------------------------------------- epilogue (both CTAs)
     const int q = warp & 3;
@@ -500,8 +688,8 @@ size_t arrived_bytes(const Split& s) { return (static_cast<size_t>(s.tail_tiles)
 
 template <bool A_MN, bool B_MN, int KIND>
 int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const CUtensorMap& tx,
-           const PairParams& p, int max_ctas, cudaStream_t stream) {
-  constexpr int smem = Layout<KIND == kAux>::kTotal + 1024;
+           const typename ParamsOf<KIND>::type& p, int max_ctas, cudaStream_t stream) {
+  constexpr int smem = Layout<staged_tiles(KIND) == 4>::kTotal + 1024;
   static bool configured = false;
   auto kern = gemm_pair_kernel<A_MN, B_MN, KIND>;
   if (!configured) {
@@ -515,7 +703,7 @@ int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, 
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(2 * pairs, 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.blockDim = dim3(threads_of(KIND), 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -614,6 +802,217 @@ MB_API int mb_gemm_pair_split_bf16(const void* A, const void* B, void* C, int M,
   if (has_aux) return dispatch<kAux>(a_mn_major != 0, b_mn_major != 0, ta, tb, tc, tx, p, max_ctas, stream);
   if (split.tail_tiles) return dispatch<kSplit>(a_mn_major != 0, b_mn_major != 0, ta, tb, tc, tx, p, max_ctas, stream);
   return dispatch<kPlain>(a_mn_major != 0, b_mn_major != 0, ta, tb, tc, tx, p, max_ctas, stream);
+}
+
+namespace {
+
+// One thread adds a sixteenth of a row's tiles; a block takes 32 rows.
+__global__ void __launch_bounds__(512)
+xent_combine_kernel(const float2* __restrict__ stats, const float* __restrict__ target, const int64_t* __restrict__ labels,
+                    float* __restrict__ loss, float* __restrict__ lse, float* __restrict__ out_stats, int rows, int tiles,
+                    int cols, int64_t v0, int64_t ignore) {
+  __shared__ float2 part[16][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
+  float m = -INFINITY, s = 0.f;
+  auto add = [&](float2 x) {
+    const float n = fmaxf(m, x.x), use = n == -INFINITY ? 0.f : n;
+    s = s * exp2f(m - use) + x.y * exp2f(x.x - use);
+    m = n;
+  };
+  if (row < rows) {
+    for (int t = w; t < tiles; t += 128) {
+      float2 x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        x[u] = t + 16 * u < tiles ? stats[static_cast<size_t>(t + 16 * u) * rows + row] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) add(x[u]);
+    }
+  }
+  part[w][lane] = make_float2(m, s);
+  __syncthreads();
+  if (w || row >= rows) return;
+  for (int k = 1; k < 16; ++k) add(part[k][lane]);
+  const int64_t lab = labels[row], at = lab - v0;
+  const float hit = (at >= 0 && at < cols) ? target[row] : 0.f;
+  constexpr double kLn2 = 0.6931471805599453;
+  if (out_stats) {
+    out_stats[3l * row] = static_cast<float>(m * kLn2);
+    out_stats[3l * row + 1] = s;
+    out_stats[3l * row + 2] = hit;
+  } else {
+    const float l = static_cast<float>((static_cast<double>(m) + log2f(s)) * kLn2);
+    lse[row] = l;
+    loss[row] = lab == ignore ? 0.f : l - hit;
+  }
+}
+
+// Sum over the groups of 32 rows, in a fixed order; a block takes 32 columns.
+__global__ void __launch_bounds__(256)
+xent_bias_grad_kernel(const float* __restrict__ sums, void* __restrict__ out, int groups, int cols, int fp32) {
+  __shared__ float part[8][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  float a = 0.f;
+  if (c < cols) {
+#pragma unroll 8
+    for (int g = w; g < groups; g += 8) a += sums[static_cast<size_t>(g) * cols + c];
+  }
+  part[w][lane] = a;
+  __syncthreads();
+  if (w || c >= cols) return;
+  for (int k = 1; k < 8; ++k) a += part[k][lane];
+  if (fp32) static_cast<float*>(out)[c] = a;
+  else static_cast<__nv_bfloat16*>(out)[c] = __float2bfloat16(a);
+}
+
+// Both operands K-major, the vocabulary on the B side; no rule on the number of tiles: there is one kernel for all sizes.
+int xent_gemm(const void* x, const void* w, void* dlogits, int ldd, XentParams& p, int ldx, int ldw, int max_ctas,
+              cudaStream_t stream) {
+  CUtensorMap ta, tb, tc, tx;
+  memset(&tc, 0, sizeof(tc));
+  memset(&tx, 0, sizeof(tx));
+  if (!make_map(&ta, x, p.M, p.K, ldx, 64, BM, false, true)) return -21;
+  if (!make_map(&tb, w, p.N, p.K, ldw, 64, BNH, false, true)) return -22;
+  if (dlogits && !make_map(&tc, dlogits, p.M, p.N, ldd, 64, BM, false, false)) return -23;
+  p.alpha = 1.f;
+  p.status = mb_status_device_ptr();
+  p.splits = 1;
+  max_ctas = clamp_ctas(max_ctas);
+  return dlogits ? launch<false, false, kXentGrad>(ta, tb, tc, tx, p, max_ctas, stream)
+                 : launch<false, false, kXentStats>(ta, tb, tc, tx, p, max_ctas, stream);
+}
+
+bool xent_args_ok(const void* x, const void* w, int M, int V, int K, int ldx, int ldw) {
+  return M >= 0 && V > 0 && K > 0 && !((K | ldx | ldw) & 7) && ldx >= K && ldw >= K &&
+         !((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15);
+}
+
+size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+// Work area of the backward pass: gradient of a piece's logits, its column sums, dx in fp32 (several pieces), and what
+// the products split (the largest of them; calls follow one another on the stream).
+struct XentArea {
+  size_t dlogits, col_sums, dx32, gemm, total;
+};
+XentArea xent_area(int M, int V, int K, int piece, bool want_x, bool want_w, bool want_b, int dw_flags, int max_ctas) {
+  XentArea a;
+  const size_t wide = (static_cast<size_t>(piece) + 7) / 8 * 8;
+  const bool many = piece < V;
+  a.dlogits = up256(2 * wide * M);
+  a.col_sums = want_b ? up256(4ul * piece * ((M + 31) / 32)) : 0;
+  a.dx32 = want_x && many ? up256(4ul * M * K) : 0;
+  a.gemm = 0;
+  auto need = [&](int m, int n, int k, int flags) {
+    const size_t b = mb_gemm_pair_workspace(m, n, k, flags, max_ctas);
+    if (b > a.gemm) a.gemm = b;
+  };
+  for (int n : {piece, V % piece ? V % piece : piece}) {
+    if (want_x) need(M, K, n, many ? EPI_OUT_FP32 : 0);
+    if (want_w) need(n, K, M, dw_flags);
+  }
+  a.total = a.dlogits + a.col_sums + a.dx32 + up256(a.gemm);
+  return a;
+}
+
+}  // namespace
+
+MB_API int mb_gemm_bf16(const void* A, const void* B, void* C, int M, int N, int K, int lda, int ldb, int ldc, int a_mn_major,
+                        int b_mn_major, int flags, const void* bias, void* aux, float alpha, int tile_n, int max_ctas,
+                        cudaStream_t stream);
+MB_API int mb_cast_f32_to_bf16(const float* in, void* out, size_t n, float scale, cudaStream_t s);
+
+// Tiles of the vocabulary that mb_xent_linear_fwd keeps statistics of.
+MB_API int mb_xent_linear_tiles(int V) { return (V + BN - 1) / BN; }
+
+// Cross entropy of logits = x [M,K] * w [V,K]^T + bias, which are not stored.  stats: [tiles][M][2] fp32 and target: [M]
+// fp32, workspaces of this call.  out_stats null: loss [M] (0 where the label is `ignore`) and lse [M], natural logarithms;
+// a label outside [v0, v0 + V) has the logit 0.  out_stats [M][3]: {maximum, sum of exponentials relative to it, label's
+// logit (0 outside)} instead, which a group of vocabulary slices combines.  K and the leading dimensions multiples of 8.
+MB_API int mb_xent_linear_fwd(const void* x, const void* w, const void* bias, const int64_t* labels, float* stats,
+                              float* target, float* loss, float* lse, float* out_stats, int M, int V, int K, int ldx,
+                              int ldw, int64_t v0, int64_t ignore, int max_ctas, cudaStream_t stream) {
+  if (!xent_args_ok(x, w, M, V, K, ldx, ldw)) return -1;
+  if (M == 0) return 0;
+  XentParams p;
+  memset(&p, 0, sizeof(p));
+  p.M = M; p.N = V; p.K = K;
+  p.bias = reinterpret_cast<const __nv_bfloat16*>(bias);
+  p.flags = bias ? EPI_BIAS : 0;
+  p.labels = labels;
+  p.v0 = v0;
+  p.segments = (K + 1023) / 1024;
+  p.stats = reinterpret_cast<float2*>(stats);
+  p.target = target;
+  const int rc = xent_gemm(x, w, nullptr, 0, p, ldx, ldw, max_ctas, stream);
+  if (rc != 0) return rc;
+  xent_combine_kernel<<<(M + 31) / 32, 512, 0, stream>>>(p.stats, target, labels, loss, lse, out_stats, M,
+                                                         mb_xent_linear_tiles(V), V, v0, ignore);
+  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+}
+
+// Bytes of workspace of mb_xent_linear_bwd, which holds the gradient of `piece` columns of logits at a time.
+MB_API size_t mb_xent_linear_bwd_workspace(int M, int V, int K, int piece, int want_x, int want_w, int want_b, int dw_fp32,
+                                           int accumulate, int max_ctas) {
+  if (M <= 0 || V <= 0 || K <= 0 || piece <= 0) return 0;
+  return xent_area(M, V, K, piece < V ? piece : V, want_x, want_w, want_b,
+                   (dw_fp32 ? EPI_OUT_FP32 : 0) | (accumulate ? EPI_ACCUM : 0), clamp_ctas(max_ctas)).total;
+}
+
+// Gradients of the loss, gloss [M] being what it is differentiated by: with d[t,v] = (exp(logit - lse) - [label]) * gloss
+// (rows whose label is `ignore`: 0), computed again piece by piece and rounded to bf16, dx [M][K] = d w (bf16), dw [V][K]
+// (+)= d^T x (bf16 or fp32, row stride lddw), dbias [V] = column sums of d (bf16 or fp32).  dx, dw and dbias may be null.
+// piece: a multiple of 256, or V.
+MB_API int mb_xent_linear_bwd(const void* x, const void* w, const void* bias, const int64_t* labels, const float* lse,
+                              const float* gloss, void* dx, void* dw, void* dbias, int M, int V, int K, int ldx, int ldw,
+                              int lddw, int dw_fp32, int accumulate, int dbias_fp32, int64_t v0, int64_t ignore, int piece,
+                              int max_ctas, void* workspace, cudaStream_t stream) {
+  if (!xent_args_ok(x, w, M, V, K, ldx, ldw) || M == 0 || piece <= 0) return -1;
+  if (piece >= V) piece = V;
+  else if (piece % 256) return -1;
+  if ((reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(workspace)) & 15) return -1;
+  const int dw_flags = (dw_fp32 ? EPI_OUT_FP32 : 0) | (accumulate ? EPI_ACCUM : 0);
+  const XentArea area = xent_area(M, V, K, piece, dx, dw, dbias, dw_flags, clamp_ctas(max_ctas));
+  uint8_t* at = static_cast<uint8_t*>(workspace);
+  void* dl = at;
+  float* sums = dbias ? reinterpret_cast<float*>(at + area.dlogits) : nullptr;
+  float* dx32 = reinterpret_cast<float*>(at + area.dlogits + area.col_sums);
+  void* gemm_area = area.gemm ? at + area.dlogits + area.col_sums + area.dx32 : nullptr;
+  auto gemm = [&](const void* a, const void* b, void* c, int m, int n, int k, int lda, int ldb, int ldc, int a_mn, int flags) {
+    const int rc = mb_gemm_pair_split_bf16(a, b, c, m, n, k, lda, ldb, ldc, a_mn, 1, flags, nullptr, nullptr, 1.f, max_ctas,
+                                           gemm_area, stream);
+    return rc != 1 ? rc : mb_gemm_bf16(a, b, c, m, n, k, lda, ldb, ldc, a_mn, 1, flags, nullptr, nullptr, 1.f, 0, max_ctas,
+                                       stream);
+  };
+  for (int c0 = 0; c0 < V; c0 += piece) {
+    const int n = V - c0 < piece ? V - c0 : piece, ldd = (n + 7) / 8 * 8;
+    const __nv_bfloat16* wp = static_cast<const __nv_bfloat16*>(w) + static_cast<size_t>(c0) * ldw;
+    XentParams p;
+    memset(&p, 0, sizeof(p));
+    p.M = M; p.N = n; p.K = K;
+    p.bias = bias ? static_cast<const __nv_bfloat16*>(bias) + c0 : nullptr;
+    p.flags = bias ? EPI_BIAS : 0;
+    p.labels = labels;
+    p.v0 = v0 + c0;
+    p.ignore = ignore;
+    p.lse = lse;
+    p.gloss = gloss;
+    p.segments = 1;
+    p.col_sums = sums;
+    int rc = xent_gemm(x, wp, dl, ldd, p, ldx, ldw, max_ctas, stream);
+    if (rc == 0 && dbias) {
+      void* dst = static_cast<uint8_t*>(dbias) + static_cast<size_t>(c0) * (dbias_fp32 ? 4 : 2);
+      xent_bias_grad_kernel<<<(n + 31) / 32, 256, 0, stream>>>(sums, dst, (M + 31) / 32, n, dbias_fp32);
+      if (cudaGetLastError() != cudaSuccess) rc = -4;
+    }
+    if (rc == 0 && dx)
+      rc = piece == V ? gemm(dl, wp, dx, M, K, n, ldd, ldw, K, 0, 0)
+                      : gemm(dl, wp, dx32, M, K, n, ldd, ldw, K, 0, EPI_OUT_FP32 | (c0 ? EPI_ACCUM : 0));
+    if (rc == 0 && dw)
+      rc = gemm(dl, x, static_cast<uint8_t*>(dw) + static_cast<size_t>(c0) * lddw * (dw_fp32 ? 4 : 2), n, K, M, ldd, ldx, lddw,
+                1, dw_flags);
+    if (rc != 0) return rc;
+  }
+  return dx && piece < V ? mb_cast_f32_to_bf16(dx32, dx, static_cast<size_t>(M) * K, 1.f, stream) : 0;
 }
 
 MB_API int mb_gemm_pair_bf16(const void* A, const void* B, void* C, int M, int N, int K, int lda, int ldb, int ldc,

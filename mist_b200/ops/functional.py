@@ -53,6 +53,8 @@ class Settings:
     # softmax; MIST_B200_ATTN_BWD_PIPELINED=0 selects the one that finishes a 64-row query block before the next.
     attn_bwd_pipelined = os.environ.get("MIST_B200_ATTN_BWD_PIPELINED", "1") != "0"
     gemm_max_ctas = 0             # >0 leaves SMs free for a concurrent communication kernel
+    # bytes of the bf16 gradient of the logits that linear_cross_entropy's backward pass holds at a time
+    xent_piece_bytes = 256 << 20
     gemm_pair = True              # large GEMMs on CTA pairs (256 x 256 tiles, tcgen05 cta_group::2)
     fuse_mlp_gelu = True          # GELU MLP as one autograd node (gelu' folded into a dgrad GEMM epilogue)
     tp_backend = "nccl"           # "nccl" | "fused": sequence-parallel linears on the GEMM+collective kernels
@@ -1268,3 +1270,6 @@ def accumulate_grad(src_bf16, dst, scale: float = 1.0, accumulate: bool = True):
         assert scale == 1.0 and accumulate
         call("mb_add_bf16", ptr(src_bf16), ptr(dst), src_bf16.numel(), stream())
     return dst
+
+
+from .linear_xent import linear_cross_entropy  # noqa: E402,F401  (needs the functions above)

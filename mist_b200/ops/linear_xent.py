@@ -1,0 +1,169 @@
+"""Vocabulary projection and cross entropy as one operator that never holds the logits.
+
+``loss[t] = log sum_v exp(x_t . w_v + b_v) - (x_t . w_label + b_label)``.  The forward pass is one GEMM whose epilogue
+keeps a maximum and a sum per row and tile; it stores two numbers per row for the backward pass.  That computes the
+logits again, a piece of the vocabulary at a time, turns them into their gradient in the GEMM's epilogue and multiplies
+the piece into the gradients of ``x`` and of the weight (reference: the projection of mist/modules/fused_dense.py:221-327
+followed by mist/modules/losses.py:48-176, which hold ``[tokens, vocabulary]`` logits between the two).
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import functional as F
+from . import native
+from .native import call, ptr, stream, use_native
+
+
+def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """``t`` as ``[rows, cols]`` that the kernels' copies can address: unit stride, rows on 16 bytes."""
+    t = t.reshape(-1, cols)
+    if t.stride(1) != 1 or t.stride(0) % 8 or t.stride(0) < cols or ptr(t) % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def piece_columns(rows: int, vocab: int) -> int:
+    """Columns of the vocabulary whose gradient the backward pass holds at a time: as many multiples of 256 as
+    ``Settings.xent_piece_bytes`` allows, in pieces of equal size."""
+    most = max(256, F.Settings.xent_piece_bytes // (2 * max(rows, 1)) // 256 * 256)
+    pieces = -(-vocab // most)
+    return min(vocab, -(-(-(-vocab // pieces)) // 256) * 256)
+
+
+def _combine_over_group(stats, labels, ignore_index, group):
+    """Per-row loss and log-sum-exp from ``{maximum, sum, label's logit}`` of every slice of the vocabulary."""
+    top = stats[:, 0].clone()
+    torch.distributed.all_reduce(top, op=torch.distributed.ReduceOp.MAX, group=group)
+    rest = stats[:, 1:].clone()
+    rest[:, 0] *= torch.exp(stats[:, 0] - top)
+    torch.distributed.all_reduce(rest, group=group)
+    lse = rest[:, 0].log() + top
+    return torch.where(labels == ignore_index, torch.zeros_like(lse), lse - rest[:, 1]), lse
+
+
+class _LinearXentFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, labels, v0, group, ignore_index):
+        ctx.v0, ctx.ignore, ctx.x_shape = v0, ignore_index, x.shape
+        ctx.param = F._bucket_owner(weight)
+        vocab, k = weight.shape
+        x2, w2 = _rows(x, k), weight
+        rows = x2.shape[0]
+        split = group is not None and torch.distributed.get_world_size(group) > 1
+        if not use_native(x2):
+            logits = x2.float() @ weight.float().t()
+            if bias is not None:
+                logits += bias.float()
+            at = labels - v0
+            inside = (at >= 0) & (at < vocab)
+            top = logits.max(-1).values
+            target = torch.where(inside, logits.gather(1, at.clamp(0, vocab - 1)[:, None])[:, 0], torch.zeros_like(top))
+            total = torch.exp(logits - top[:, None]).sum(-1)
+            if split:
+                loss, lse = _combine_over_group(torch.stack([top, total, target], 1), labels, ignore_index, group)
+            else:
+                lse = total.log() + top
+                loss = torch.where(labels == ignore_index, torch.zeros_like(lse), lse - target)
+        else:
+            w2 = _rows(weight, k)
+            tiles = native.kernels().mb_xent_linear_tiles(vocab)
+            # [tile][row] statistics, labels' logits, and per row: loss and lse, or what the group combines
+            work = torch.empty((2 * tiles + 1) * rows, dtype=torch.float32, device=x.device)
+            out = torch.empty(3 if split else 2, rows, dtype=torch.float32, device=x.device)
+            loss, lse = out[0], out[1]
+            call("mb_xent_linear_fwd", ptr(x2), ptr(w2), ptr(bias), ptr(labels), ptr(work), ptr(work) + 8 * tiles * rows,
+                 ptr(loss), ptr(lse), ptr(out) if split else 0, rows, vocab, k, x2.stride(0), w2.stride(0), v0, ignore_index,
+                 F.Settings.gemm_max_ctas, stream())
+            if split:
+                loss, lse = _combine_over_group(out.view(rows, 3), labels, ignore_index, group)
+        ctx.save_for_backward(x2, weight, bias, labels, lse)
+        return loss
+
+    @staticmethod
+    def backward(ctx, gloss):
+        x2, weight, bias, labels, lse = ctx.saved_tensors
+        rows, k = x2.shape
+        vocab = weight.shape[0]
+        want_x, want_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        want_b = bias is not None and ctx.needs_input_grad[2]
+        bucket = getattr(ctx.param, "grad_bucket", None) if want_w else None
+        accumulate = bucket is not None and bool(getattr(ctx.param, "grad_accumulate", False))
+        direct = bucket is not None and bucket.dtype in (torch.float32, weight.dtype) and bucket.stride(1) == 1
+        dw = None
+        if direct:
+            dw = bucket
+        elif want_w:
+            dw = torch.empty(vocab, k, dtype=weight.dtype if bucket is None else torch.float32, device=x2.device)
+        dx = torch.empty(rows, k, dtype=x2.dtype, device=x2.device) if want_x else None
+        db = torch.empty(vocab, dtype=bias.dtype, device=x2.device) if want_b else None
+        add = direct and accumulate
+        gloss = gloss.float().contiguous()
+        if rows == 0:
+            for t in (db, None if add else dw):
+                if t is not None:
+                    t.zero_()
+        elif use_native(x2):
+            w2, piece, ctas = _rows(weight, k), piece_columns(rows, vocab), F.Settings.gemm_max_ctas
+            fp32 = int(dw is not None and dw.dtype == torch.float32)
+            area = native.kernels().mb_xent_linear_bwd_workspace(rows, vocab, k, piece, want_x, want_w, want_b, fp32, add, ctas)
+            workspace = torch.empty(area, dtype=torch.uint8, device=x2.device)
+            call("mb_xent_linear_bwd", ptr(x2), ptr(w2), ptr(bias), ptr(labels), ptr(lse), ptr(gloss), ptr(dx), ptr(dw), ptr(db),
+                 rows, vocab, k, x2.stride(0), w2.stride(0), 0 if dw is None else dw.stride(0), fp32, add, 0, ctx.v0, ctx.ignore,
+                 piece, ctas, ptr(workspace), stream())
+        else:
+            _reference_backward(x2, weight, bias, labels, lse, gloss, ctx.v0, ctx.ignore, dx, dw, add, db)
+        if bucket is not None:
+            if not direct:
+                bucket.add_(dw) if accumulate else bucket.copy_(dw)      # any type and order
+            ctx.param.grad_accumulate = True
+        return (None if dx is None else dx.reshape(ctx.x_shape), dw if bucket is None else None, db, None, None, None, None)
+
+
+def _reference_backward(x2, weight, bias, labels, lse, gloss, v0, ignore, dx, dw, accumulate, db):
+    logits = x2.float() @ weight.float().t()
+    if bias is not None:
+        logits += bias.float()
+    p = torch.exp(logits - lse[:, None])
+    at = labels - v0
+    inside = (at >= 0) & (at < weight.shape[0])
+    p[inside, at[inside]] -= 1.0
+    p = torch.where((labels == ignore)[:, None], torch.zeros_like(p), p * gloss[:, None])
+    if dw is not None:
+        g = p.t() @ x2.float()
+        dw.add_(g.to(dw.dtype)) if accumulate else dw.copy_(g)
+    if db is not None:
+        db.copy_(p.sum(0))
+    if dx is not None:
+        dx.copy_(p @ weight.float())
+
+
+def linear_cross_entropy(x, weight, labels, bias=None, vocab_start: int = 0, group=None, ignore_index: int = -100):
+    """Loss (fp32) of every row of ``x`` ``[..., hidden]`` against ``labels`` ``[...]``: the cross entropy of the logits
+    ``x @ weight.T + bias``, which are computed in fp32 and not kept.  Rows labelled ``ignore_index`` have loss 0 and
+    give no gradient.
+
+    ``weight`` ``[vocab, hidden]`` (and ``bias`` ``[vocab]``) may be this rank's slice of the vocabulary, starting at
+    ``vocab_start``; ``group`` is then the group of the slices, and ``x`` is the same on every rank of it (its gradient is
+    this slice's share).  The weight's gradient goes into its bucket where it has one."""
+    if F._elsewhere(x):
+        with torch.cuda.device(x.device):
+            return linear_cross_entropy(x, weight, labels, bias, vocab_start, group, ignore_index)
+    if weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.shape[0] == 0:
+        raise ValueError(f"x {tuple(x.shape)} does not fit a weight {tuple(weight.shape)}")
+    if labels.shape != x.shape[:-1] or labels.is_floating_point():
+        raise ValueError(f"labels: integers of shape {tuple(x.shape[:-1])} expected, got {tuple(labels.shape)} of {labels.dtype}")
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise ValueError(f"bias {tuple(bias.shape)} does not fit a weight {tuple(weight.shape)}")
+    for t in (weight, labels, bias):
+        if t is not None and t.device != x.device:
+            raise ValueError("x, weight, labels and bias have to be on one device")
+    if use_native(x):
+        if any(t is not None and t.dtype != torch.bfloat16 for t in (x, weight, bias)) or x.shape[-1] % 8:
+            raise ValueError("the kernels take bf16 of a hidden size that is a multiple of 8")
+        if bias is not None and not bias.is_contiguous():
+            bias = bias.contiguous()
+    labels = labels.reshape(-1).long().contiguous()
+    return _LinearXentFn.apply(x, weight, bias, labels, int(vocab_start), group, int(ignore_index)).reshape(x.shape[:-1])
