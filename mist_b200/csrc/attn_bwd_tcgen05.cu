@@ -21,6 +21,8 @@
 // csrc/flash_attn/src/flash_bwd_kernel.h, flash_bwd_launch_template.h:12-43; the kernel
 // families dot_do_o / dq_dk_dv_loop / convert_dq map onto the three kernels here).
 #include "sm100.cuh"
+#include "packed_plan.cuh"
+#include <type_traits>
 
 using namespace sm100;
 
@@ -623,7 +625,7 @@ MB_API int mb_attn_bwd(const void* dout, const void* q, const void* k, const voi
   p.seqlens_k = seqlens_k;
   p.status = mb_status_device_ptr();
   if (pipelined) {
-    const auto kern = d > 80 ? wide::attn_bwd_wide_kernel<true> : wide::attn_bwd_wide_kernel<false>;
+    const auto kern = d > 80 ? wide::attn_bwd_wide_kernel<true, false> : wide::attn_bwd_wide_kernel<false, false>;
     static bool cfg[2] = {false, false};
     if (!cfg[d > 80]) {
       if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, wide::kSmem) != cudaSuccess)
@@ -663,6 +665,90 @@ MB_API int mb_attn_bwd(const void* dout, const void* q, const void* k, const voi
     if (blocks > 148 * 16) blocks = 148 * 16;
     attn_convert_dq_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
         dq_acc, reinterpret_cast<__nv_bfloat16*>(dq), batch, sq, nh, d, dq_bs, dq_ts, dq_hs, pipelined ? scale : 1.f);
+  }
+  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+}
+
+// Backward pass of mb_attn_fwd_packed: dout, o [total_q][nh][d] contiguous, delta [nh][total_q] and dq_acc [nh][total_q][d]
+// fp32 scratch (dq_acc zeroed by this call), dq [total_q][nh][d], dk / dv [total_k][nh / unit_heads][d] with element strides
+// of rows and heads.  Rows that belong to no sequence get zeros.
+MB_API int mb_attn_bwd_packed(const void* dout, const void* q, const void* k, const void* v, const void* o, const float* lse,
+                              float* delta, float* dq_acc, void* dq, void* dk, void* dv, const void* plan, int n, int total_q,
+                              int total_k, int nh, int nh_kv, int unit_heads, int d, long q_ts, long q_hs, long k_ts, long k_hs,
+                              long v_ts, long v_hs, long dq_ts, long dq_hs, long dk_ts, long dk_hs, long dv_ts, long dv_hs,
+                              float scale, int causal, cudaStream_t stream) {
+  if (d % 16 || d > 128 || d < 16 || n < 0 || total_q < 0 || total_k < 0) return -1;
+  if (nh_kv < 1 || nh % nh_kv || unit_heads < 1 || (nh / nh_kv) % unit_heads) return -1;
+  if ((q_ts | q_hs | k_ts | k_hs | v_ts | v_hs | dq_ts | dq_hs | dk_ts | dk_hs | dv_ts | dv_hs) & 7) return -1;
+  if ((reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
+       reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(dq) |
+       reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv) | reinterpret_cast<uintptr_t>(dq_acc) |
+       reinterpret_cast<uintptr_t>(plan)) & 15)
+    return -1;
+  const long rows = static_cast<long>(total_q) * nh, units = nh / unit_heads;
+  const long most = packed_backward_items(total_k, n) * units;
+  if (rows > 0x7fffffff || most > 0x3fffffff) return -1;
+  if (total_q > 0) {
+    attn_delta_kernel<<<static_cast<unsigned>((rows + 16 * kDeltaRows - 1) / (16 * kDeltaRows)), 256, 0, stream>>>(
+        reinterpret_cast<const __nv_bfloat16*>(dout), reinterpret_cast<const __nv_bfloat16*>(o), delta, 1, total_q, nh, d,
+        rows * d, static_cast<long>(nh) * d, d, rows * d, static_cast<long>(nh) * d, d);
+    if (cudaMemsetAsync(dq_acc, 0, sizeof(float) * rows * static_cast<size_t>(d), stream) != cudaSuccess) return -4;
+  }
+  if (total_k > 0) {
+    const bool queries = total_q > 0;      // none: maps over the keys stand in, no item loads through them
+    CUtensorMap tq, tk, tv, tdo, tdq;
+    const void* qp = queries ? q : k;
+    const int qn = queries ? total_q : total_k, qh = queries ? nh : nh_kv;
+    const long qs = queries ? q_ts : k_ts, qhs = queries ? q_hs : k_hs;
+    if (!make_map4(&tq, qp, 1, qn, qh, d, qs * qn, qs, qhs, wide::BB)) return -2;
+    if (!make_map4(&tk, k, 1, total_k, nh_kv, d, k_ts * total_k, k_ts, k_hs, wide::BB)) return -2;
+    if (!make_map4(&tv, v, 1, total_k, nh_kv, d, v_ts * total_k, v_ts, v_hs, wide::BB)) return -2;
+    if (queries) {
+      if (!make_map4(&tdo, dout, 1, total_q, nh, d, rows * d, static_cast<long>(nh) * d, d, wide::BB)) return -2;
+      if (!make_map_dq(&tdq, dq_acc, nh, total_q, d, wide::BB)) return -2;
+    } else {
+      tdo = tdq = tq;
+    }
+    wide::PackedParams p;
+    p.lse = lse; p.delta = delta;
+    p.dk = reinterpret_cast<__nv_bfloat16*>(dk);
+    p.dv = reinterpret_cast<__nv_bfloat16*>(dv);
+    p.dk_bs = p.dv_bs = 0;
+    p.dk_ts = dk_ts; p.dk_hs = dk_hs;
+    p.dv_ts = dv_ts; p.dv_hs = dv_hs;
+    p.sq = total_q; p.sk = total_k; p.nh = nh; p.nh_kv = nh_kv; p.d = d;
+    p.nchunks = (d + 63) / 64;
+    p.scale = scale;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    p.causal = causal;
+    p.seqlens_q = p.seqlens_k = nullptr;
+    p.status = mb_status_device_ptr();
+    const uint8_t* list = static_cast<const uint8_t*>(plan) + packed_list_offset(total_q, total_k, n, 1, causal != 0);
+    p.count = reinterpret_cast<const int*>(list);
+    p.items = reinterpret_cast<const PackedItem*>(list + 16);
+    const auto kern = d > 80 ? wide::attn_bwd_wide_kernel<true, true> : wide::attn_bwd_wide_kernel<false, true>;
+    int dev = 0;
+    static bool cfg[64][2] = {};
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -3;
+    if (!cfg[dev][d > 80]) {
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, wide::kSmem) != cudaSuccess) return -3;
+      cfg[dev][d > 80] = true;
+    }
+    wide::Sched sch;
+    sch.nblk = sch.total = 0;      // from the plan
+    sch.units = static_cast<int>(units);
+    sch.unit_heads = unit_heads;
+    sch.bu = sch.units;
+    const long unit_bytes = 8l * unit_heads * (total_q > 0 ? total_q : 1) * d;
+    const long group = (48l << 20) / unit_bytes;
+    sch.group = static_cast<int>(group < 1 ? 1 : (group < units ? group : units));
+    kern<<<most < 148 ? static_cast<int>(most) : 148, wide::kThreads, wide::kSmem, stream>>>(tq, tk, tv, tdo, tdq, p, sch);
+  }
+  if (total_q > 0) {
+    long blocks = (rows * (d / 8) + 255) / 256;
+    if (blocks > 148 * 16) blocks = 148 * 16;
+    attn_convert_dq_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
+        dq_acc, reinterpret_cast<__nv_bfloat16*>(dq), 1, total_q, nh, d, 0, dq_ts, dq_hs, scale);
   }
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }

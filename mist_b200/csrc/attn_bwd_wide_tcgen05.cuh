@@ -33,6 +33,8 @@
 //   dq_full, dq_empty  MMA <-> dQ warps   dQ is complete / is in registers
 //   fin_full           MMA -> softmax     one phase per work item: dV, dK are complete
 //   vec_full/vec_empty[2]                 LSE and delta of the block's queries
+//   k_cut, q_cut[2], do_cut               packed sequences: a tile that ends inside, before warp 23 zeroes its rows behind
+//                                         the end and passes it on as k_full, q_full, do_full
 #pragma once
 
 namespace wide {
@@ -44,9 +46,17 @@ constexpr int kDqChunk = BB * 128;        // [128 q][32 fp32]
 constexpr int oK = 0, oV = kTile, oQ = 2 * kTile, oDO = 4 * kTile, oDS = 5 * kTile, oDQ = 6 * kTile;
 constexpr int oVec = oDQ + 2 * kDqChunk;  // -LSE*log2(e) and -delta of two query blocks
 constexpr int oBar = oVec + 2 * 2 * BB * 4;
-constexpr int kNumBars = 4 + 4 + 2 + 2 + 1 + 2 + 2 + 1 + 4;
+constexpr int kNumBars = 4 + 4 + 2 + 2 + 1 + 2 + 2 + 1 + 4 + 4;
 constexpr int kSmem = oBar + kNumBars * 8 + 16;
 static_assert(kSmem <= 232448, "attention backward: shared memory over the per-CTA limit");
+
+// Sequences packed back to back: sq and sk are all rows, batch is 1, the items of a plan take the place of key blocks.
+struct PackedParams : BwdParams {
+  const int* count;          // number of items
+  const PackedItem* items;
+};
+template <bool PACKED>
+using ParamsOf = std::conditional_t<PACKED, PackedParams, BwdParams>;
 
 struct Sched {
   int nblk;         // key blocks
@@ -59,14 +69,47 @@ struct Sched {
 
 struct Work {
   int batch, unit, kv0, sq_b, sk_b, coff, i_start, per_head, n_iter;
+  int q_row, k_row;      // first rows of the sequence (packed sequences; 0 otherwise)
 };
 
 __device__ __forceinline__ int work_index(int n) {
   return n * gridDim.x + ((n & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
+// Query blocks that see a key block.
+__device__ __forceinline__ void fill_blocks(Work& w, int kv0, bool causal, int unit_heads) {
+  w.kv0 = kv0;
+  w.coff = w.sk_b - w.sq_b;
+  w.i_start = 0;
+  if (causal) {
+    const int first_q = w.kv0 - w.coff;      // first query row that sees key kv0
+    w.i_start = first_q <= 0 ? 0 : first_q / BB;
+  }
+  w.per_head = w.kv0 < w.sk_b ? max(0, (w.sq_b + BB - 1) / BB - w.i_start) : 0;
+  w.n_iter = w.per_head * unit_heads;
+}
+
+__device__ __forceinline__ Work work_at(const PackedParams& p, const Sched& s, int t) {
+  Work w;
+  const int per_group = s.group * s.nblk;
+  const int g = t / per_group, r = t - g * per_group;
+  const int gsize = min(s.group, s.bu - g * s.group);
+  const int at = r / gsize;
+  w.unit = g * s.group + (r - at * gsize);
+  w.batch = 0;
+  const int4 a = *reinterpret_cast<const int4*>(&p.items[at]);
+  const int first = p.items[at].first;
+  w.q_row = a.x;
+  w.sq_b = a.y;
+  w.k_row = a.z;
+  w.sk_b = a.w;
+  fill_blocks(w, first, p.causal, s.unit_heads);
+  return w;
+}
+
 __device__ __forceinline__ Work work_at(const BwdParams& p, const Sched& s, int t) {
   Work w;
+  w.q_row = w.k_row = 0;
   const int per_group = s.group * s.nblk;
   const int g = t / per_group, r = t - g * per_group;
   const int gsize = min(s.group, s.bu - g * s.group);
@@ -77,15 +120,7 @@ __device__ __forceinline__ Work work_at(const BwdParams& p, const Sched& s, int 
   // real tokens of this sample (right-padded batches); the tensors keep their padded extents p.sq / p.sk
   w.sq_b = p.seqlens_q ? min(p.sq, p.seqlens_q[w.batch]) : p.sq;
   w.sk_b = p.seqlens_k ? min(p.sk, p.seqlens_k[w.batch]) : p.sk;
-  w.kv0 = jb * BB;
-  w.coff = w.sk_b - w.sq_b;
-  w.i_start = 0;
-  if (p.causal) {
-    const int first_q = w.kv0 - w.coff;      // first query row that sees key kv0
-    w.i_start = first_q <= 0 ? 0 : first_q / BB;
-  }
-  w.per_head = w.kv0 < w.sk_b ? max(0, (w.sq_b + BB - 1) / BB - w.i_start) : 0;
-  w.n_iter = w.per_head * s.unit_heads;
+  fill_blocks(w, jb * BB, p.causal, s.unit_heads);
   return w;
 }
 
@@ -106,11 +141,11 @@ __device__ __forceinline__ void store16(__nv_bfloat16* dst, const uint32_t* v, f
   }
 }
 
-template <bool kAlias>
+template <bool kAlias, bool PACKED>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
-                     const __grid_constant__ CUtensorMap tm_dq, const BwdParams p, const Sched sch) {
+                     const __grid_constant__ CUtensorMap tm_dq, const ParamsOf<PACKED> p, const Sched dealt) {
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + oBar);
   uint64_t* k_full = bars;
@@ -131,6 +166,9 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   uint64_t* fin_full = bars + 17;
   uint64_t* vec_full = bars + 18;
   uint64_t* vec_empty = bars + 20;
+  uint64_t* k_cut = bars + 22;
+  uint64_t* q_cut = bars + 23;
+  uint64_t* do_cut = bars + 25;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kNumBars);
 
   const int warp = threadIdx.x >> 5;
@@ -143,7 +181,7 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   if (threadIdx.x == 0) {
     for (int i = 0; i < kNumBars; ++i) {
       const uint64_t* b = bars + i;
-      mbar_init(bars + i, (b == p_full || b == ds_full || b >= vec_empty) ? 16 : (b == dq_empty ? 4 : 1));   // warps
+      mbar_init(bars + i, (b == p_full || b == ds_full || (b >= vec_empty && b < k_cut)) ? 16 : (b == dq_empty ? 4 : 1));   // warps
     }
     fence_barrier_init();
     prefetch_tmap(&tm_q);
@@ -164,6 +202,11 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   const uint32_t t_dq = kAlias ? t_dp : tmem_base + 256;
   const uint32_t t_dv = tmem_base + (kAlias ? 256 : 336), t_dk = tmem_base + (kAlias ? 384 : 416);
   constexpr uint32_t kChunk = BB * 128;
+  Sched sch = dealt;
+  if constexpr (PACKED) {
+    sch.nblk = *p.count;
+    sch.total = sch.nblk * sch.bu;
+  }
 
   // Registers: 768 threads were launched with 80 each; 512 * 64 + 128 * 160 + 128 * 64 is the same sum.
   if (warp >= 20) {
@@ -174,15 +217,16 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         int n = 0, items = 0;                // query blocks and work items so far
         bool ok = true;
         auto load = [&](int off, const CUtensorMap* tm, uint64_t* full, uint64_t* empty, int uses, int head, int row,
-                        int batch) {
+                        int batch, uint64_t* cut) {
           if (!ok) return;
           if (uses > 0 && !mbar_wait(empty, (uses - 1) & 1)) {
             report(p.status, MB_ERR_TIMEOUT_EMPTY);
             ok = false;
             return;
           }
-          mbar_expect_tx(full, p.nchunks * kChunk);
-          for (int c = 0; c < p.nchunks; ++c) tma_load_4d(smem + off + c * kChunk, tm, full, 64 * c, head, row, batch);
+          uint64_t* bar = PACKED && cut ? cut : full;
+          mbar_expect_tx(bar, p.nchunks * kChunk);
+          for (int c = 0; c < p.nchunks; ++c) tma_load_4d(smem + off + c * kChunk, tm, bar, 64 * c, head, row, batch);
         };
         for (int r = 0; ok; ++r) {
           const int t = work_index(r);
@@ -190,18 +234,54 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           const Work w = work_at(p, sch, t);
           if (w.n_iter == 0) continue;
           const int head0 = w.unit * sch.unit_heads, head_kv = head0 / (p.nh / p.nh_kv);
-          load(oK, &tm_k, k_full, k_empty, items, head_kv, w.kv0, w.batch);
+          const int kv0 = w.k_row + w.kv0;
+          load(oK, &tm_k, k_full, k_empty, items, head_kv, kv0, w.batch, w.kv0 + BB > w.sk_b ? k_cut : nullptr);
           int hh = 0, i = 0;
           for (int it = 0; it < w.n_iter && ok; ++it) {
-            const int st = n & 1, q0 = (w.i_start + i) * BB;
-            load(oQ + st * kTile, &tm_q, &q_full[st], &q_empty[st], n >> 1, head0 + hh, q0, w.batch);
-            if (it == 0) load(oV, &tm_v, v_full, v_empty, items, head_kv, w.kv0, w.batch);
-            load(oDO, &tm_do, do_full, do_empty, n, head0 + hh, q0, w.batch);
+            const int st = n & 1, q0 = w.q_row + (w.i_start + i) * BB;
+            const bool cut = i == w.per_head - 1 && q0 + BB > w.q_row + w.sq_b;
+            load(oQ + st * kTile, &tm_q, &q_full[st], &q_empty[st], n >> 1, head0 + hh, q0, w.batch, cut ? &q_cut[st] : nullptr);
+            if (it == 0) load(oV, &tm_v, v_full, v_empty, items, head_kv, kv0, w.batch, nullptr);
+            load(oDO, &tm_do, do_full, do_empty, n, head0 + hh, q0, w.batch, cut ? do_cut : nullptr);
             ++n;
             if (++i == w.per_head) { i = 0; ++hh; }
           }
           ++items;
         }
+      }
+    } else if (PACKED && warp == 23) {
+      // ------------------- rows behind the last key of K and behind the last query of Q and dO
+      // They belong to the next sequence.  Their probabilities are 0, but 0 times an infinity is not.
+      int n = 0;
+      uint32_t uses = 0;                   // parities: bit 0 K, 1 and 2 Q, 3 dO
+      bool ok = true;
+      auto zero_rows = [&](int off, int from, uint64_t* cut, uint64_t* full, int bit) {
+        if (!ok) return;
+        if (!mbar_wait(cut, (uses >> bit) & 1)) {
+          report(p.status, MB_ERR_TIMEOUT_FULL);
+          ok = false;
+          return;
+        }
+        uses ^= 1u << bit;
+        for (int at = from * 128 + lane * 16; at < static_cast<int>(kChunk); at += 512)
+          for (int c = 0; c < p.nchunks; ++c)
+            *reinterpret_cast<uint4*>(smem + off + c * kChunk + at) = make_uint4(0, 0, 0, 0);
+        fence_async_smem();
+        mbar_arrive_warp(full);
+      };
+      for (int r = 0; ok; ++r) {
+        const int t = work_index(r);
+        if (t >= sch.total) break;
+        const Work w = work_at(p, sch, t);
+        if (w.n_iter == 0) continue;
+        if (w.kv0 + BB > w.sk_b) zero_rows(oK, w.sk_b - w.kv0, k_cut, k_full, 0);
+        const int rest = w.sq_b - (w.i_start + w.per_head - 1) * BB;      // queries of the last block
+        for (int hh = 0; hh < sch.unit_heads && rest < BB && ok; ++hh) {
+          const int st = (n + (hh + 1) * w.per_head - 1) & 1;
+          zero_rows(oQ + st * kTile, rest, &q_cut[st], &q_full[st], 1 + st);
+          zero_rows(oDO, rest, do_cut, do_full, 3);
+        }
+        n += w.n_iter;
       }
     } else if (warp == 22) {
       // ------------------------------------------- LSE and delta of every query block
@@ -214,7 +294,7 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         const Work w = work_at(p, sch, t);
         int hh = 0, i = 0;
         for (int it = 0; it < w.n_iter; ++it, ++n) {
-          const long row = (static_cast<long>(w.batch) * p.nh + w.unit * sch.unit_heads + hh) * p.sq;
+          const long row = (static_cast<long>(w.batch) * p.nh + w.unit * sch.unit_heads + hh) * p.sq + w.q_row;
           const int q = (w.i_start + i) * BB + lane;
           float lse[4], delta[4];
 #pragma unroll
@@ -384,6 +464,10 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         tmem_ld_wait();
         tc_fence_before();
         mbar_arrive_warp(dq_empty);
+        if (PACKED && (w.i_start + i) * BB + r >= w.sq_b) {      // rows of the next sequence
+#pragma unroll
+          for (int c = 0; c < 128; ++c) qr[c] = 0;
+        }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           if (c >= nw) break;
@@ -400,7 +484,7 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             asm volatile(
                 "cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group "
                 "[%0, {%2, %3, %4}], [%1];\n" ::"l"(reinterpret_cast<uint64_t>(&tm_dq)),
-                "r"(smem_u32(sdq_ + buf * kDqChunk)), "r"(32 * c), "r"((w.i_start + i) * BB),
+                "r"(smem_u32(sdq_ + buf * kDqChunk)), "r"(32 * c), "r"(w.q_row + (w.i_start + i) * BB),
                 "r"(w.batch * p.nh + w.unit * sch.unit_heads + hh)
                 : "memory");
             tma_commit();
@@ -458,7 +542,8 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           pf[c + 2] = __float_as_uint(mb::fast_exp2(xb.x));
           pf[c + 3] = __float_as_uint(mb::fast_exp2(xb.y));
         }
-        if ((q0 + BB > w.sq_b) || (kv_last >= w.sk_b) || (p.causal && kv_last > q0 + w.coff)) {
+        const bool masked = (q0 + BB > w.sq_b) || (kv_last >= w.sk_b) || (p.causal && kv_last > q0 + w.coff);
+        if (masked) {
           // visible columns of this key row: lo <= c < hi
           const int lo = p.causal ? kv_idx - w.coff - q0 - c0 : 0;
           const int hi = kv_idx < w.sk_b ? w.sq_b - q0 - c0 : 0;
@@ -499,6 +584,14 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             ds[c >> 1] = pack2(a.x, a.y);
             ds[(c >> 1) + 1] = pack2(b.x, b.y);
           }
+          if (PACKED && masked) {      // 0 times what the rows of another sequence hold
+            const int lo = p.causal ? kv_idx - w.coff - q0 - c0 - 16 * h : 0;
+            const int hi = kv_idx < w.sk_b ? w.sq_b - q0 - c0 - 16 * h : 0;
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              if (c < lo || c >= hi) ds[c >> 1] &= (c & 1) ? 0x0000ffffu : 0xffff0000u;
+            }
+          }
 #pragma unroll
           for (int g = 0; g < 2; ++g)
             *reinterpret_cast<uint4*>(sds_ + (((4 * (part & 1) + 2 * h + g) ^ (r & 7)) << 4)) =
@@ -520,8 +613,8 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         ++items;
         tc_fence_after();
       }
-      __nv_bfloat16* dkrow = p.dk + w.batch * p.dk_bs + static_cast<long>(kv_idx) * p.dk_ts + w.unit * p.dk_hs;
-      __nv_bfloat16* dvrow = p.dv + w.batch * p.dv_bs + static_cast<long>(kv_idx) * p.dv_ts + w.unit * p.dv_hs;
+      __nv_bfloat16* dkrow = p.dk + w.batch * p.dk_bs + static_cast<long>(w.k_row + kv_idx) * p.dk_ts + w.unit * p.dk_hs;
+      __nv_bfloat16* dvrow = p.dv + w.batch * p.dv_bs + static_cast<long>(w.k_row + kv_idx) * p.dv_ts + w.unit * p.dv_hs;
       for (int c = part * 16; c < p.d; c += 64) {
         uint32_t a[16], b[16];
         if (w.n_iter > 0) {
@@ -532,7 +625,7 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 #pragma unroll
           for (int u = 0; u < 16; ++u) a[u] = b[u] = 0;
         }
-        if (kv_idx < p.sk) {
+        if (kv_idx < (PACKED ? w.sk_b : p.sk)) {      // rows behind a packed sequence are the next one's
           store16(dvrow + c, a, 1.f, wide_store);
           store16(dkrow + c, b, p.scale, wide_store);
         }

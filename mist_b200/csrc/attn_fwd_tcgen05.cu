@@ -32,6 +32,8 @@
 // (reference: csrc/flash_attn/src/flash_fwd_kernel.h, flash_fwd_launch_template.h:13-28,
 // dispatch mist/modules/flash_attn.py:46-213).
 #include "sm100.cuh"
+#include "packed_plan.cuh"
+#include <type_traits>
 
 using namespace sm100;
 
@@ -44,8 +46,8 @@ constexpr int kSlots = 5;                 // ring of K and V tiles in the order 
 constexpr int kTile = 2 * 128 * 128;      // 128 rows of up to two 64-wide chunks
 constexpr int oRing = 2 * kTile;
 constexpr int oBar = oRing + kSlots * kTile;
-// q_full[2], q_empty[2], full[5], empty[5], s_full[2], p_full[2][2], o_full[2]
-constexpr int kNumBars = 2 + 2 + kSlots + kSlots + 2 + 4 + 2;
+// q_full[2], q_empty[2], full[5], empty[5], s_full[2], p_full[2][2], o_full[2], packed sequences only: tail[5]
+constexpr int kNumBars = 2 + 2 + kSlots + kSlots + 2 + 4 + 2 + kSlots;
 constexpr int oMax = oBar + kNumBars * 8 + 16;      // [tile][half][row] maxima (and, at the end, sums)
 constexpr int kSmem = oMax + 2 * 2 * BM * 4;
 static_assert(kSmem <= 232448, "attention forward: shared memory over the per-CTA limit");
@@ -63,6 +65,14 @@ struct AttnParams {
   const int* seqlens_k;
   int* status;
 };
+
+// Sequences packed back to back: sq and sk are all rows, batch is 1, the items of a plan take the place of tiles.
+struct PackedParams : AttnParams {
+  const int* count;          // number of items
+  const PackedItem* items;
+};
+template <bool PACKED>
+using ParamsOf = std::conditional_t<PACKED, PackedParams, AttnParams>;
 
 __device__ __forceinline__ void report(int* status, int code) {
   if (status) atomicCAS(status, 0, code);
@@ -82,6 +92,7 @@ struct Sched {
 
 struct Work {
   int q0[2], nb[2], nbmax, head, batch, sq_b, sk_b, coff;
+  int q_row, k_row;      // first rows of the sequence (packed sequences; 0 otherwise)
 };
 
 __device__ __forceinline__ int work_index(int n) {
@@ -89,8 +100,45 @@ __device__ __forceinline__ int work_index(int n) {
   return n * gridDim.x + c;
 }
 
+// What the two tiles of a work item see: blocks of keys.
+__device__ __forceinline__ void fill_tiles(Work& w, int first, bool causal) {
+  w.coff = w.sk_b - w.sq_b;
+  w.nbmax = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int q0 = first + i * BM;
+    int nb = (q0 < w.sq_b) ? (w.sk_b + BN - 1) / BN : 0;
+    if (causal) {
+      const int last = q0 + BM - 1 + w.coff;
+      nb = min(nb, last < 0 ? 0 : last / BN + 1);
+    }
+    w.q0[i] = q0;
+    w.nb[i] = nb;
+    w.nbmax = max(w.nbmax, nb);
+  }
+}
+
+__device__ __forceinline__ Work work_at(const PackedParams& p, const Sched& s, int t) {
+  Work w;
+  const int items = s.total / p.nh, per_group = s.group * items;
+  const int g = t / per_group, r = t - g * per_group;
+  const int gsize = min(s.group, p.nh - g * s.group);
+  const int at = r / gsize;
+  w.head = g * s.group + (r - at * gsize);
+  w.batch = 0;
+  const int4 a = *reinterpret_cast<const int4*>(&p.items[at]);
+  const int first = p.items[at].first;
+  w.q_row = a.x;
+  w.sq_b = a.y;
+  w.k_row = a.z;
+  w.sk_b = a.w;
+  fill_tiles(w, first, p.causal);
+  return w;
+}
+
 __device__ __forceinline__ Work work_at(const AttnParams& p, const Sched& s, int t) {
   Work w;
+  w.q_row = w.k_row = 0;
   const int per_group = s.group * s.npairs;
   const int g = t / per_group, r = t - g * per_group;
   const int gsize = min(s.group, s.bh - g * s.group);
@@ -100,20 +148,7 @@ __device__ __forceinline__ Work work_at(const AttnParams& p, const Sched& s, int
   w.head = bh - w.batch * p.nh;
   w.sq_b = p.seqlens_q ? min(p.sq, p.seqlens_q[w.batch]) : p.sq;
   w.sk_b = p.seqlens_k ? min(p.sk, p.seqlens_k[w.batch]) : p.sk;
-  w.coff = w.sk_b - w.sq_b;
-  w.nbmax = 0;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int q0 = (2 * (s.npairs - 1 - qi) + i) * BM;
-    int nb = (q0 < w.sq_b) ? (w.sk_b + BN - 1) / BN : 0;
-    if (p.causal) {
-      const int last = q0 + BM - 1 + w.coff;
-      nb = min(nb, last < 0 ? 0 : last / BN + 1);
-    }
-    w.q0[i] = q0;
-    w.nb[i] = nb;
-    w.nbmax = max(w.nbmax, nb);
-  }
+  fill_tiles(w, 2 * (s.npairs - 1 - qi) * BM, p.causal);
   return w;
 }
 
@@ -131,9 +166,10 @@ __device__ __forceinline__ void store16(__nv_bfloat16* dst, const float* f, bool
   }
 }
 
+template <bool PACKED>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                    const __grid_constant__ CUtensorMap tm_v, const AttnParams p, const Sched sch) {
+                    const __grid_constant__ CUtensorMap tm_v, const ParamsOf<PACKED> p, const Sched dealt) {
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + oBar);
   uint64_t* q_full = bars;
@@ -143,6 +179,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   uint64_t* s_full = empty + kSlots;
   uint64_t* p_full = s_full + 2;            // [tile][first, second 32 keys of each half]
   uint64_t* o_full = p_full + 4;
+  uint64_t* tail = o_full + 2;              // [slot] a V tile that ends inside, before its rows behind the end are zeroed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kNumBars);
 
   const int warp = threadIdx.x >> 5;
@@ -164,6 +201,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
+      if (PACKED) mbar_init(&tail[i], 1);
     }
     fence_barrier_init();
     prefetch_tmap(&tm_q);
@@ -179,6 +217,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   constexpr uint32_t kChunk = 128 * 128;
+  Sched sch = dealt;
+  if constexpr (PACKED) sch.total = *p.count * p.nh;
+  // The last V tile of a sequence that ends inside it also holds rows of the next one.  Their probabilities are 0, but 0
+  // times an infinity is not: such a tile is loaded on a barrier of its own, warp 19 zeroes those rows and passes it on.
+  auto ends_inside = [](const Work& w) { return PACKED && w.nbmax * BN > w.sk_b; };
 
   if (warp >= 16) {
     // 640 threads were launched with 96 registers; 512 * 104 + 128 * 64 is the same sum
@@ -188,16 +231,17 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       if (lane == 0) {
         int n = 0, slot = 0;
         bool ok = true;
-        auto load = [&](const CUtensorMap* tm, int row, int head_kv, int batch) {
+        auto load = [&](const CUtensorMap* tm, int row, int head_kv, int batch, bool cut) {
           if (n >= kSlots && !mbar_wait(&empty[slot], (n / kSlots - 1) & 1)) {
             report(p.status, MB_ERR_TIMEOUT_EMPTY);
             ok = false;
             return;
           }
           uint8_t* dst = smem + oRing + slot * kTile;
-          mbar_expect_tx(&full[slot], p.nchunks * kChunk);
+          uint64_t* bar = PACKED && cut ? &tail[slot] : &full[slot];
+          mbar_expect_tx(bar, p.nchunks * kChunk);
           for (int c = 0; c < p.nchunks; ++c)
-            tma_load_4d(dst + c * kChunk, tm, &full[slot], 64 * c, head_kv, row, batch);
+            tma_load_4d(dst + c * kChunk, tm, bar, 64 * c, head_kv, row, batch);
           ++n;
           if (++slot == kSlots) slot = 0;
         };
@@ -207,8 +251,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           const Work w = work_at(p, sch, t);
           const int head_kv = w.head / (p.nh / p.nh_kv);
           for (int j = 0; j < w.nbmax && ok; ++j) {
-            load(&tm_k, j * BN, head_kv, w.batch);
-            if (ok) load(&tm_v, j * BN, head_kv, w.batch);
+            load(&tm_k, w.k_row + j * BN, head_kv, w.batch, false);
+            if (ok) load(&tm_v, w.k_row + j * BN, head_kv, w.batch, j == w.nbmax - 1 && ends_inside(w));
           }
         }
       }
@@ -231,10 +275,35 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             }
             mbar_expect_tx(&q_full[i], p.nchunks * kChunk);
             for (int c = 0; c < p.nchunks; ++c)
-              tma_load_4d(smem + i * kTile + c * kChunk, &tm_q, &q_full[i], 64 * c, w.head, w.q0[i], w.batch);
+              tma_load_4d(smem + i * kTile + c * kChunk, &tm_q, &q_full[i], 64 * c, w.head, w.q_row + w.q0[i],
+                          w.batch);
             ++cq[i];
           }
         }
+      }
+    } else if (PACKED && warp == 19) {
+      // --------------------------------------------------- rows behind the last key
+      int n = 0;                 // ring positions of the items so far
+      uint32_t uses = 0;         // parity of each slot's tails
+      bool ok = true;
+      for (int r = 0; ok; ++r) {
+        const int t = work_index(r);
+        if (t >= sch.total) break;
+        const Work w = work_at(p, sch, t);
+        n += 2 * w.nbmax;
+        if (!ends_inside(w)) continue;
+        const int slot = (n - 1) % kSlots;
+        if (!mbar_wait(&tail[slot], (uses >> slot) & 1)) {
+          report(p.status, MB_ERR_TIMEOUT_FULL);
+          ok = false;
+          break;
+        }
+        uses ^= 1u << slot;
+        uint8_t* v = smem + oRing + slot * kTile;
+        for (int at = (w.sk_b - (w.nbmax - 1) * BN) * 128 + lane * 16; at < static_cast<int>(kChunk); at += 512)
+          for (int c = 0; c < p.nchunks; ++c) *reinterpret_cast<uint4*>(v + c * kChunk + at) = make_uint4(0, 0, 0, 0);
+        fence_async_smem();
+        mbar_arrive_warp(&full[slot]);
       }
     } else if (warp == 17) {
       // ------------------------------------------------------------- MMA issuer
@@ -465,7 +534,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       pair_sync();
       const bool real_row = qi < w.sq_b;
       const float inv = (real_row && l_run > 0.f) ? 1.f / l_run : 0.f;
-      __nv_bfloat16* orow = p.o + w.batch * p.o_batch_stride + static_cast<long>(qi) * p.o_tok_stride +
+      const bool own_row = qi < (PACKED ? w.sq_b : p.sq);      // rows behind a packed sequence are the next one's
+      __nv_bfloat16* orow = p.o + w.batch * p.o_batch_stride + static_cast<long>(w.q_row + qi) * p.o_tok_stride +
                             static_cast<long>(w.head) * p.o_head_stride;
       for (int c = 16 * h; c < p.d; c += 32) {
         uint32_t o[16];
@@ -476,7 +546,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll
           for (int u = 0; u < 16; ++u) o[u] = 0;
         }
-        if (qi < p.sq) {
+        if (own_row) {
           float f[16];
 #pragma unroll
           for (int u = 0; u < 16; ++u) f[u] = __uint_as_float(o[u]) * inv;
@@ -484,8 +554,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
       }
       tc_fence_before();
-      if (h == 0 && qi < p.sq)
-        p.lse[(static_cast<long>(w.batch) * p.nh + w.head) * p.sq + qi] =
+      if (h == 0 && own_row)
+        p.lse[(static_cast<long>(w.batch) * p.nh + w.head) * p.sq + w.q_row + qi] =
             (real_row && l_run > 0.f) ? (m_run + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
     }
   }
@@ -592,7 +662,7 @@ MB_API int mb_attn_fwd(const void* q, const void* k, const void* v, void* o, flo
   }
   static bool cfg = false;
   if (!cfg) {
-    if (cudaFuncSetAttribute(attn_fwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+    if (cudaFuncSetAttribute(attn_fwd_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
       return -3;
     cfg = true;
   }
@@ -605,6 +675,65 @@ MB_API int mb_attn_fwd(const void* q, const void* k, const void* v, void* o, flo
   const long group = (kv_heads < 1 ? 1 : kv_heads) * (nh / nh_kv);
   sch.group = static_cast<int>(group < sch.bh ? group : sch.bh);
   sch.total = static_cast<int>(units);
-  attn_fwd_kernel<<<units < 148 ? static_cast<int>(units) : 148, kThreads, kSmem, stream>>>(tq, tk, tv, p, sch);
+  attn_fwd_kernel<false><<<units < 148 ? static_cast<int>(units) : 148, kThreads, kSmem, stream>>>(tq, tk, tv, p, sch);
+  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+}
+
+// Attention over sequences packed back to back: q, o [total_q][nh][d], k / v [total_k][nh_kv][d] (element strides of rows
+// and heads), lse [nh][total_q].  `plan`: what mb_packed_plan wrote for these totals and n sequences.  Rows that belong to
+// no sequence and queries that see no key get zeros and lse = -inf; what a sequence holds reaches no other.
+MB_API int mb_attn_fwd_packed(const void* q, const void* k, const void* v, void* o, float* lse, const void* plan, int n,
+                              int total_q, int total_k, int nh, int nh_kv, int d, long q_ts, long q_hs, long k_ts, long k_hs,
+                              long v_ts, long v_hs, long o_ts, long o_hs, float scale, int causal, cudaStream_t stream) {
+  if (d % 16 || d > 128 || d < 16 || nh_kv < 1 || nh % nh_kv || n < 0 || total_q < 0 || total_k < 0) return -1;
+  if ((q_ts | q_hs | k_ts | k_hs | v_ts | v_hs | o_ts | o_hs) & 7) return -1;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+       reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(plan)) & 15)
+    return -1;
+  if (total_q == 0) return 0;
+  const long most = packed_forward_items(total_q, n) * nh;
+  if (most > 0x3fffffff) return -1;
+  CUtensorMap tq, tk, tv;
+  // no keys at all: maps over the queries stand in, no item loads through them
+  const bool keys = total_k > 0;
+  if (!make_map(&tq, q, 1, total_q, nh, d, q_ts * total_q, q_ts, q_hs, BM)) return -2;
+  if (!make_map(&tk, keys ? k : q, 1, keys ? total_k : total_q, keys ? nh_kv : nh, d, keys ? k_ts * total_k : q_ts * total_q,
+                keys ? k_ts : q_ts, keys ? k_hs : q_hs, BN))
+    return -2;
+  if (!make_map(&tv, keys ? v : q, 1, keys ? total_k : total_q, keys ? nh_kv : nh, d, keys ? v_ts * total_k : q_ts * total_q,
+                keys ? v_ts : q_ts, keys ? v_hs : q_hs, BN))
+    return -2;
+  PackedParams p;
+  p.o = reinterpret_cast<__nv_bfloat16*>(o);
+  p.lse = lse;
+  p.sq = total_q; p.sk = total_k; p.nh = nh; p.nh_kv = nh_kv; p.d = d;
+  p.d_mma = d;
+  p.nchunks = (d + 63) / 64;
+  p.o_batch_stride = 0; p.o_tok_stride = o_ts; p.o_head_stride = o_hs;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.causal = causal;
+  p.seqlens_q = nullptr;
+  p.seqlens_k = nullptr;
+  p.status = mb_status_device_ptr();
+  const uint8_t* list = static_cast<const uint8_t*>(plan) + packed_list_offset(total_q, total_k, n, 0, causal != 0);
+  p.count = reinterpret_cast<const int*>(list);
+  p.items = reinterpret_cast<const PackedItem*>(list + 16);
+  int dev = 0;
+  static bool cfg[64] = {};
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -3;
+  if (!cfg[dev]) {
+    if (cudaFuncSetAttribute(attn_fwd_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+      return -3;
+    cfg[dev] = true;
+  }
+  Sched sch;
+  sch.npairs = 0;
+  sch.bh = nh;
+  const long kv_bytes = 4l * total_k * d;
+  const long kv_heads = kv_bytes > 0 ? (40l << 20) / kv_bytes : 1;
+  const long group = (kv_heads < 1 ? 1 : kv_heads) * (nh / nh_kv);
+  sch.group = static_cast<int>(group < nh ? group : nh);
+  sch.total = 0;
+  attn_fwd_kernel<true><<<most < 148 ? static_cast<int>(most) : 148, kThreads, kSmem, stream>>>(tq, tk, tv, p, sch);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }

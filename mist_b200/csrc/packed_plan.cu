@@ -1,0 +1,112 @@
+// Builds the work lists of attention over packed sequences (packed_plan.cuh) on the device, so that the offsets never
+// have to be read back to the host.  A step builds them once and every layer's attention walks them.
+#include "common.cuh"
+#include "packed_plan.cuh"
+
+namespace {
+
+constexpr int kThreads = 1024;
+constexpr int kCosts = 8192;       // blocks of 128 a tile walks; dearer ones count as the dearest
+
+// Blocks 0 - 3: one list each.  Counting sort by cost: a warp per sequence, a lane per item.  The offsets are clamped to the tensors,
+// so no content of theirs makes an attention kernel leave them.  Rows behind the last sequence get items without keys (or
+// queries), whose outputs are zeros.  Items of one cost come in no fixed order; no result depends on it but the order in
+// which dQ is summed.
+__global__ void __launch_bounds__(kThreads)
+packed_plan_kernel(const int* cu_q, const int* cu_k, int n, int total_q, int total_k, uint8_t* plan, int64_t* positions) {
+  __shared__ int count[kCosts];
+  __shared__ int part[32];
+  if (blockIdx.x >= 4) {      // a row's place in its sequence: the last offset that is not above it
+    const int row = (blockIdx.x - 4) * kThreads + threadIdx.x;
+    if (row >= total_q) return;
+    int lo = 0, hi = n;       // the first offset counts as 0
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (cu_q[mid] <= row) lo = mid;
+      else hi = mid - 1;
+    }
+    positions[row] = lo ? row - cu_q[lo] : row;
+    return;
+  }
+  const int backward = blockIdx.x >> 1, causal = blockIdx.x & 1;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint8_t* list = plan + packed_list_offset(total_q, total_k, n, backward, causal);
+  PackedItem* items = reinterpret_cast<PackedItem*>(list + 16);
+  const int cap = static_cast<int>(backward ? packed_backward_items(total_k, n) : packed_forward_items(total_q, n));
+  for (int i = tid; i < kCosts; i += kThreads) count[i] = 0;
+  __syncthreads();
+  auto clamped = [](int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); };
+  auto walk = [&](auto&& f) {
+    for (int b = warp; b <= n; b += kThreads / 32) {
+      PackedItem it;
+      const int q0 = b ? clamped(cu_q[b], 0, total_q) : 0, k0 = b ? clamped(cu_k[b], 0, total_k) : 0;
+      const int q1 = b < n ? clamped(cu_q[b + 1], q0, total_q) : total_q;
+      const int k1 = b < n ? clamped(cu_k[b + 1], k0, total_k) : total_k;
+      it.q_row = q0;
+      it.sq = (b == n && backward) ? 0 : q1 - q0;
+      it.k_row = k0;
+      it.sk = (b == n && !backward) ? 0 : k1 - k0;
+      it.pad[0] = it.pad[1] = it.pad[2] = 0;
+      const int step = backward ? 128 : 256, len = backward ? it.sk : it.sq;
+      for (int first = lane * step; first < len; first += 32 * step) {
+        it.first = first;
+        const int off = it.sk - it.sq;        // query i sees keys up to i + off
+        int cost;
+        if (backward) {
+          const int from = causal ? max(0, first - off) / 128 : 0;
+          cost = max(0, (it.sq + 127) / 128 - from);
+        } else {
+          const int last = causal ? min(it.sk, min(it.sq, first + 256) + off) : it.sk;
+          cost = max(0, last + 127) / 128;
+        }
+        f(it, kCosts - 1 - min(cost, kCosts - 1));
+      }
+    }
+  };
+  walk([&](const PackedItem&, int c) { atomicAdd(&count[c], 1); });
+  __syncthreads();
+  // exclusive sum over the costs
+  constexpr int per = kCosts / kThreads;
+  int mine[per], sum = 0;
+#pragma unroll
+  for (int i = 0; i < per; ++i) {
+    mine[i] = sum;
+    sum += count[tid * per + i];
+  }
+  int upto = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 31) part[warp] = upto;
+  __syncthreads();
+  int before = upto - sum;
+  for (int w = 0; w < warp; ++w) before += part[w];
+#pragma unroll
+  for (int i = 0; i < per; ++i) count[tid * per + i] = before + mine[i];
+  if (tid == kThreads - 1) *reinterpret_cast<int4*>(list) = make_int4(min(before + sum, cap), 0, 0, 0);
+  __syncthreads();
+  walk([&](const PackedItem& it, int c) {
+    const int at = atomicAdd(&count[c], 1);
+    if (at < cap) items[at] = it;
+  });
+}
+
+}  // namespace
+
+// Bytes of a plan for n sequences in tensors of total_q and total_k rows.
+MB_API long mb_packed_plan_bytes(int n, int total_q, int total_k) {
+  if (n < 0 || total_q < 0 || total_k < 0) return 0;
+  return packed_list_offset(total_q, total_k, n, 1, 1) + packed_list_bytes(packed_backward_items(total_k, n));
+}
+
+// cu_q, cu_k: n + 1 offsets each, in device memory; positions [total_q]: every query row's place in its sequence.  The plan (16-byte aligned) serves causal and full attention, forward
+// and backward, with any number of heads.
+MB_API int mb_packed_plan(const int* cu_q, const int* cu_k, int n, int total_q, int total_k, void* plan, int64_t* positions,
+                          cudaStream_t stream) {
+  if (n < 0 || total_q < 0 || total_k < 0 || (reinterpret_cast<uintptr_t>(plan) & 15)) return -1;
+  packed_plan_kernel<<<4 + (total_q + kThreads - 1) / kThreads, kThreads, 0, stream>>>(
+      cu_q, cu_k, n, total_q, total_k, static_cast<uint8_t*>(plan), positions);
+  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+}

@@ -866,24 +866,22 @@ def attention(q, k, v, scale: Optional[float] = None, causal: bool = True, seqle
 
 def attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k=None, scale: Optional[float] = None, causal: bool = True):
     """Attention over sequences packed back to back without padding: q ``[total_q, nh, d]``, k / v
-    ``[total_k, nh_kv, d]``, ``cu_seqlens_*`` the ``batch + 1`` cumulative lengths (a tensor or a list;
-    a tensor is read back to the host once).  Returns ``[total_q, nh, d]``.  Each sequence is one launch
-    of the ordinary kernel on a view of the packed tensors (the interface of the reference's
-    ``flash_attn_varlen`` entry points, csrc/flash_attn/flash_api.cpp ``varlen_fwd`` / ``varlen_bwd``)."""
-    cq = cu_seqlens_q.tolist() if isinstance(cu_seqlens_q, torch.Tensor) else list(cu_seqlens_q)
-    ck = cq if cu_seqlens_k is None else (
-        cu_seqlens_k.tolist() if isinstance(cu_seqlens_k, torch.Tensor) else list(cu_seqlens_k))
-    assert len(cq) == len(ck) and cq[0] == 0 and ck[0] == 0
-    outs = []
-    for i in range(len(cq) - 1):
-        qi, ki, vi = q[cq[i]:cq[i + 1]], k[ck[i]:ck[i + 1]], v[ck[i]:ck[i + 1]]
-        if qi.shape[0] == 0:
-            continue
-        if ki.shape[0] == 0:
-            outs.append(torch.zeros_like(qi))
-            continue
-        outs.append(attention(qi.unsqueeze(0), ki.unsqueeze(0), vi.unsqueeze(0), scale, causal).squeeze(0))
-    return torch.cat(outs, 0) if outs else q.new_zeros(q.shape)
+    ``[total_k, nh_kv, d]``, ``cu_seqlens_*`` the ``batch + 1`` cumulative lengths (a tensor or a list), or a
+    :class:`PackedSequences` in the place of ``cu_seqlens_q``.  One launch covers all sequences, in the forward pass and
+    in the backward pass; offsets on the device are not read back.  A causal query sees the keys up to its own place, the
+    sequences aligned at their ends.  Queries without a key, and rows behind the last sequence, give zeros.
+    Returns ``[total_q, nh, d]``, or where the offsets are known on the host as many rows as they say (the interface of the
+    reference's ``flash_attn_varlen`` entry points, csrc/flash_attn/flash_api.cpp ``varlen_fwd`` / ``varlen_bwd``)."""
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k, scale, causal)
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    if isinstance(cu_seqlens_q, PackedSequences):
+        return packed_attention.attention(q, k, v, cu_seqlens_q, scale, causal)
+    seqs = PackedSequences(cu_seqlens_q, q.shape[0], cu_seqlens_k, k.shape[0], device=q.device)
+    out = packed_attention.attention(q, k, v, seqs, scale, causal)
+    return out if seqs.host_q is None or seqs.host_q[-1] == q.shape[0] else out[:seqs.host_q[-1]]
 
 
 class _PackedAttnFn(torch.autograd.Function):
@@ -895,17 +893,22 @@ class _PackedAttnFn(torch.autograd.Function):
     produced as one packed tensor, so autograd never splits or re-concatenates q/k/v."""
 
     @staticmethod
-    def forward(ctx, qkv, cos, sin, rot, scale, causal, kv_heads, seqlens):
-        ctx.kv_heads, ctx.seqlens, ctx.shape = kv_heads, seqlens, qkv.shape
+    def forward(ctx, qkv, cos, sin, rot, scale, causal, kv_heads, seqlens, packed):
+        ctx.kv_heads, ctx.seqlens, ctx.shape, ctx.packed = kv_heads, seqlens, qkv.shape, packed
         if qkv.dim() == 5:
             qkv = qkv.reshape(*qkv.shape[:2], -1, qkv.shape[4])
+        if packed is not None:
+            qkv = qkv.reshape(1, -1, *qkv.shape[2:])
         if rot:
             qkv = _PackedAttnFn._rotate(qkv, cos, sin, rot, False, kv_heads)
         q, k, v = _PackedAttnFn._split(qkv, kv_heads)
-        o, lse = attn_fwd(q, k, v, scale, causal, seqlens_q=seqlens, seqlens_k=seqlens)
+        if packed is not None:
+            o, lse = packed_attention.forward(q[0], k[0], v[0], packed, scale, causal)
+        else:
+            o, lse = attn_fwd(q, k, v, scale, causal, seqlens_q=seqlens, seqlens_k=seqlens)
         ctx.rot, ctx.scale, ctx.causal = rot, scale, causal
         ctx.save_for_backward(qkv, o, lse, cos, sin)
-        return o
+        return o if packed is None else o.view(*ctx.shape[:2], *o.shape[1:])
 
     @staticmethod
     def _split(qkv, nkv):
@@ -928,11 +931,16 @@ class _PackedAttnFn(torch.autograd.Function):
         qkv, o, lse, cos, sin = ctx.saved_tensors
         from . import attention_bwd
         dqkv = torch.empty_like(qkv)
-        attention_bwd.backward(dout, *_PackedAttnFn._split(qkv, ctx.kv_heads), o, lse, ctx.scale, ctx.causal,
-                               out=_PackedAttnFn._split(dqkv, ctx.kv_heads), seqlens=(ctx.seqlens, ctx.seqlens))
+        if ctx.packed is not None:
+            q, k, v, dq, dk, dv = (t[0] for x in (qkv, dqkv) for t in _PackedAttnFn._split(x, ctx.kv_heads))
+            packed_attention.backward(dout.reshape(o.shape), q, k, v, o, lse, ctx.packed, ctx.scale, ctx.causal,
+                                      out=(dq, dk, dv))
+        else:
+            attention_bwd.backward(dout, *_PackedAttnFn._split(qkv, ctx.kv_heads), o, lse, ctx.scale, ctx.causal,
+                                   out=_PackedAttnFn._split(dqkv, ctx.kv_heads), seqlens=(ctx.seqlens, ctx.seqlens))
         if ctx.rot:
             dqkv = _PackedAttnFn._rotate(dqkv, cos, sin, ctx.rot, True, ctx.kv_heads)
-        return dqkv.view(ctx.shape), None, None, None, None, None, None, None
+        return dqkv.view(ctx.shape), None, None, None, None, None, None, None, None
 
 
 class _KVPackedAttnFn(torch.autograd.Function):
@@ -955,12 +963,30 @@ class _KVPackedAttnFn(torch.autograd.Function):
         return dq, dkv, None, None, None, None
 
 
-def attention_projected(qkv, kv_heads: int, scale: float, causal: bool, rotary=None, seqlens=None):
+def attention_projected(qkv, kv_heads: int, scale: float, causal: bool, rotary=None, seqlens=None, packed=None):
     """Self attention on a projection output ``[b, s, q heads + 2 * kv_heads, d]`` or ``[b, s, 3, kv_heads, d]``, the
     gradient packed the same way.
-    ``seqlens``: as in :func:`attention`; ``rotary``: ``(cos, sin, rot_dim)``, rotated in place on the device."""
+    ``seqlens``: as in :func:`attention`; ``rotary``: ``(cos, sin, rot_dim)``, rotated in place on the device.
+    ``packed``: a :class:`PackedSequences` of the ``b * s`` tokens, each of which attends inside its sequence (then the
+    tables of ``rotary`` have a row for every token: :meth:`PackedSequences.rotary`)."""
     cos, sin, rot = rotary if rotary is not None else (None, None, 0)
-    return _PackedAttnFn.apply(qkv, cos, sin, int(rot), float(scale), bool(causal), int(kv_heads), seqlens)
+    if packed is not None:
+        if _elsewhere(qkv):
+            with torch.cuda.device(qkv.device):
+                return attention_projected(qkv, kv_heads, scale, causal, rotary, seqlens, packed)
+        if seqlens is not None:
+            raise ValueError("packed sequences have no padding: seqlens cannot be given beside them")
+        rows, heads = qkv.flatten(0, 1), qkv.numel() // max(qkv.shape[0] * qkv.shape[1] * qkv.shape[-1], 1)
+        packed.check(rows, rows)
+        if not packed.same or (qkv.numel() and (heads <= 2 * kv_heads or (heads - 2 * kv_heads) % kv_heads)):
+            raise ValueError(f"self attention of {heads} heads in all, {kv_heads} of them for keys, over one packing expected")
+        if use_native(qkv):
+            packed_attention.check_kernel_types(qkv)
+            if not qkv.is_contiguous() or ptr(qkv) % 16:
+                if rot:
+                    raise ValueError("the rotation in place needs a contiguous projection output")
+                qkv = qkv.clone(memory_format=torch.contiguous_format)
+    return _PackedAttnFn.apply(qkv, cos, sin, int(rot), float(scale), bool(causal), int(kv_heads), seqlens, packed)
 
 
 def attention_kvpacked(q, kv, scale: float, causal: bool, seqlens_q=None, seqlens_k=None):
@@ -1272,4 +1298,6 @@ def accumulate_grad(src_bf16, dst, scale: float = 1.0, accumulate: bool = True):
     return dst
 
 
+from . import packed as packed_attention  # noqa: E402
 from .linear_xent import linear_cross_entropy  # noqa: E402,F401  (needs the functions above)
+from .packed import PackedSequences  # noqa: E402
