@@ -173,7 +173,8 @@ class TrainingSession:
         if self.G == 1:
             batches = [dict(batch)]
         else:
-            parts = {k: v.chunk(self.G) for k, v in batch.items()}
+            # (a list or tuple holds one value per micro batch: the packings of batches of packed sequences)
+            parts = {k: v if isinstance(v, (list, tuple)) else v.chunk(self.G) for k, v in batch.items()}
             batches = [{k: parts[k][i] for k in batch} for i in range(self.G)]
         if self.pipeline is not None:
             return self.pipeline.train_step(batches)

@@ -6,7 +6,7 @@ import torch
 import torch.nn as nn
 
 from ..config import AttnMaskType, ModelConfig
-from ..modules.layers import get_norm, vocab_parallel_cross_entropy
+from ..modules.layers import get_norm, linear_vocab_parallel_cross_entropy, vocab_parallel_cross_entropy
 from ..ops import functional as F
 from ..parallel import dist_ops
 from .language_model import TransformerLanguageModel
@@ -25,10 +25,13 @@ class BertLMHead(nn.Module):
             nn.init.normal_(self.dense.weight, std=0.02)
             nn.init.zeros_(self.dense.bias)
 
-    def forward(self, hidden, word_embeddings_weight):
+    def forward(self, hidden, word_embeddings_weight, labels=None):
+        """Logits, or with ``labels`` the loss of every token, the logits never held."""
         x = F.linear(hidden, self.dense.weight, self.dense.bias, activation="gelu")
         x = self.norm(x)
         x = dist_ops.copy_to_group(x, self.process_group)
+        if labels is not None:
+            return linear_vocab_parallel_cross_entropy(x, word_embeddings_weight, labels, self.process_group, self.bias)
         return F.linear(x, word_embeddings_weight, self.bias)
 
 
@@ -95,12 +98,13 @@ class BertModel(nn.Module):
                 input_ids.shape[0], -1, hidden.shape[-1])
         wte = (self.language_model.embedding.word_embeddings.weight if self.pre_process
                else self.word_embeddings.weight)
-        logits = self.lm_head(hidden, wte)
+        fused = self.cfg.fused_lm_loss and lm_labels is not None and not F._sym(hidden)
+        logits = None if fused else self.lm_head(hidden, wte)
         binary_logits = self.binary_head(pooled) if (self.add_binary_head and pooled is not None) else None
         if lm_labels is None:
             return logits, binary_logits
-        loss = vocab_parallel_cross_entropy(logits.reshape(-1, logits.shape[-1]), lm_labels.reshape(-1),
-                                            self.language_model.pre_post_process_group).mean()
+        loss = self.lm_head(hidden, wte, lm_labels).mean() if fused else vocab_parallel_cross_entropy(
+            logits.reshape(-1, logits.shape[-1]), lm_labels.reshape(-1), self.language_model.pre_post_process_group).mean()
         if binary_logits is not None and sentence_order is not None:
             loss = loss + torch.nn.functional.cross_entropy(binary_logits.float(), sentence_order)
         return loss

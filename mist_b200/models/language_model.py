@@ -11,7 +11,8 @@ import torch
 import torch.nn as nn
 
 from ..config import ModelConfig, PositionEmbeddingType
-from ..modules.layers import ColumnParallelLinear, PaddingMask, VocabParallelEmbedding, vocab_parallel_cross_entropy
+from ..modules.layers import (ColumnParallelLinear, PaddingMask, VocabParallelEmbedding,
+                              linear_vocab_parallel_cross_entropy, vocab_parallel_cross_entropy)
 from ..ops import functional as F
 from ..parallel import dist_ops
 from .transformer import ParallelTransformer
@@ -95,13 +96,20 @@ class TransformerLanguageModel(nn.Module):
                 dec_attn_mask=None, enc_dec_attn_mask=None):
         """``enc_attn_mask`` / ``dec_attn_mask``: ``[batch, seq]`` key-padding masks (non-zero = real
         token) of the encoder / decoder tokens; ``enc_dec_attn_mask``: mask of the encoder tokens as
-        cross attention sees them (defaults to ``enc_attn_mask``).  Masks without padding are dropped."""
+        cross attention sees them (defaults to ``enc_attn_mask``).  Masks without padding are dropped.
+        A single-stack model takes a :class:`~mist_b200.ops.packed.PackedSequences` of its ``batch * seq`` tokens as
+        ``enc_attn_mask``: documents packed back to back, which attend inside themselves and whose positions start at 0."""
         bs = enc_input_ids.shape[0] if enc_input_ids is not None else None
         if enc_hidden_states is None and self.encoder is None and self.enc_hidden_input is not None:
             enc_hidden_states = self.enc_hidden_input
         enc_mask = PaddingMask.prepare(enc_attn_mask)
         dec_mask = PaddingMask.prepare(dec_attn_mask)
         cross_mask = PaddingMask.prepare(enc_dec_attn_mask) if enc_dec_attn_mask is not None else enc_mask
+        if isinstance(enc_mask, F.PackedSequences):
+            if self.decoder is not None or isinstance(dec_mask, F.PackedSequences):
+                raise NotImplementedError("packed sequences in an encoder-decoder model")
+            if enc_position_ids is None and enc_input_ids is not None:
+                enc_position_ids = enc_mask.positions.view(enc_input_ids.shape)
         if self.pre_process and self.encoder is not None:
             hidden = self.embedding(enc_input_ids, enc_position_ids, tokentype_ids)
         else:
@@ -159,22 +167,28 @@ class TransformerLanguageModel(nn.Module):
 
 
 class LMHead(nn.Module):
-    """Vocabulary projection (column parallel, no bias) + vocab-parallel cross entropy."""
+    """Vocabulary projection (column parallel, no bias) + vocab-parallel cross entropy; with ``fused_lm_loss`` the two are
+    one operator where labels are given."""
 
     def __init__(self, cfg: ModelConfig, process_group=None, sequence_parallel=False, device=None, dtype=None):
         super().__init__()
         self.process_group = process_group
+        self.fused_loss = cfg.fused_lm_loss
         self.proj = ColumnParallelLinear(cfg.hidden_size, cfg.vocab_size, process_group=process_group,
                                          bias=False, sequence_parallel=sequence_parallel, device=device,
                                          dtype=dtype or cfg.params_dtype)
 
     def forward(self, hidden, labels=None, weight=None):
-        if weight is not None:   # tied embeddings
+        fused = self.fused_loss and labels is not None and not F._sym(hidden)
+        if weight is not None or fused:   # tied embeddings
             x = hidden
             if self.proj.sequence_parallel:
                 x = dist_ops.all_gather(x.reshape(-1, x.shape[-1]), self.process_group)
             else:
                 x = dist_ops.copy_to_group(x, self.process_group)
+            if fused:
+                return linear_vocab_parallel_cross_entropy(x, self.proj.weight if weight is None else weight, labels,
+                                                           self.process_group).mean()
             logits = F.linear(x, weight)
         else:
             logits = self.proj(hidden)

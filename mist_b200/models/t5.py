@@ -6,7 +6,7 @@ import torch
 import torch.nn as nn
 
 from ..config import ModelConfig
-from ..modules.layers import vocab_parallel_cross_entropy
+from ..modules.layers import linear_vocab_parallel_cross_entropy, vocab_parallel_cross_entropy
 from ..ops import functional as F
 from ..parallel import dist_ops
 from .language_model import TransformerLanguageModel
@@ -21,11 +21,14 @@ class T5LMHead(nn.Module):
         self.sequence_parallel = sequence_parallel
         self.bias = nn.Parameter(torch.zeros(local_vocab, device=device, dtype=dtype))
 
-    def forward(self, hidden, word_embeddings_weight):
+    def forward(self, hidden, word_embeddings_weight, labels=None):
+        """Logits, or with ``labels`` the loss of every token, the logits never held."""
         if self.sequence_parallel:      # token shards -> all tokens; the backward pass reduce-scatters
             x = dist_ops.all_gather(hidden.reshape(-1, hidden.shape[-1]), self.process_group)
         else:
             x = dist_ops.copy_to_group(hidden, self.process_group)
+        if labels is not None:
+            return linear_vocab_parallel_cross_entropy(x, word_embeddings_weight, labels, self.process_group, self.bias)
         return F.linear(x, word_embeddings_weight, self.bias)
 
 
@@ -75,6 +78,8 @@ class T5Model(nn.Module):
             enc_dec_attn_mask=encoder_decoder_attn_mask)
         if not self.post_process:
             return dec_out, enc_out
+        if self.cfg.fused_lm_loss and lm_labels is not None and not F._sym(dec_out):
+            return self.lm_head(dec_out, self.language_model.embedding.word_embeddings.weight, lm_labels).mean()
         logits = self.lm_head(dec_out, self.language_model.embedding.word_embeddings.weight)
         if lm_labels is None:
             return logits

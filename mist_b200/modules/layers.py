@@ -281,9 +281,9 @@ class PaddingMask:
 
     @staticmethod
     def prepare(mask) -> Optional["PaddingMask"]:
-        """``None`` for no mask or a mask without padding; masks already prepared pass through."""
-        if mask is None:
-            return None
+        """``None`` for no mask or a mask without padding; masks already prepared, and packed sequences, pass through."""
+        if mask is None or isinstance(mask, F.PackedSequences):
+            return mask
         pm = mask if isinstance(mask, PaddingMask) else PaddingMask(mask)
         return None if pm.all_valid else pm
 
@@ -453,11 +453,32 @@ class ParallelMHA(nn.Module):
         ctx = ctx.reshape(b, s, -1)
         return self.out_proj(ctx, residual=residual)
 
+    def _forward_packed(self, x, batch_size, residual, packed):
+        """Self attention over sequences packed back to back in the ``b * s`` tokens of ``x``."""
+        if (self.cross_attn or not self.use_flash_attn or self.rotary_interleaved or self.rotary_scale_base is not None
+                or getattr(self, "inference_params", None) is not None):
+            raise NotImplementedError("packed sequences: self attention by the flash kernels, plain rotary embeddings, no cache")
+        qkv = self.Wqkv(x)
+        if qkv.dim() == 2:
+            qkv = qkv.view(batch_size, -1, qkv.shape[-1])
+        rotary = None
+        if self.rotary_emb_dim > 0:
+            rotary = packed.rotary(self.rotary_emb_dim, self.rotary_emb_base)
+            qkv = self._own(qkv)           # rotated in place
+        ctx = F.attention_projected(qkv.reshape(*qkv.shape[:2], -1, self.head_dim), self.local_heads_kv, self.softmax_scale,
+                                    self.causal, rotary, packed=packed)
+        return self.out_proj(ctx.flatten(2), residual=residual)
+
     def forward(self, x, x_kv=None, batch_size=None, residual=None, attention_mask: Optional[PaddingMask] = None,
                 kv_mask: Optional[PaddingMask] = None):
         """``x``: [b, s, h], or a [b*s/tp, h] token shard under sequence parallelism (then
         ``batch_size`` is needed to recover the sequence length).  ``attention_mask`` marks the
-        real tokens of ``x`` (queries, and keys too in self attention); ``kv_mask`` those of ``x_kv``."""
+        real tokens of ``x`` (queries, and keys too in self attention), or is the
+        :class:`~mist_b200.ops.packed.PackedSequences` that its tokens are made of; ``kv_mask`` marks those of ``x_kv``."""
+        if isinstance(kv_mask, F.PackedSequences):
+            raise NotImplementedError("packed sequences as the keys of cross attention")
+        if isinstance(attention_mask, F.PackedSequences):
+            return self._forward_packed(x, batch_size, residual, attention_mask)
         if getattr(self, "inference_params", None) is not None:
             return self._forward_cached(x, residual)
         masked = attention_mask is not None or kv_mask is not None
@@ -676,3 +697,13 @@ def vocab_parallel_cross_entropy(logits, labels, process_group=None, ignore_inde
     mean_log_prob = sum_logits / K - (lmax + sum_exp.log())
     smooth = (1.0 - s) * loss - s * mean_log_prob
     return torch.where(labels.reshape(-1) == ignore_index, torch.zeros_like(smooth), smooth)
+
+
+def linear_vocab_parallel_cross_entropy(x, weight, labels, process_group=None, bias=None, ignore_index=-100):
+    """Per-token loss of the logits ``x @ weight.T + bias`` against global labels, the logits never held; ``weight`` and
+    ``bias`` are this rank's slice of the vocabulary, ``x`` (``[tokens, hidden]``) is the same on every rank."""
+    ws = group_size(process_group)
+    group = None if (ws == 1 or isinstance(process_group, dist_ops.FakeGroup)) else process_group
+    return F.linear_cross_entropy(x.reshape(-1, x.shape[-1]), weight, labels.reshape(-1), bias,
+                                  vocab_start=group_rank(process_group) * weight.shape[0], group=group,
+                                  ignore_index=ignore_index)
