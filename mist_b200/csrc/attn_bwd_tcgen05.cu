@@ -425,10 +425,12 @@ constexpr int kDeltaRows = 4;
 __host__ __device__ inline unsigned delta_first_row(unsigned block, unsigned thread) {
   return (block * 16u + (thread >> 4)) * kDeltaRows;
 }
+// `claimed`, where given, is set to 0 on the way.
 __global__ void __launch_bounds__(256)
 attn_delta_kernel(const __nv_bfloat16* __restrict__ dout, const __nv_bfloat16* __restrict__ o,
                   float* __restrict__ delta, int batch, int sq, int nh, int d, long do_bs,
-                  long do_ts, long do_hs, long o_bs, long o_ts, long o_hs) {
+                  long do_ts, long do_hs, long o_bs, long o_ts, long o_hs, int* claimed) {
+  if (claimed && blockIdx.x == 0 && threadIdx.x == 0) *claimed = 0;
   const unsigned first = delta_first_row(blockIdx.x, threadIdx.x);
   const int sub = threadIdx.x & 15;
   const unsigned total = static_cast<unsigned>(batch) * sq * nh;
@@ -599,7 +601,7 @@ MB_API int mb_attn_bwd(const void* dout, const void* q, const void* k, const voi
     long blocks = (rows + 16 * kDeltaRows - 1) / (16 * kDeltaRows);
     attn_delta_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
         reinterpret_cast<const __nv_bfloat16*>(dout), reinterpret_cast<const __nv_bfloat16*>(o), delta, batch, sq,
-        nh, d, o_bs, o_ts, d, o_bs, o_ts, d);
+        nh, d, o_bs, o_ts, d, o_bs, o_ts, d, nullptr);
   }
   if (cudaMemsetAsync(dq_acc, 0, sizeof(float) * batch * nh * static_cast<size_t>(sq) * d, stream) != cudaSuccess)
     return -4;
@@ -670,10 +672,10 @@ MB_API int mb_attn_bwd(const void* dout, const void* q, const void* k, const voi
 }
 
 // Backward pass of mb_attn_fwd_packed: dout, o [total_q][nh][d] contiguous, delta [nh][total_q] and dq_acc [nh][total_q][d]
-// fp32 scratch (dq_acc zeroed by this call), dq [total_q][nh][d], dk / dv [total_k][nh / unit_heads][d] with element strides
+// fp32 scratch (dq_acc and the int `claimed` zeroed by this call), dq [total_q][nh][d], dk / dv [total_k][nh / unit_heads][d] with element strides
 // of rows and heads.  Rows that belong to no sequence get zeros.
 MB_API int mb_attn_bwd_packed(const void* dout, const void* q, const void* k, const void* v, const void* o, const float* lse,
-                              float* delta, float* dq_acc, void* dq, void* dk, void* dv, const void* plan, int n, int total_q,
+                              float* delta, float* dq_acc, int* claimed, void* dq, void* dk, void* dv, const void* plan, int n, int total_q,
                               int total_k, int nh, int nh_kv, int unit_heads, int d, long q_ts, long q_hs, long k_ts, long k_hs,
                               long v_ts, long v_hs, long dq_ts, long dq_hs, long dk_ts, long dk_hs, long dv_ts, long dv_hs,
                               float scale, int causal, cudaStream_t stream) {
@@ -691,9 +693,10 @@ MB_API int mb_attn_bwd_packed(const void* dout, const void* q, const void* k, co
   if (total_q > 0) {
     attn_delta_kernel<<<static_cast<unsigned>((rows + 16 * kDeltaRows - 1) / (16 * kDeltaRows)), 256, 0, stream>>>(
         reinterpret_cast<const __nv_bfloat16*>(dout), reinterpret_cast<const __nv_bfloat16*>(o), delta, 1, total_q, nh, d,
-        rows * d, static_cast<long>(nh) * d, d, rows * d, static_cast<long>(nh) * d, d);
+        rows * d, static_cast<long>(nh) * d, d, rows * d, static_cast<long>(nh) * d, d, claimed);
     if (cudaMemsetAsync(dq_acc, 0, sizeof(float) * rows * static_cast<size_t>(d), stream) != cudaSuccess) return -4;
   }
+  if (total_q == 0 && cudaMemsetAsync(claimed, 0, sizeof(int), stream) != cudaSuccess) return -4;
   if (total_k > 0) {
     const bool queries = total_q > 0;      // none: maps over the keys stand in, no item loads through them
     CUtensorMap tq, tk, tv, tdo, tdq;
@@ -726,6 +729,7 @@ MB_API int mb_attn_bwd_packed(const void* dout, const void* q, const void* k, co
     const uint8_t* list = static_cast<const uint8_t*>(plan) + packed_list_offset(total_q, total_k, n, 1, causal != 0);
     p.count = reinterpret_cast<const int*>(list);
     p.items = reinterpret_cast<const PackedItem*>(list + 16);
+    p.claimed = claimed;
     const auto kern = d > 80 ? wide::attn_bwd_wide_kernel<true, true> : wide::attn_bwd_wide_kernel<false, true>;
     int dev = 0;
     static bool cfg[64][2] = {};

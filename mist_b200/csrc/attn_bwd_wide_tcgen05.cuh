@@ -33,8 +33,11 @@
 //   dq_full, dq_empty  MMA <-> dQ warps   dQ is complete / is in registers
 //   fin_full           MMA -> softmax     one phase per work item: dV, dK are complete
 //   vec_full/vec_empty[2]                 LSE and delta of the block's queries
-//   k_cut, q_cut[2], do_cut               packed sequences: a tile that ends inside, before warp 23 zeroes its rows behind
-//                                         the end and passes it on as k_full, q_full, do_full
+//   k_cut, q_cut[2], v_cut, do_cut        packed sequences: a tile that ends inside has arrived; S^T uses K and Q as they
+//                                         are, warp 23 zeroes the rows between the end and the next multiple of 16 and
+//                                         passes the tile on as k_full, q_full, v_full, do_full; the products over keys and
+//                                         over queries stop there.  (Masking dS^T instead of zeroing V cost 15 - 20 % of
+//                                         all blocks: 32 heads of 64, 2 x 4096 tokens 598 us against 514.)
 #pragma once
 
 namespace wide {
@@ -46,14 +49,16 @@ constexpr int kDqChunk = BB * 128;        // [128 q][32 fp32]
 constexpr int oK = 0, oV = kTile, oQ = 2 * kTile, oDO = 4 * kTile, oDS = 5 * kTile, oDQ = 6 * kTile;
 constexpr int oVec = oDQ + 2 * kDqChunk;  // -LSE*log2(e) and -delta of two query blocks
 constexpr int oBar = oVec + 2 * 2 * BB * 4;
-constexpr int kNumBars = 4 + 4 + 2 + 2 + 1 + 2 + 2 + 1 + 4 + 4;
-constexpr int kSmem = oBar + kNumBars * 8 + 16;
+constexpr int kNumBars = 4 + 4 + 2 + 2 + 1 + 2 + 2 + 1 + 4 + 5;
+constexpr int oItems = (oBar + kNumBars * 8 + 16 + 15) / 16 * 16;      // packed sequences: items of this CTA
+constexpr int kSmem = oItems + ItemRing::kBytes;
 static_assert(kSmem <= 232448, "attention backward: shared memory over the per-CTA limit");
 
 // Sequences packed back to back: sq and sk are all rows, batch is 1, the items of a plan take the place of key blocks.
 struct PackedParams : BwdParams {
   const int* count;          // number of items
   const PackedItem* items;
+  int* claimed;              // items that were claimed beyond the first of each CTA
 };
 template <bool PACKED>
 using ParamsOf = std::conditional_t<PACKED, PackedParams, BwdParams>;
@@ -89,21 +94,15 @@ __device__ __forceinline__ void fill_blocks(Work& w, int kv0, bool causal, int u
   w.n_iter = w.per_head * unit_heads;
 }
 
-__device__ __forceinline__ Work work_at(const PackedParams& p, const Sched& s, int t) {
+__device__ __forceinline__ Work work_of(const int4& a, const int4& b, bool causal, int unit_heads) {
   Work w;
-  const int per_group = s.group * s.nblk;
-  const int g = t / per_group, r = t - g * per_group;
-  const int gsize = min(s.group, s.bu - g * s.group);
-  const int at = r / gsize;
-  w.unit = g * s.group + (r - at * gsize);
-  w.batch = 0;
-  const int4 a = *reinterpret_cast<const int4*>(&p.items[at]);
-  const int first = p.items[at].first;
   w.q_row = a.x;
   w.sq_b = a.y;
   w.k_row = a.z;
   w.sk_b = a.w;
-  fill_blocks(w, first, p.causal, s.unit_heads);
+  w.unit = b.y;
+  w.batch = 0;
+  fill_blocks(w, b.x, causal, unit_heads);
   return w;
 }
 
@@ -145,7 +144,7 @@ template <bool kAlias, bool PACKED>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
-                     const __grid_constant__ CUtensorMap tm_dq, const ParamsOf<PACKED> p, const Sched dealt) {
+                     const __grid_constant__ CUtensorMap tm_dq, const ParamsOf<PACKED> p, const Sched sch) {
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + oBar);
   uint64_t* k_full = bars;
@@ -169,7 +168,9 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   uint64_t* k_cut = bars + 22;
   uint64_t* q_cut = bars + 23;
   uint64_t* do_cut = bars + 25;
+  uint64_t* v_cut = bars + 26;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kNumBars);
+  const ItemRing ring(smem + oItems);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -183,6 +184,7 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       const uint64_t* b = bars + i;
       mbar_init(bars + i, (b == p_full || b == ds_full || (b >= vec_empty && b < k_cut)) ? 16 : (b == dq_empty ? 4 : 1));   // warps
     }
+    if (PACKED) ring.init(23);
     fence_barrier_init();
     prefetch_tmap(&tm_q);
     prefetch_tmap(&tm_k);
@@ -202,11 +204,19 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   const uint32_t t_dq = kAlias ? t_dp : tmem_base + 256;
   const uint32_t t_dv = tmem_base + (kAlias ? 256 : 336), t_dk = tmem_base + (kAlias ? 384 : 416);
   constexpr uint32_t kChunk = BB * 128;
-  Sched sch = dealt;
-  if constexpr (PACKED) {
-    sch.nblk = *p.count;
-    sch.total = sch.nblk * sch.bu;
-  }
+  // Item r of this CTA, for a warp; false behind the last.
+  auto next_item = [&](int r, Work& w) -> bool {
+    if constexpr (PACKED) {
+      int4 a, b;
+      if (!ring.take<true>(r, a, b)) return false;
+      w = work_of(a, b, p.causal, sch.unit_heads);
+    } else {
+      const int t = work_index(r);
+      if (t >= sch.total) return false;
+      w = work_at(p, sch, t);
+    }
+    return true;
+  };
 
   // Registers: 768 threads were launched with 80 each; 512 * 64 + 128 * 160 + 128 * 64 is the same sum.
   if (warp >= 20) {
@@ -228,21 +238,38 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           mbar_expect_tx(bar, p.nchunks * kChunk);
           for (int c = 0; c < p.nchunks; ++c) tma_load_4d(smem + off + c * kChunk, tm, bar, 64 * c, head, row, batch);
         };
+        int count = 0;
+        if constexpr (PACKED) count = *p.count;
         for (int r = 0; ok; ++r) {
-          const int t = work_index(r);
-          if (t >= sch.total) break;
-          const Work w = work_at(p, sch, t);
+          Work w;
+          if constexpr (PACKED) {
+            int4 a, b;
+            if (!ring.claim(r, p.claimed, p.items, count, sch.bu, sch.group, a, b, ok)) {
+              if (!ok) report(p.status, MB_ERR_TIMEOUT_EMPTY);
+              break;
+            }
+            w = work_of(a, b, p.causal, sch.unit_heads);
+          } else {
+            const int t = work_index(r);
+            if (t >= sch.total) break;
+            w = work_at(p, sch, t);
+          }
           if (w.n_iter == 0) continue;
           const int head0 = w.unit * sch.unit_heads, head_kv = head0 / (p.nh / p.nh_kv);
           const int kv0 = w.k_row + w.kv0;
-          load(oK, &tm_k, k_full, k_empty, items, head_kv, kv0, w.batch, w.kv0 + BB > w.sk_b ? k_cut : nullptr);
+          auto load_k = [&]() {
+            load(oK, &tm_k, k_full, k_empty, items, head_kv, kv0, w.batch, w.kv0 + BB > w.sk_b ? k_cut : nullptr);
+          };
+          if (!PACKED) load_k();
           int hh = 0, i = 0;
           for (int it = 0; it < w.n_iter && ok; ++it) {
             const int st = n & 1, q0 = w.q_row + (w.i_start + i) * BB;
             const bool cut = i == w.per_head - 1 && q0 + BB > w.q_row + w.sq_b;
             load(oQ + st * kTile, &tm_q, &q_full[st], &q_empty[st], n >> 1, head0 + hh, q0, w.batch, cut ? &q_cut[st] : nullptr);
-            if (it == 0) load(oV, &tm_v, v_full, v_empty, items, head_kv, kv0, w.batch, nullptr);
+            if (it == 0) load(oV, &tm_v, v_full, v_empty, items, head_kv, kv0, w.batch, w.kv0 + BB > w.sk_b ? v_cut : nullptr);
             load(oDO, &tm_do, do_full, do_empty, n, head0 + hh, q0, w.batch, cut ? do_cut : nullptr);
+            // K's place is the last to become free: behind it, the other tiles of a short item would arrive late
+            if (PACKED && it == 0) load_k();
             ++n;
             if (++i == w.per_head) { i = 0; ++hh; }
           }
@@ -253,8 +280,9 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       // ------------------- rows behind the last key of K and behind the last query of Q and dO
       // They belong to the next sequence.  Their probabilities are 0, but 0 times an infinity is not.
       int n = 0;
-      uint32_t uses = 0;                   // parities: bit 0 K, 1 and 2 Q, 3 dO
+      uint32_t uses = 0;                   // parities: bit 0 K, 1 and 2 Q, 3 dO, 4 V
       bool ok = true;
+      // products over these rows go on to the next multiple of 16
       auto zero_rows = [&](int off, int from, uint64_t* cut, uint64_t* full, int bit) {
         if (!ok) return;
         if (!mbar_wait(cut, (uses >> bit) & 1)) {
@@ -263,23 +291,31 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           return;
         }
         uses ^= 1u << bit;
-        for (int at = from * 128 + lane * 16; at < static_cast<int>(kChunk); at += 512)
+        for (int at = from * 128 + lane * 16; at < ((from + 15) & ~15) * 128; at += 512)
           for (int c = 0; c < p.nchunks; ++c)
             *reinterpret_cast<uint4*>(smem + off + c * kChunk + at) = make_uint4(0, 0, 0, 0);
         fence_async_smem();
         mbar_arrive_warp(full);
       };
       for (int r = 0; ok; ++r) {
-        const int t = work_index(r);
-        if (t >= sch.total) break;
-        const Work w = work_at(p, sch, t);
+        Work w;
+        if (!next_item(r, w)) break;
         if (w.n_iter == 0) continue;
-        if (w.kv0 + BB > w.sk_b) zero_rows(oK, w.sk_b - w.kv0, k_cut, k_full, 0);
+        // what is needed first comes first: V and dO for dP^T, then Q and K for dK and dQ
+        const bool cut_k = w.kv0 + BB > w.sk_b;
+        if (cut_k) zero_rows(oV, w.sk_b - w.kv0, v_cut, v_full, 4);
         const int rest = w.sq_b - (w.i_start + w.per_head - 1) * BB;      // queries of the last block
+        bool k_left = cut_k;
+        if (k_left && (w.per_head > 1 || rest >= BB)) {
+          zero_rows(oK, w.sk_b - w.kv0, k_cut, k_full, 0);
+          k_left = false;
+        }
         for (int hh = 0; hh < sch.unit_heads && rest < BB && ok; ++hh) {
           const int st = (n + (hh + 1) * w.per_head - 1) & 1;
-          zero_rows(oQ + st * kTile, rest, &q_cut[st], &q_full[st], 1 + st);
           zero_rows(oDO, rest, do_cut, do_full, 3);
+          zero_rows(oQ + st * kTile, rest, &q_cut[st], &q_full[st], 1 + st);
+          if (k_left) zero_rows(oK, w.sk_b - w.kv0, k_cut, k_full, 0);
+          k_left = false;
         }
         n += w.n_iter;
       }
@@ -289,9 +325,8 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       int n = 0;
       bool ok = true;
       for (int r = 0; ok; ++r) {
-        const int t = work_index(r);
-        if (t >= sch.total) break;
-        const Work w = work_at(p, sch, t);
+        Work w;
+        if (!next_item(r, w)) break;
         int hh = 0, i = 0;
         for (int it = 0; it < w.n_iter; ++it, ++n) {
           const long row = (static_cast<long>(w.batch) * p.nh + w.unit * sch.unit_heads + hh) * p.sq + w.q_row;
@@ -343,8 +378,26 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           if (kk < ksteps) mma_f16_ss(d_tmem, da + off, db + off, idesc_s, kk != 0 ? 1u : 0u);
         }
       };
-      auto issue_s = [&](int nn) {
-        if (!wait(&q_full[nn & 1], nn >> 1, MB_ERR_TIMEOUT_FULL)) return;
+      uint32_t cuts = 0;             // parities of k_cut (bit 0) and q_cut (1, 2)
+      // a tile as it arrived, or (`cut`) before its rows behind the end are zeroed
+      auto wait_tile = [&](uint64_t* full, int phase, uint64_t* cut_bar, bool cut, int bit) -> bool {
+        if (!PACKED || !cut) return wait(full, phase, MB_ERR_TIMEOUT_FULL);
+        if (!wait(cut_bar, (cuts >> bit) & 1, MB_ERR_TIMEOUT_FULL)) return false;
+        cuts ^= 1u << bit;
+        return true;
+      };
+      // 16-row steps of a product; a test in the unrolled loop cost 17 % of a block at head size 64
+      auto steps = [&](int count, auto&& product) {
+        if (!PACKED || count == BB / 16) {
+#pragma unroll
+          for (int kk = 0; kk < BB / 16; ++kk) product(kk);
+        } else {
+#pragma unroll 1
+          for (int kk = 0; kk < count; ++kk) product(kk);
+        }
+      };
+      auto issue_s = [&](int nn, bool cut) {
+        if (!wait_tile(&q_full[nn & 1], nn >> 1, &q_cut[nn & 1], cut, 1 + (nn & 1))) return;
         tc_fence_after();
         if (elect_one()) {
           product_kk(t_s, base + oK, base + oQ + (nn & 1) * kTile);
@@ -366,45 +419,56 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         __syncwarp();
       };
       for (int r = 0; ok; ++r) {
-        const int t = work_index(r);
-        if (t >= sch.total) break;
-        const Work w = work_at(p, sch, t);
+        Work w;
+        if (!next_item(r, w)) break;
         if (w.n_iter == 0) continue;
-        if (!wait(k_full, items, MB_ERR_TIMEOUT_FULL)) break;
-        issue_s(n);
+        const bool cut_k = PACKED && w.kv0 + BB > w.sk_b;
+        // whether the queries end inside a block: the last one of each head
+        const bool cut_q = PACKED && (w.i_start + w.per_head) * BB > w.sq_b;
+        int left = w.per_head;                        // blocks of the head, this one included
+        if (!wait_tile(k_full, items, k_cut, cut_k, 0)) break;
+        issue_s(n, cut_q && left == 1);
         if (!wait(v_full, items, MB_ERR_TIMEOUT_FULL)) break;
         issue_dp(n, w.n_iter == 1);
         for (int it = 0; it < w.n_iter && ok; ++it, ++n) {
           const bool next = it + 1 < w.n_iter;
+          const bool cut = cut_q && left == 1;
+          // 16-row steps of the products over this block's queries and over the keys
+          const int q_steps = cut ? (w.sq_b - (w.i_start + w.per_head - 1) * BB + 15) / 16 : BB / 16;
+          const int k_steps = cut_k ? (w.sk_b - w.kv0 + 15) / 16 : BB / 16;
+          if (--left == 0) left = w.per_head;
+          const bool cut_next = cut_q && left == 1;
           if (!wait(p_full, n, MB_ERR_TIMEOUT_TMEM)) break;
           tc_fence_after();
           if (elect_one()) {
             const uint64_t d_do = make_smem_desc_sw128(base + oDO, kChunk, 1024);
-#pragma unroll
-            for (int kk = 0; kk < BB / 16; ++kk)
-              // P^T of query columns 32 w ... lies over the first half of those S^T columns
+            // P^T of query columns 32 w ... lies over the first half of those S^T columns
+            steps(q_steps, [&](int kk) {
               mma_f16_ts(t_dv, t_s + (kk >> 1) * 32 + (kk & 1) * 8, d_do + kk * (2048 >> 4), idesc_dkv, (it | kk) != 0);
+            });
             mma_commit(do_empty);
           }
           __syncwarp();
-          if (next) issue_s(n + 1);
+          if (next) issue_s(n + 1, cut_next);
           if (!wait(ds_full, n, MB_ERR_TIMEOUT_TMEM)) break;
+          if (cut && !wait(&q_full[n & 1], n >> 1, MB_ERR_TIMEOUT_FULL)) break;
+          if (cut_k && it == 0 && !wait(k_full, items, MB_ERR_TIMEOUT_FULL)) break;
           tc_fence_after();
           auto issue_dk = [&]() {
             const uint64_t d_ds_k = make_smem_desc_sw128(base + oDS, 16, 1024);
             const uint64_t d_q_mn = make_smem_desc_sw128(base + oQ + (n & 1) * kTile, kChunk, 1024);
-#pragma unroll
-            for (int kk = 0; kk < BB / 16; ++kk)
+            steps(q_steps, [&](int kk) {
               mma_f16_ss(t_dk, d_ds_k + (((kk >> 2) * kChunk + (kk & 3) * 32) >> 4), d_q_mn + kk * (2048 >> 4), idesc_dkv,
                          (it | kk) != 0);
+            });
             mma_commit(&q_empty[n & 1]);
           };
           auto issue_dq = [&]() {
             const uint64_t d_ds_mn = make_smem_desc_sw128(base + oDS, kChunk, 1024);
             const uint64_t d_k_mn = make_smem_desc_sw128(base + oK, kChunk, 1024);
-#pragma unroll
-            for (int kk = 0; kk < BB / 16; ++kk)
+            steps(k_steps, [&](int kk) {
               mma_f16_ss(t_dq, d_ds_mn + kk * (2048 >> 4), d_k_mn + kk * (2048 >> 4), idesc_dq, kk != 0);
+            });
             mma_commit(dq_full);
             if (!next) mma_commit(k_empty);
           };
@@ -446,9 +510,8 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     int n = 0, buf = 0;
     bool ok = true;
     for (int rnd = 0; ok; ++rnd) {
-      const int t = work_index(rnd);
-      if (t >= sch.total) break;
-      const Work w = work_at(p, sch, t);
+      Work w;
+      if (!next_item(rnd, w)) break;
       int hh = 0, i = 0;
       for (int it = 0; it < w.n_iter; ++it, ++n) {
         if (!mbar_wait(dq_full, n & 1)) {
@@ -511,9 +574,8 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     int n = 0, items = 0;
     bool ok = true;
     for (int rnd = 0; ok; ++rnd) {
-      const int t = work_index(rnd);
-      if (t >= sch.total) break;
-      const Work w = work_at(p, sch, t);
+      Work w;
+      if (!next_item(rnd, w)) break;
       const int kv_idx = w.kv0 + r, kv_last = w.kv0 + BB - 1;
       int i = 0;
       for (int it = 0; it < w.n_iter; ++it, ++n) {
@@ -542,8 +604,7 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           pf[c + 2] = __float_as_uint(mb::fast_exp2(xb.x));
           pf[c + 3] = __float_as_uint(mb::fast_exp2(xb.y));
         }
-        const bool masked = (q0 + BB > w.sq_b) || (kv_last >= w.sk_b) || (p.causal && kv_last > q0 + w.coff);
-        if (masked) {
+        if ((q0 + BB > w.sq_b) || (kv_last >= w.sk_b) || (p.causal && kv_last > q0 + w.coff)) {
           // visible columns of this key row: lo <= c < hi
           const int lo = p.causal ? kv_idx - w.coff - q0 - c0 : 0;
           const int hi = kv_idx < w.sk_b ? w.sq_b - q0 - c0 : 0;
@@ -583,14 +644,6 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                 mb::add_f32x2(mb::pack_f32x2(__uint_as_float(dr[c + 2]), __uint_as_float(dr[c + 3])), d2.y)));
             ds[c >> 1] = pack2(a.x, a.y);
             ds[(c >> 1) + 1] = pack2(b.x, b.y);
-          }
-          if (PACKED && masked) {      // 0 times what the rows of another sequence hold
-            const int lo = p.causal ? kv_idx - w.coff - q0 - c0 - 16 * h : 0;
-            const int hi = kv_idx < w.sk_b ? w.sq_b - q0 - c0 - 16 * h : 0;
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              if (c < lo || c >= hi) ds[c >> 1] &= (c & 1) ? 0x0000ffffu : 0xffff0000u;
-            }
           }
 #pragma unroll
           for (int g = 0; g < 2; ++g)

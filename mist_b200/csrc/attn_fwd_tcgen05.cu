@@ -48,7 +48,8 @@ constexpr int oRing = 2 * kTile;
 constexpr int oBar = oRing + kSlots * kTile;
 // q_full[2], q_empty[2], full[5], empty[5], s_full[2], p_full[2][2], o_full[2], packed sequences only: tail[5]
 constexpr int kNumBars = 2 + 2 + kSlots + kSlots + 2 + 4 + 2 + kSlots;
-constexpr int oMax = oBar + kNumBars * 8 + 16;      // [tile][half][row] maxima (and, at the end, sums)
+constexpr int oItems = (oBar + kNumBars * 8 + 16 + 15) / 16 * 16;    // packed sequences: items of this CTA
+constexpr int oMax = oItems + ItemRing::kBytes;     // [tile][half][row] maxima (and, at the end, sums)
 constexpr int kSmem = oMax + 2 * 2 * BM * 4;
 static_assert(kSmem <= 232448, "attention forward: shared memory over the per-CTA limit");
 
@@ -70,6 +71,7 @@ struct AttnParams {
 struct PackedParams : AttnParams {
   const int* count;          // number of items
   const PackedItem* items;
+  int* claimed;              // items that were claimed beyond the first of each CTA; null: there are no more
 };
 template <bool PACKED>
 using ParamsOf = std::conditional_t<PACKED, PackedParams, AttnParams>;
@@ -118,21 +120,15 @@ __device__ __forceinline__ void fill_tiles(Work& w, int first, bool causal) {
   }
 }
 
-__device__ __forceinline__ Work work_at(const PackedParams& p, const Sched& s, int t) {
+__device__ __forceinline__ Work work_of(const int4& a, const int4& b, bool causal) {
   Work w;
-  const int items = s.total / p.nh, per_group = s.group * items;
-  const int g = t / per_group, r = t - g * per_group;
-  const int gsize = min(s.group, p.nh - g * s.group);
-  const int at = r / gsize;
-  w.head = g * s.group + (r - at * gsize);
-  w.batch = 0;
-  const int4 a = *reinterpret_cast<const int4*>(&p.items[at]);
-  const int first = p.items[at].first;
   w.q_row = a.x;
   w.sq_b = a.y;
   w.k_row = a.z;
   w.sk_b = a.w;
-  fill_tiles(w, first, p.causal);
+  w.head = b.y;
+  w.batch = 0;
+  fill_tiles(w, b.x, causal);
   return w;
 }
 
@@ -169,7 +165,7 @@ __device__ __forceinline__ void store16(__nv_bfloat16* dst, const float* f, bool
 template <bool PACKED>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                    const __grid_constant__ CUtensorMap tm_v, const ParamsOf<PACKED> p, const Sched dealt) {
+                    const __grid_constant__ CUtensorMap tm_v, const ParamsOf<PACKED> p, const Sched sch) {
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + oBar);
   uint64_t* q_full = bars;
@@ -181,6 +177,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   uint64_t* o_full = p_full + 4;
   uint64_t* tail = o_full + 2;              // [slot] a V tile that ends inside, before its rows behind the end are zeroed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kNumBars);
+  const ItemRing ring(smem + oItems);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -203,6 +200,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       mbar_init(&empty[i], 1);
       if (PACKED) mbar_init(&tail[i], 1);
     }
+    if (PACKED) ring.init(19);
     fence_barrier_init();
     prefetch_tmap(&tm_q);
     prefetch_tmap(&tm_k);
@@ -217,10 +215,24 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   constexpr uint32_t kChunk = 128 * 128;
-  Sched sch = dealt;
-  if constexpr (PACKED) sch.total = *p.count * p.nh;
   // The last V tile of a sequence that ends inside it also holds rows of the next one.  Their probabilities are 0, but 0
-  // times an infinity is not: such a tile is loaded on a barrier of its own, warp 19 zeroes those rows and passes it on.
+  // times an infinity is not: P V stops at the next multiple of 16 rows, and such a tile is loaded on a barrier of its own,
+  // warp 19 zeroes the rows up to there and passes it on.
+  // Item r of this CTA for a warp (or, not WHOLE, for the one lane of it that works); false behind the last.
+  auto next_item = [&](int r, Work& w, auto whole) -> bool {
+    if constexpr (PACKED) {
+      int4 a, b;
+      if (!ring.take<decltype(whole)::value>(r, a, b)) return false;
+      w = work_of(a, b, p.causal);
+    } else {
+      const int t = work_index(r);
+      if (t >= sch.total) return false;
+      w = work_at(p, sch, t);
+    }
+    return true;
+  };
+  constexpr std::true_type kWarp{};
+  constexpr std::false_type kLane{};
   auto ends_inside = [](const Work& w) { return PACKED && w.nbmax * BN > w.sk_b; };
 
   if (warp >= 16) {
@@ -245,10 +257,20 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           ++n;
           if (++slot == kSlots) slot = 0;
         };
+        int count = 0;
+        if constexpr (PACKED) count = *p.count;
         for (int r = 0; ok; ++r) {
-          const int t = work_index(r);
-          if (t >= sch.total) break;
-          const Work w = work_at(p, sch, t);
+          Work w;
+          if constexpr (PACKED) {
+            int4 a, b;
+            if (!ring.claim(r, p.claimed, p.items, count, p.nh, sch.group, a, b, ok)) {
+              if (!ok) report(p.status, MB_ERR_TIMEOUT_EMPTY);
+              break;
+            }
+            w = work_of(a, b, p.causal);
+          } else {
+            if (!next_item(r, w, kLane)) break;
+          }
           const int head_kv = w.head / (p.nh / p.nh_kv);
           for (int j = 0; j < w.nbmax && ok; ++j) {
             load(&tm_k, w.k_row + j * BN, head_kv, w.batch, false);
@@ -262,9 +284,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         int cq[2] = {0, 0};
         bool ok = true;
         for (int r = 0; ok; ++r) {
-          const int t = work_index(r);
-          if (t >= sch.total) break;
-          const Work w = work_at(p, sch, t);
+          Work w;
+          if (!next_item(r, w, kLane)) break;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             if (w.nb[i] == 0 || !ok) continue;
@@ -287,9 +308,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       uint32_t uses = 0;         // parity of each slot's tails
       bool ok = true;
       for (int r = 0; ok; ++r) {
-        const int t = work_index(r);
-        if (t >= sch.total) break;
-        const Work w = work_at(p, sch, t);
+        Work w;
+        if (!next_item(r, w, kWarp)) break;
         n += 2 * w.nbmax;
         if (!ends_inside(w)) continue;
         const int slot = (n - 1) % kSlots;
@@ -300,7 +320,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
         uses ^= 1u << slot;
         uint8_t* v = smem + oRing + slot * kTile;
-        for (int at = (w.sk_b - (w.nbmax - 1) * BN) * 128 + lane * 16; at < static_cast<int>(kChunk); at += 512)
+        const int end = w.sk_b - (w.nbmax - 1) * BN;
+        for (int at = end * 128 + lane * 16; at < ((end + 15) & ~15) * 128; at += 512)
           for (int c = 0; c < p.nchunks; ++c) *reinterpret_cast<uint4*>(v + c * kChunk + at) = make_uint4(0, 0, 0, 0);
         fence_async_smem();
         mbar_arrive_warp(&full[slot]);
@@ -324,11 +345,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       // The next item of the list with a block to compute; nbmax = 0 at the end of the list.
       auto next_work = [&]() -> Work {
         for (;;) {
-          const int t = work_index(round++);
           Work w;
           w.nbmax = 0;
-          if (t < sch.total) w = work_at(p, sch, t);
-          if (t >= sch.total || w.nbmax > 0) return w;
+          if (!next_item(round++, w, kWarp) || w.nbmax > 0) return w;
         }
       };
       // Next slot of the ring, once it is full.
@@ -371,9 +390,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         first_s(cur, 1, at);
       }
       while (ok && cur.nbmax > 0) {
-        const Work nxt = next_work();
+        Work nxt;
+        nxt.nbmax = 0;
+        if constexpr (!PACKED) nxt = next_work();
         for (int j = 0; j < cur.nbmax && ok; ++j) {
           const bool inside = j + 1 < cur.nbmax;
+          if constexpr (PACKED) {
+            if (!inside) nxt = next_work();      // claimed behind this item's last load
+          }
           const int at_v = take_slot();
           int at_k = 0;
           if (inside || nxt.nbmax > 0) at_k = take_slot();
@@ -390,11 +414,20 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                 tc_fence_after();
                 if (elect_one()) {
                   // part 0: the first 32 keys of both halves; 16 keys are 8 columns of P and 2048 B of V
-#pragma unroll
-                  for (int u = 0; u < 4; ++u) {
-                    const int kk = 4 * (u >> 1) + 2 * part + (u & 1);
+                  auto product = [&](int kk) {
                     mma_f16_ts(t_o, t_s + 64 * (kk >> 2) + 8 * (kk & 3), dv + kk * (2048 >> 4), idesc_o,
                                (j | kk) != 0 ? 1u : 0u);
+                  };
+                  const int keys = cur.sk_b - j * BN;
+                  if (!PACKED || keys >= BN) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) product(4 * (u >> 1) + 2 * part + (u & 1));
+                  } else {
+#pragma unroll 1
+                    for (int u = 0; u < 4; ++u) {
+                      const int kk = 4 * (u >> 1) + 2 * part + (u & 1);
+                      if (kk * 16 < keys) product(kk);
+                    }
                   }
                   if (part == 1 && j == active - 1) mma_commit(&o_full[i]);
                 }
@@ -429,9 +462,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     int cs = 0, co = 0;               // S tiles and O tiles so far
     bool ok = true;
     for (int rnd = 0; ok; ++rnd) {
-      const int t = work_index(rnd);
-      if (t >= sch.total) break;
-      const Work w = work_at(p, sch, t);
+      Work w;
+      if (!next_item(rnd, w, kWarp)) break;
       const int q0 = i ? w.q0[1] : w.q0[0], nb = i ? w.nb[1] : w.nb[0];
       const int qi = q0 + r;
       const int vis = (p.causal ? min(w.sk_b - 1, qi + w.coff) : w.sk_b - 1) - 64 * h;   // last visible key of the row
@@ -679,10 +711,16 @@ MB_API int mb_attn_fwd(const void* q, const void* k, const void* v, void* o, flo
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
+// Ints of zeroed workspace of mb_attn_fwd_packed: 0 where every work item has a CTA of its own.
+MB_API int mb_attn_fwd_packed_counters(int n, int total_q, int nh) {
+  return packed_forward_items(total_q, n) * nh > 148 ? 1 : 0;
+}
+
 // Attention over sequences packed back to back: q, o [total_q][nh][d], k / v [total_k][nh_kv][d] (element strides of rows
 // and heads), lse [nh][total_q].  `plan`: what mb_packed_plan wrote for these totals and n sequences.  Rows that belong to
-// no sequence and queries that see no key get zeros and lse = -inf; what a sequence holds reaches no other.
-MB_API int mb_attn_fwd_packed(const void* q, const void* k, const void* v, void* o, float* lse, const void* plan, int n,
+// no sequence and queries that see no key get zeros and lse = -inf; what a sequence holds reaches no other.  `claimed`: one
+// int for this call alone (zeroed here), or null where mb_attn_fwd_packed_counters is 0.
+MB_API int mb_attn_fwd_packed(const void* q, const void* k, const void* v, void* o, float* lse, const void* plan, int* claimed, int n,
                               int total_q, int total_k, int nh, int nh_kv, int d, long q_ts, long q_hs, long k_ts, long k_hs,
                               long v_ts, long v_hs, long o_ts, long o_hs, float scale, int causal, cudaStream_t stream) {
   if (d % 16 || d > 128 || d < 16 || nh_kv < 1 || nh % nh_kv || n < 0 || total_q < 0 || total_k < 0) return -1;
@@ -692,7 +730,8 @@ MB_API int mb_attn_fwd_packed(const void* q, const void* k, const void* v, void*
     return -1;
   if (total_q == 0) return 0;
   const long most = packed_forward_items(total_q, n) * nh;
-  if (most > 0x3fffffff) return -1;
+  if (most > 0x3fffffff || (most > 148 && !claimed)) return -1;
+  if (claimed && cudaMemsetAsync(claimed, 0, sizeof(int), stream) != cudaSuccess) return -4;
   CUtensorMap tq, tk, tv;
   // no keys at all: maps over the queries stand in, no item loads through them
   const bool keys = total_k > 0;
@@ -718,6 +757,7 @@ MB_API int mb_attn_fwd_packed(const void* q, const void* k, const void* v, void*
   const uint8_t* list = static_cast<const uint8_t*>(plan) + packed_list_offset(total_q, total_k, n, 0, causal != 0);
   p.count = reinterpret_cast<const int*>(list);
   p.items = reinterpret_cast<const PackedItem*>(list + 16);
+  p.claimed = claimed;
   int dev = 0;
   static bool cfg[64] = {};
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -3;
@@ -729,6 +769,7 @@ MB_API int mb_attn_fwd_packed(const void* q, const void* k, const void* v, void*
   Sched sch;
   sch.npairs = 0;
   sch.bh = nh;
+  // heads whose keys and values of all sequences take about a third of L2 together, at least one key / value head
   const long kv_bytes = 4l * total_k * d;
   const long kv_heads = kv_bytes > 0 ? (40l << 20) / kv_bytes : 1;
   const long group = (kv_heads < 1 ? 1 : kv_heads) * (nh / nh_kv);

@@ -122,8 +122,11 @@ def forward(q, k, v, packed: PackedSequences, scale: float, causal: bool):
                 o[a], lse[:, a] = oi[0], li[0]
         return o, lse
     o = torch.empty(total, nh, d, dtype=q.dtype, device=q.device)
-    lse = torch.empty(nh, total, dtype=torch.float32, device=q.device)
-    call("mb_attn_fwd_packed", ptr(q), ptr(k), ptr(v), ptr(o), ptr(lse), ptr(packed.plan), packed.n, total, k.shape[0], nh,
+    lse = torch.empty(nh * total + 1, dtype=torch.float32, device=q.device)      # and the count of claimed work items
+    claimed = ptr(lse) + 4 * nh * total
+    lse = lse[:nh * total].view(nh, total)
+    call("mb_attn_fwd_packed", ptr(q), ptr(k), ptr(v), ptr(o), ptr(lse), ptr(packed.plan),
+         claimed if native.kernels().mb_attn_fwd_packed_counters(packed.n, total, nh) else 0, packed.n, total, k.shape[0], nh,
          k.shape[1], d, q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), nh * d, d, scale,
          int(causal), stream())
     return o, lse
@@ -154,10 +157,10 @@ def backward(dout, q, k, v, o, lse, packed: PackedSequences, scale: float, causa
     gk, gv = dk, dv
     if parts > 1:        # a CTA sums `unit` heads of a group; the rest is added from a copy per unit
         gk, gv = (torch.empty(k.shape[0], nkv * parts, d, dtype=q.dtype, device=q.device) for _ in range(2))
-    delta = torch.empty(nh, total, dtype=torch.float32, device=q.device)
+    delta = torch.empty(nh * total + 1, dtype=torch.float32, device=q.device)    # and the count of claimed work items
     dq_acc = torch.empty(nh, total, d, dtype=torch.float32, device=q.device)
-    call("mb_attn_bwd_packed", ptr(dout), ptr(q), ptr(k), ptr(v), ptr(o), ptr(lse), ptr(delta), ptr(dq_acc), ptr(dq), ptr(gk),
-         ptr(gv), ptr(packed.plan), packed.n, total, k.shape[0], nh, nkv, unit, d, q.stride(0), q.stride(1), k.stride(0),
+    call("mb_attn_bwd_packed", ptr(dout), ptr(q), ptr(k), ptr(v), ptr(o), ptr(lse), ptr(delta), ptr(dq_acc),
+         ptr(delta) + 4 * nh * total, ptr(dq), ptr(gk), ptr(gv), ptr(packed.plan), packed.n, total, k.shape[0], nh, nkv, unit, d, q.stride(0), q.stride(1), k.stride(0),
          k.stride(1), v.stride(0), v.stride(1), dq.stride(0), dq.stride(1), gk.stride(0), gk.stride(1), gv.stride(0),
          gv.stride(1), scale, int(causal), stream())
     if parts > 1:
