@@ -727,8 +727,8 @@ MB_API int mb_attn_bwd_packed(const void* dout, const void* q, const void* k, co
     p.seqlens_q = p.seqlens_k = nullptr;
     p.status = mb_status_device_ptr();
     const uint8_t* list = static_cast<const uint8_t*>(plan) + packed_list_offset(total_q, total_k, n, 1, causal != 0);
-    p.count = reinterpret_cast<const int*>(list);
-    p.items = reinterpret_cast<const PackedItem*>(list + 16);
+    p.list = reinterpret_cast<const PackedHeader*>(list);
+    p.items = reinterpret_cast<const PackedItem*>(p.list + 1);
     p.claimed = claimed;
     const auto kern = d > 80 ? wide::attn_bwd_wide_kernel<true, true> : wide::attn_bwd_wide_kernel<false, true>;
     int dev = 0;

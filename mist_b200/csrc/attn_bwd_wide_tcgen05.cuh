@@ -56,7 +56,7 @@ static_assert(kSmem <= 232448, "attention backward: shared memory over the per-C
 
 // Sequences packed back to back: sq and sk are all rows, batch is 1, the items of a plan take the place of key blocks.
 struct PackedParams : BwdParams {
-  const int* count;          // number of items
+  const PackedHeader* list;
   const PackedItem* items;
   int* claimed;              // items that were claimed beyond the first of each CTA
 };
@@ -238,13 +238,16 @@ attn_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           mbar_expect_tx(bar, p.nchunks * kChunk);
           for (int c = 0; c < p.nchunks; ++c) tma_load_4d(smem + off + c * kChunk, tm, bar, 64 * c, head, row, batch);
         };
-        int count = 0;
-        if constexpr (PACKED) count = *p.count;
+        int count = 0, group = 0;
+        if constexpr (PACKED) {
+          count = p.list->count;
+          group = heads_together(p.list, sch.group, sch.bu);
+        }
         for (int r = 0; ok; ++r) {
           Work w;
           if constexpr (PACKED) {
             int4 a, b;
-            if (!ring.claim(r, p.claimed, p.items, count, sch.bu, sch.group, a, b, ok)) {
+            if (!ring.claim(r, p.claimed, p.items, count, sch.bu, group, a, b, ok)) {
               if (!ok) report(p.status, MB_ERR_TIMEOUT_EMPTY);
               break;
             }

@@ -69,7 +69,7 @@ struct AttnParams {
 
 // Sequences packed back to back: sq and sk are all rows, batch is 1, the items of a plan take the place of tiles.
 struct PackedParams : AttnParams {
-  const int* count;          // number of items
+  const PackedHeader* list;
   const PackedItem* items;
   int* claimed;              // items that were claimed beyond the first of each CTA; null: there are no more
 };
@@ -257,13 +257,16 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           ++n;
           if (++slot == kSlots) slot = 0;
         };
-        int count = 0;
-        if constexpr (PACKED) count = *p.count;
+        int count = 0, group = 0;
+        if constexpr (PACKED) {
+          count = p.list->count;
+          group = heads_together(p.list, sch.group, p.nh);
+        }
         for (int r = 0; ok; ++r) {
           Work w;
           if constexpr (PACKED) {
             int4 a, b;
-            if (!ring.claim(r, p.claimed, p.items, count, p.nh, sch.group, a, b, ok)) {
+            if (!ring.claim(r, p.claimed, p.items, count, p.nh, group, a, b, ok)) {
               if (!ok) report(p.status, MB_ERR_TIMEOUT_EMPTY);
               break;
             }
@@ -755,8 +758,8 @@ MB_API int mb_attn_fwd_packed(const void* q, const void* k, const void* v, void*
   p.seqlens_k = nullptr;
   p.status = mb_status_device_ptr();
   const uint8_t* list = static_cast<const uint8_t*>(plan) + packed_list_offset(total_q, total_k, n, 0, causal != 0);
-  p.count = reinterpret_cast<const int*>(list);
-  p.items = reinterpret_cast<const PackedItem*>(list + 16);
+  p.list = reinterpret_cast<const PackedHeader*>(list);
+  p.items = reinterpret_cast<const PackedItem*>(p.list + 1);
   p.claimed = claimed;
   int dev = 0;
   static bool cfg[64] = {};

@@ -15,7 +15,7 @@ constexpr int kCosts = 8192;       // blocks of 128 a tile walks; dearer ones co
 __global__ void __launch_bounds__(kThreads)
 packed_plan_kernel(const int* cu_q, const int* cu_k, int n, int total_q, int total_k, uint8_t* plan, int64_t* positions) {
   __shared__ int count[kCosts];
-  __shared__ int part[32];
+  __shared__ int part[32], all_costs, dearest;
   if (blockIdx.x >= 4) {      // a row's place in its sequence: the last offset that is not above it
     const int row = (blockIdx.x - 4) * kThreads + threadIdx.x;
     if (row >= total_q) return;
@@ -31,9 +31,11 @@ packed_plan_kernel(const int* cu_q, const int* cu_k, int n, int total_q, int tot
   const int backward = blockIdx.x >> 1, causal = blockIdx.x & 1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* list = plan + packed_list_offset(total_q, total_k, n, backward, causal);
-  PackedItem* items = reinterpret_cast<PackedItem*>(list + 16);
+  PackedHeader* header = reinterpret_cast<PackedHeader*>(list);
+  PackedItem* items = reinterpret_cast<PackedItem*>(header + 1);
   const int cap = static_cast<int>(backward ? packed_backward_items(total_k, n) : packed_forward_items(total_q, n));
   for (int i = tid; i < kCosts; i += kThreads) count[i] = 0;
+  if (tid == 0) all_costs = dearest = 0;
   __syncthreads();
   auto clamped = [](int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); };
   auto walk = [&](auto&& f) {
@@ -63,7 +65,10 @@ packed_plan_kernel(const int* cu_q, const int* cu_k, int n, int total_q, int tot
       }
     }
   };
-  walk([&](const PackedItem&, int c) { atomicAdd(&count[c], 1); });
+  walk([&](const PackedItem&, int c) {
+    atomicAdd(&count[c], 1);
+    atomicMax(&dearest, kCosts - 1 - c);
+  });
   __syncthreads();
   // exclusive sum over the costs
   constexpr int per = kCosts / kThreads;
@@ -85,8 +90,17 @@ packed_plan_kernel(const int* cu_q, const int* cu_k, int n, int total_q, int tot
   for (int w = 0; w < warp; ++w) before += part[w];
 #pragma unroll
   for (int i = 0; i < per; ++i) count[tid * per + i] = before + mine[i];
-  if (tid == kThreads - 1) *reinterpret_cast<int4*>(list) = make_int4(min(before + sum, cap), 0, 0, 0);
+  int costs = 0;
+#pragma unroll
+  for (int i = 0; i < per; ++i) costs += ((i + 1 < per ? mine[i + 1] : sum) - mine[i]) * (kCosts - 1 - (tid * per + i));
+  if (costs) atomicAdd(&all_costs, costs);
   __syncthreads();
+  if (tid == kThreads - 1) {
+    header->count = min(before + sum, cap);
+    header->cost = all_costs;
+    header->dearest = dearest;
+    header->pad = 0;
+  }
   walk([&](const PackedItem& it, int c) {
     const int at = atomicAdd(&count[c], 1);
     if (at < cap) items[at] = it;

@@ -12,11 +12,16 @@ struct __align__(16) PackedItem {
   int pad[3];
 };
 
-// A plan in memory: four lists one behind the other, each a header of 16 bytes (the number of items first) and its items;
-// [forward, backward] x [whole sequences visible, causal].  The items of a list are ordered by cost, dearest first.
+// A plan in memory: four lists one behind the other, each a header and its items; [forward, backward] x [whole sequences
+// visible, causal].  The items of a list are ordered by cost (blocks of 128 rows that they walk), dearest first.
+struct PackedHeader {
+  int count, cost, dearest, pad;      // items, what they cost together, what the dearest costs
+};
 __host__ __device__ inline long packed_forward_items(long total_q, long n) { return total_q / 256 + n + 1; }
 __host__ __device__ inline long packed_backward_items(long total_k, long n) { return total_k / 128 + n + 1; }
-__host__ __device__ inline long packed_list_bytes(long items) { return 16 + items * static_cast<long>(sizeof(PackedItem)); }
+__host__ __device__ inline long packed_list_bytes(long items) {
+  return static_cast<long>(sizeof(PackedHeader)) + items * static_cast<long>(sizeof(PackedItem));
+}
 __host__ __device__ inline long packed_list_offset(long total_q, long total_k, long n, int backward, int causal) {
   const long f = packed_list_bytes(packed_forward_items(total_q, n)), b = packed_list_bytes(packed_backward_items(total_k, n));
   return backward ? 2 * f + causal * b : causal * f;
@@ -27,6 +32,16 @@ __host__ __device__ inline long packed_list_offset(long total_q, long total_k, l
 // over 8: backward 1262 us, forward 481 in the worst order of groups).  The thread that loads claims the next item when it
 // has issued the last load of this one, and hands it to the other warps through a ring in shared memory.  Claiming earlier
 // would tie items to CTAs that are still busy.
+
+// Heads that are walked together: those whose tensors share L2, but so many that the dearest item, with which the last group
+// begins, is no longer than the group's share of a CTA (16384 tokens in 14 documents, 8 units of 4 heads: backward 897 us in
+// groups of 1, 845 of 2, 788 of 4, 858 of 8).
+__device__ __forceinline__ int heads_together(const PackedHeader* h, int in_l2, int heads) {
+  const long cost = h->cost > 0 ? h->cost : 1;
+  const long need = (static_cast<long>(h->dearest) * gridDim.x + cost - 1) / cost;
+  return static_cast<int>(need > heads ? heads : (need > in_l2 ? need : in_l2));
+}
+
 struct ItemRing {
   static constexpr int kSlots = 4;
   static constexpr int kBytes = kSlots * 32 + 2 * kSlots * 8;
@@ -41,8 +56,8 @@ struct ItemRing {
       sm100::mbar_init(&empty[i], consumer_warps);
     }
   }
-  // Claims item r of this CTA (the first one is the CTA's index) out of items x heads, `group` heads walked together, and
-  // publishes it; by one thread.  false: the wait gave up, or there is no item; a and b are the item.
+  // Claims item r of this CTA (the first one is the CTA's index) out of items x heads and publishes it; by one thread.
+  // false: the wait gave up, or there is no item; a and b are the item.  `group` heads are walked together.
   __device__ __forceinline__ bool claim(int r, int* counter, const PackedItem* items, int count, int heads, int group, int4& a,
                                         int4& b, bool& ok) const {
     const int total = count * heads;
@@ -55,7 +70,7 @@ struct ItemRing {
       const int gsize = min(group, heads - g * group);
       const int at = rest / gsize;
       a = *reinterpret_cast<const int4*>(&items[at]);
-      b = make_int4(items[at].first, g * group + (rest - at * gsize), 1, 0);
+      b = make_int4(items[at].first, g * group + rest % gsize, 1, 0);
     }
     const int s = r % kSlots;
     if (r >= kSlots && !sm100::mbar_wait(&empty[s], (r / kSlots - 1) & 1)) {

@@ -17,7 +17,7 @@ from mist_b200.ops import native
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 BF = 2.0 ** -8
-ITEM = 32
+ITEM, HEAD = 32, 16
 
 
 def _cu(lens):
@@ -152,18 +152,19 @@ def test_a_sequence_reaches_no_other(poison, causal, d):
 def _lists(seqs):
     """(backward, causal) -> items of a plan, as the kernels read them."""
     plan, n = seqs.plan.cpu(), seqs.n
-    fwd, bwd = 16 + ITEM * (seqs.total_q // 256 + n + 1), 16 + ITEM * (seqs.total_k // 128 + n + 1)
+    fwd, bwd = HEAD + ITEM * (seqs.total_q // 256 + n + 1), HEAD + ITEM * (seqs.total_k // 128 + n + 1)
     assert plan.numel() == 2 * (fwd + bwd)
-    out = {}
+    out, heads = {}, {}
     for backward in (0, 1):
         for causal in (0, 1):
             at = 2 * fwd + causal * bwd if backward else causal * fwd
             size = bwd if backward else fwd
             words = plan[at:at + size].view(torch.int32)
             count = int(words[0])
-            assert 0 <= count <= (size - 16) // ITEM
+            assert 0 <= count <= (size - HEAD) // ITEM
             out[backward, causal] = words[4:4 + 8 * count].view(-1, 8)[:, :5].tolist()
-    return out
+            heads[backward, causal] = words[:4].tolist()
+    return out, heads
 
 
 @pytest.mark.parametrize("lens_q,lens_k,extra", [(SHORT, SHORT, 0), (EDGES, EDGES, 7), ([], [], 10), ([5000], [5000], 0),
@@ -173,7 +174,8 @@ def test_plan_covers_every_row_once(lens_q, lens_k, extra):
     tq, tk = cu_q[-1] + extra, cu_k[-1] + extra
     seqs = F.PackedSequences(torch.tensor(cu_q, device=DEV), tq, torch.tensor(cu_k, device=DEV), tk)
     assert seqs.positions.tolist() == [i for n in lens_q for i in range(n)] + list(range(extra))
-    for (backward, causal), items in _lists(seqs).items():
+    lists, heads = _lists(seqs)
+    for (backward, causal), items in lists.items():
         step, total = (128, tk) if backward else (256, tq)
         seen, costs = torch.zeros(total, dtype=torch.int32), []
         for q_row, sq, k_row, sk, first in items:
@@ -187,13 +189,14 @@ def test_plan_covers_every_row_once(lens_q, lens_k, extra):
                 costs.append(max(0, -(-(min(sk, min(sq, first + 256) + off) if causal else sk) // 128)))
         assert (seen == 1).all()
         assert costs == sorted(costs, reverse=True)
+        assert heads[backward, causal] == [len(items), sum(costs), max(costs, default=0), 0]
 
 
 @pytest.mark.parametrize("cu", [[0, 50, 20, 90], [3, 10, 200, 400], [0, -7, 60, 2 ** 31 - 1], [5, 4, 3, 2]])
 def test_plan_of_impossible_offsets_stays_inside(cu):
     total = 100
     seqs = F.PackedSequences(torch.tensor(cu, device=DEV), total)
-    for items in _lists(seqs).values():
+    for items in _lists(seqs)[0].values():
         for q_row, sq, k_row, sk, first in items:
             assert 0 <= q_row and 0 <= sq and q_row + sq <= total
             assert 0 <= k_row and 0 <= sk and k_row + sk <= total and first >= 0
