@@ -425,12 +425,23 @@ constexpr int kDeltaRows = 4;
 __host__ __device__ inline unsigned delta_first_row(unsigned block, unsigned thread) {
   return (block * 16u + (thread >> 4)) * kDeltaRows;
 }
-// `claimed`, where given, is set to 0 on the way.
+// What the backward pass of packed sequences also needs: the count of claimed work items set to 0, the fp32 dQ of tiles that
+// more than one block of keys sees set to 0, and dQ itself where no key is visible.
+struct DeltaExtras {
+  int* claimed;
+  float* dq_acc;
+  const uint8_t* single;
+  int single_bit;
+  const float* lse;
+  __nv_bfloat16* dq;
+  long dq_ts, dq_hs;
+};
+template <bool PACKED>
 __global__ void __launch_bounds__(256)
 attn_delta_kernel(const __nv_bfloat16* __restrict__ dout, const __nv_bfloat16* __restrict__ o,
                   float* __restrict__ delta, int batch, int sq, int nh, int d, long do_bs,
-                  long do_ts, long do_hs, long o_bs, long o_ts, long o_hs, int* claimed) {
-  if (claimed && blockIdx.x == 0 && threadIdx.x == 0) *claimed = 0;
+                  long do_ts, long do_hs, long o_bs, long o_ts, long o_hs, const DeltaExtras e) {
+  if (PACKED && blockIdx.x == 0 && threadIdx.x == 0) *e.claimed = 0;
   const unsigned first = delta_first_row(blockIdx.x, threadIdx.x);
   const int sub = threadIdx.x & 15;
   const unsigned total = static_cast<unsigned>(batch) * sq * nh;
@@ -459,12 +470,23 @@ attn_delta_kernel(const __nv_bfloat16* __restrict__ dout, const __nv_bfloat16* _
 #pragma unroll
     for (int m = 8; m > 0; m >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, m);
     if (sub == 0 && first + u < total) delta[at[u]] = acc;
+    if (PACKED && sub * 8 < d && first + u < total) {
+      const unsigned q = at[u] % sq, h = at[u] / sq;
+      if (!(e.single[q] & e.single_bit)) {
+        float4* dst = reinterpret_cast<float4*>(e.dq_acc + static_cast<size_t>(at[u]) * d + sub * 8);
+        dst[0] = dst[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      if (e.lse[at[u]] == -INFINITY)
+        *reinterpret_cast<uint4*>(e.dq + q * e.dq_ts + h * e.dq_hs + sub * 8) = make_uint4(0, 0, 0, 0);
+    }
   }
 }
 
-// dq[b][q][h][:] = bf16(scale * dq_acc[b][h][q][:])
+// dq[b][q][h][:] = bf16(scale * dq_acc[b][h][q][:]); PACKED: but for the rows whose `single` has the bit
+template <bool PACKED>
 __global__ void attn_convert_dq_kernel(const float* __restrict__ acc, __nv_bfloat16* __restrict__ dq, int batch,
-                                       int sq, int nh, int d, long dq_bs, long dq_ts, long dq_hs, float scale) {
+                                       int sq, int nh, int d, long dq_bs, long dq_ts, long dq_hs, float scale,
+                                       const uint8_t* single, int single_bit) {
   const int vpr = d >> 3;
   const long nvec = static_cast<long>(batch) * nh * sq * vpr;
   for (long i = static_cast<long>(blockIdx.x) * blockDim.x + threadIdx.x; i < nvec;
@@ -472,6 +494,7 @@ __global__ void attn_convert_dq_kernel(const float* __restrict__ acc, __nv_bfloa
     const int v = static_cast<int>(i % vpr);
     long t = i / vpr;
     const int q = static_cast<int>(t % sq);
+    if (PACKED && (single[q] & single_bit)) continue;
     t /= sq;
     const int h = static_cast<int>(t % nh);
     const int b = static_cast<int>(t / nh);
@@ -599,9 +622,9 @@ MB_API int mb_attn_bwd(const void* dout, const void* q, const void* k, const voi
     long rows = static_cast<long>(batch) * sq * nh;
     if (rows > 0x7fffffff) return -1;
     long blocks = (rows + 16 * kDeltaRows - 1) / (16 * kDeltaRows);
-    attn_delta_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
+    attn_delta_kernel<false><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
         reinterpret_cast<const __nv_bfloat16*>(dout), reinterpret_cast<const __nv_bfloat16*>(o), delta, batch, sq,
-        nh, d, o_bs, o_ts, d, o_bs, o_ts, d, nullptr);
+        nh, d, o_bs, o_ts, d, o_bs, o_ts, d, DeltaExtras());
   }
   if (cudaMemsetAsync(dq_acc, 0, sizeof(float) * batch * nh * static_cast<size_t>(sq) * d, stream) != cudaSuccess)
     return -4;
@@ -665,17 +688,46 @@ MB_API int mb_attn_bwd(const void* dout, const void* q, const void* k, const voi
     long nvec = static_cast<long>(batch) * nh * sq * (d / 8);
     long blocks = (nvec + 255) / 256;
     if (blocks > 148 * 16) blocks = 148 * 16;
-    attn_convert_dq_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
-        dq_acc, reinterpret_cast<__nv_bfloat16*>(dq), batch, sq, nh, d, dq_bs, dq_ts, dq_hs, pipelined ? scale : 1.f);
+    attn_convert_dq_kernel<false><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
+        dq_acc, reinterpret_cast<__nv_bfloat16*>(dq), batch, sq, nh, d, dq_bs, dq_ts, dq_hs, pipelined ? scale : 1.f, nullptr, 0);
   }
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
-// Backward pass of mb_attn_fwd_packed: dout, o [total_q][nh][d] contiguous, delta [nh][total_q] and dq_acc [nh][total_q][d]
-// fp32 scratch (dq_acc and the int `claimed` zeroed by this call), dq [total_q][nh][d], dk / dv [total_k][nh / unit_heads][d] with element strides
-// of rows and heads.  Rows that belong to no sequence get zeros.
+MB_API int mb_attn_sum_parts(const void* dk_parts, const void* dv_parts, void* dk, void* dv, int batch, int sk, int nh_kv,
+                             int parts, int d, long dk_bs, long dk_ts, long dk_hs, long dv_bs, long dv_ts, long dv_hs,
+                             cudaStream_t stream);
+
+namespace {
+// Workspace of mb_attn_bwd_packed.
+struct PackedArea {
+  size_t delta, claimed, dq_acc, parts, total;      // offsets; parts: dK, then dV, of every unit of heads
+};
+PackedArea packed_area(int total_q, int total_k, int nh, int nh_kv, int unit_heads, int d) {
+  auto up = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
+  PackedArea a;
+  const size_t rows = static_cast<size_t>(total_q) * nh;
+  a.delta = 0;
+  a.claimed = up(4 * rows);
+  a.dq_acc = a.claimed + 256;
+  a.parts = a.dq_acc + up(4 * rows * d);
+  a.total = a.parts + (nh / nh_kv > unit_heads ? 2 * up(2ul * total_k * (nh / unit_heads) * d) : 0);
+  return a;
+}
+}  // namespace
+
+// Bytes of workspace of mb_attn_bwd_packed.
+MB_API size_t mb_attn_bwd_packed_workspace(int total_q, int total_k, int nh, int nh_kv, int unit_heads, int d) {
+  if (total_q < 0 || total_k < 0 || nh_kv < 1 || unit_heads < 1 || d < 1) return 0;
+  return packed_area(total_q, total_k, nh, nh_kv, unit_heads, d).total;
+}
+
+// Backward pass of mb_attn_fwd_packed: dout, o [total_q][nh][d] contiguous, dq [total_q][nh][d], dk / dv [total_k][nh_kv][d]
+// with element strides of rows and heads.  Rows that belong to no sequence get zeros.  A CTA sums the dK, dV of unit_heads
+// query heads of a group; where a group has more, bf16 parts are added by a kernel of their own.  The workspace is for this
+// call alone, on 16 bytes.
 MB_API int mb_attn_bwd_packed(const void* dout, const void* q, const void* k, const void* v, const void* o, const float* lse,
-                              float* delta, float* dq_acc, int* claimed, void* dq, void* dk, void* dv, const void* plan, int n, int total_q,
+                              void* dq, void* dk, void* dv, const void* plan, void* workspace, int n, int total_q,
                               int total_k, int nh, int nh_kv, int unit_heads, int d, long q_ts, long q_hs, long k_ts, long k_hs,
                               long v_ts, long v_hs, long dq_ts, long dq_hs, long dk_ts, long dk_hs, long dv_ts, long dv_hs,
                               float scale, int causal, cudaStream_t stream) {
@@ -684,77 +736,99 @@ MB_API int mb_attn_bwd_packed(const void* dout, const void* q, const void* k, co
   if ((q_ts | q_hs | k_ts | k_hs | v_ts | v_hs | dq_ts | dq_hs | dk_ts | dk_hs | dv_ts | dv_hs) & 7) return -1;
   if ((reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
        reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(dq) |
-       reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv) | reinterpret_cast<uintptr_t>(dq_acc) |
+       reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv) | reinterpret_cast<uintptr_t>(workspace) |
        reinterpret_cast<uintptr_t>(plan)) & 15)
     return -1;
   const long rows = static_cast<long>(total_q) * nh, units = nh / unit_heads;
   const long most = packed_backward_items(total_k, n) * units;
   if (rows > 0x7fffffff || most > 0x3fffffff) return -1;
+  const PackedArea area = packed_area(total_q, total_k, nh, nh_kv, unit_heads, d);
+  uint8_t* at = static_cast<uint8_t*>(workspace);
+  float* delta = reinterpret_cast<float*>(at + area.delta);
+  float* dq_acc = reinterpret_cast<float*>(at + area.dq_acc);
+  int* claimed = reinterpret_cast<int*>(at + area.claimed);
   if (total_q > 0) {
-    attn_delta_kernel<<<static_cast<unsigned>((rows + 16 * kDeltaRows - 1) / (16 * kDeltaRows)), 256, 0, stream>>>(
+    DeltaExtras e;
+    e.claimed = claimed;
+    e.dq_acc = dq_acc;
+    e.single = static_cast<const uint8_t*>(plan) + packed_single_offset(total_q, total_k, n);
+    e.single_bit = causal ? 2 : 1;
+    e.lse = lse;
+    e.dq = reinterpret_cast<__nv_bfloat16*>(dq);
+    e.dq_ts = dq_ts; e.dq_hs = dq_hs;
+    attn_delta_kernel<true><<<static_cast<unsigned>((rows + 16 * kDeltaRows - 1) / (16 * kDeltaRows)), 256, 0, stream>>>(
         reinterpret_cast<const __nv_bfloat16*>(dout), reinterpret_cast<const __nv_bfloat16*>(o), delta, 1, total_q, nh, d,
-        rows * d, static_cast<long>(nh) * d, d, rows * d, static_cast<long>(nh) * d, d, claimed);
-    if (cudaMemsetAsync(dq_acc, 0, sizeof(float) * rows * static_cast<size_t>(d), stream) != cudaSuccess) return -4;
+        rows * d, static_cast<long>(nh) * d, d, rows * d, static_cast<long>(nh) * d, d, e);
+  } else if (cudaMemsetAsync(claimed, 0, sizeof(int), stream) != cudaSuccess) {
+    return -4;
   }
-  if (total_q == 0 && cudaMemsetAsync(claimed, 0, sizeof(int), stream) != cudaSuccess) return -4;
-  if (total_k > 0) {
-    const bool queries = total_q > 0;      // none: maps over the keys stand in, no item loads through them
-    CUtensorMap tq, tk, tv, tdo, tdq;
-    const void* qp = queries ? q : k;
-    const int qn = queries ? total_q : total_k, qh = queries ? nh : nh_kv;
-    const long qs = queries ? q_ts : k_ts, qhs = queries ? q_hs : k_hs;
-    if (!make_map4(&tq, qp, 1, qn, qh, d, qs * qn, qs, qhs, wide::BB)) return -2;
-    if (!make_map4(&tk, k, 1, total_k, nh_kv, d, k_ts * total_k, k_ts, k_hs, wide::BB)) return -2;
-    if (!make_map4(&tv, v, 1, total_k, nh_kv, d, v_ts * total_k, v_ts, v_hs, wide::BB)) return -2;
-    if (queries) {
-      if (!make_map4(&tdo, dout, 1, total_q, nh, d, rows * d, static_cast<long>(nh) * d, d, wide::BB)) return -2;
-      if (!make_map_dq(&tdq, dq_acc, nh, total_q, d, wide::BB)) return -2;
-    } else {
-      tdo = tdq = tq;
-    }
-    wide::PackedParams p;
-    p.lse = lse; p.delta = delta;
-    p.dk = reinterpret_cast<__nv_bfloat16*>(dk);
-    p.dv = reinterpret_cast<__nv_bfloat16*>(dv);
-    p.dk_bs = p.dv_bs = 0;
-    p.dk_ts = dk_ts; p.dk_hs = dk_hs;
-    p.dv_ts = dv_ts; p.dv_hs = dv_hs;
-    p.sq = total_q; p.sk = total_k; p.nh = nh; p.nh_kv = nh_kv; p.d = d;
-    p.nchunks = (d + 63) / 64;
-    p.scale = scale;
-    p.scale_log2 = scale * 1.4426950408889634f;
-    p.causal = causal;
-    p.seqlens_q = p.seqlens_k = nullptr;
-    p.status = mb_status_device_ptr();
-    const uint8_t* list = static_cast<const uint8_t*>(plan) + packed_list_offset(total_q, total_k, n, 1, causal != 0);
-    p.list = reinterpret_cast<const PackedHeader*>(list);
-    p.items = reinterpret_cast<const PackedItem*>(p.list + 1);
-    p.claimed = claimed;
-    const auto kern = d > 80 ? wide::attn_bwd_wide_kernel<true, true> : wide::attn_bwd_wide_kernel<false, true>;
-    int dev = 0;
-    static bool cfg[64][2] = {};
-    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -3;
-    if (!cfg[dev][d > 80]) {
-      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, wide::kSmem) != cudaSuccess) return -3;
-      cfg[dev][d > 80] = true;
-    }
-    wide::Sched sch;
-    sch.nblk = sch.total = 0;      // from the plan
-    sch.units = static_cast<int>(units);
-    sch.unit_heads = unit_heads;
-    sch.bu = sch.units;
-    const long unit_bytes = 8l * unit_heads * (total_q > 0 ? total_q : 1) * d;
-    const long group = (48l << 20) / unit_bytes;
-    sch.group = static_cast<int>(group < 1 ? 1 : (group < units ? group : units));
-    kern<<<most < 148 ? static_cast<int>(most) : 148, wide::kThreads, wide::kSmem, stream>>>(tq, tk, tv, tdo, tdq, p, sch);
+  if (total_k == 0) return cudaGetLastError() == cudaSuccess ? 0 : -4;
+  const bool queries = total_q > 0;      // none: maps over the keys stand in, no item loads through them
+  CUtensorMap tq, tk, tv, tdo, tdq;
+  const void* qp = queries ? q : k;
+  const int qn = queries ? total_q : total_k, qh = queries ? nh : nh_kv;
+  const long qs = queries ? q_ts : k_ts, qhs = queries ? q_hs : k_hs;
+  if (!make_map4(&tq, qp, 1, qn, qh, d, qs * qn, qs, qhs, wide::BB)) return -2;
+  if (!make_map4(&tk, k, 1, total_k, nh_kv, d, k_ts * total_k, k_ts, k_hs, wide::BB)) return -2;
+  if (!make_map4(&tv, v, 1, total_k, nh_kv, d, v_ts * total_k, v_ts, v_hs, wide::BB)) return -2;
+  if (queries) {
+    if (!make_map4(&tdo, dout, 1, total_q, nh, d, rows * d, static_cast<long>(nh) * d, d, wide::BB)) return -2;
+    if (!make_map_dq(&tdq, dq_acc, nh, total_q, d, wide::BB)) return -2;
+  } else {
+    tdo = tdq = tq;
   }
-  if (total_q > 0) {
+  const int parts = nh / nh_kv / unit_heads;
+  __nv_bfloat16* part_k = reinterpret_cast<__nv_bfloat16*>(at + area.parts);
+  __nv_bfloat16* part_v = reinterpret_cast<__nv_bfloat16*>(at + area.parts + (area.total - area.parts) / 2);
+  wide::PackedParams p;
+  p.lse = lse; p.delta = delta;
+  p.dk = parts > 1 ? part_k : reinterpret_cast<__nv_bfloat16*>(dk);
+  p.dv = parts > 1 ? part_v : reinterpret_cast<__nv_bfloat16*>(dv);
+  p.dk_bs = p.dv_bs = 0;
+  p.dk_ts = parts > 1 ? units * d : dk_ts; p.dk_hs = parts > 1 ? d : dk_hs;
+  p.dv_ts = parts > 1 ? units * d : dv_ts; p.dv_hs = parts > 1 ? d : dv_hs;
+  p.sq = total_q; p.sk = total_k; p.nh = nh; p.nh_kv = nh_kv; p.d = d;
+  p.nchunks = (d + 63) / 64;
+  p.scale = scale;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.causal = causal;
+  p.seqlens_q = p.seqlens_k = nullptr;
+  p.status = mb_status_device_ptr();
+  const uint8_t* list = static_cast<const uint8_t*>(plan) + packed_list_offset(total_q, total_k, n, 1, causal != 0);
+  p.list = reinterpret_cast<const PackedHeader*>(list);
+  p.items = reinterpret_cast<const PackedItem*>(p.list + 1);
+  p.claimed = claimed;
+  p.dq = reinterpret_cast<__nv_bfloat16*>(dq);
+  p.dq_ts = dq_ts; p.dq_hs = dq_hs;
+  const auto kern = d > 80 ? wide::attn_bwd_wide_kernel<true, true> : wide::attn_bwd_wide_kernel<false, true>;
+  int dev = 0;
+  static bool cfg[64][2] = {};
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -3;
+  if (!cfg[dev][d > 80]) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, wide::kSmem) != cudaSuccess) return -3;
+    cfg[dev][d > 80] = true;
+  }
+  wide::Sched sch;
+  sch.nblk = sch.total = 0;      // from the plan
+  sch.units = static_cast<int>(units);
+  sch.unit_heads = unit_heads;
+  sch.bu = sch.units;
+  // head units whose Q, dO and fp32 dQ take about a third of L2 together, at least one
+  const long unit_bytes = 8l * unit_heads * (total_q > 0 ? total_q : 1) * d;
+  const long group = (48l << 20) / unit_bytes;
+  sch.group = static_cast<int>(group < 1 ? 1 : (group < units ? group : units));
+  kern<<<most < 148 ? static_cast<int>(most) : 148, wide::kThreads, wide::kSmem, stream>>>(tq, tk, tv, tdo, tdq, p, sch);
+  if (queries) {
     long blocks = (rows * (d / 8) + 255) / 256;
     if (blocks > 148 * 16) blocks = 148 * 16;
-    attn_convert_dq_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
-        dq_acc, reinterpret_cast<__nv_bfloat16*>(dq), 1, total_q, nh, d, 0, dq_ts, dq_hs, scale);
+    attn_convert_dq_kernel<true><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
+        dq_acc, p.dq, 1, total_q, nh, d, 0, dq_ts, dq_hs, scale,
+        static_cast<const uint8_t*>(plan) + packed_single_offset(total_q, total_k, n), causal ? 2 : 1);
   }
-  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+  if (cudaGetLastError() != cudaSuccess) return -4;
+  return parts > 1 ? mb_attn_sum_parts(part_k, part_v, dk, dv, 1, total_k, nh_kv, parts, d, 0, dk_ts, dk_hs, 0, dv_ts, dv_hs,
+                                       stream)
+                   : 0;
 }
 
 // dk_parts, dv_parts: contiguous [b][sk][nh_kv * parts][d]; dk, dv: [b][sk][nh_kv][d] with the given element strides

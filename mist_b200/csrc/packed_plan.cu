@@ -13,9 +13,10 @@ constexpr int kCosts = 8192;       // blocks of 128 a tile walks; dearer ones co
 // queries), whose outputs are zeros.  Items of one cost come in no fixed order; no result depends on it but the order in
 // which dQ is summed.
 __global__ void __launch_bounds__(kThreads)
-packed_plan_kernel(const int* cu_q, const int* cu_k, int n, int total_q, int total_k, uint8_t* plan, int64_t* positions) {
+packed_plan_kernel(const int* cu_q, const int* cu_k, int n, int total_q, int total_k, uint8_t* plan) {
   __shared__ int count[kCosts];
   __shared__ int part[32], all_costs, dearest;
+  auto clamped = [](int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); };
   if (blockIdx.x >= 4) {      // a row's place in its sequence: the last offset that is not above it
     const int row = (blockIdx.x - 4) * kThreads + threadIdx.x;
     if (row >= total_q) return;
@@ -25,7 +26,14 @@ packed_plan_kernel(const int* cu_q, const int* cu_k, int n, int total_q, int tot
       if (cu_q[mid] <= row) lo = mid;
       else hi = mid - 1;
     }
-    positions[row] = lo ? row - cu_q[lo] : row;
+    const int q0 = lo ? cu_q[lo] : 0, at = row - q0;
+    reinterpret_cast<int64_t*>(plan + packed_positions_offset(total_q, total_k, n))[row] = at;
+    // the numbers of the sequence as the lists have them
+    const int k0 = lo ? clamped(cu_k[lo], 0, total_k) : 0;
+    const int sq = (lo < n ? clamped(cu_q[lo + 1], q0, total_q) : total_q) - q0;
+    const int sk = lo < n ? clamped(cu_k[lo + 1], k0, total_k) - k0 : 0;
+    plan[packed_single_offset(total_q, total_k, n) + row] =
+        (packed_key_blocks(at & ~127, sq, sk, false) <= 1 ? 1 : 0) | (packed_key_blocks(at & ~127, sq, sk, true) <= 1 ? 2 : 0);
     return;
   }
   const int backward = blockIdx.x >> 1, causal = blockIdx.x & 1;
@@ -37,7 +45,6 @@ packed_plan_kernel(const int* cu_q, const int* cu_k, int n, int total_q, int tot
   for (int i = tid; i < kCosts; i += kThreads) count[i] = 0;
   if (tid == 0) all_costs = dearest = 0;
   __syncthreads();
-  auto clamped = [](int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); };
   auto walk = [&](auto&& f) {
     for (int b = warp; b <= n; b += kThreads / 32) {
       PackedItem it;
@@ -112,15 +119,16 @@ packed_plan_kernel(const int* cu_q, const int* cu_k, int n, int total_q, int tot
 // Bytes of a plan for n sequences in tensors of total_q and total_k rows.
 MB_API long mb_packed_plan_bytes(int n, int total_q, int total_k) {
   if (n < 0 || total_q < 0 || total_k < 0) return 0;
-  return packed_list_offset(total_q, total_k, n, 1, 1) + packed_list_bytes(packed_backward_items(total_k, n));
+  return packed_single_offset(total_q, total_k, n) + total_q;
 }
+// Where in a plan every query row's place in its sequence stands: total_q numbers of 64 bits.
+MB_API long mb_packed_plan_positions(int n, int total_q, int total_k) { return packed_positions_offset(total_q, total_k, n); }
 
-// cu_q, cu_k: n + 1 offsets each, in device memory; positions [total_q]: every query row's place in its sequence.  The plan (16-byte aligned) serves causal and full attention, forward
+// cu_q, cu_k: n + 1 offsets each, in device memory.  The plan (16-byte aligned) serves causal and full attention, forward
 // and backward, with any number of heads.
-MB_API int mb_packed_plan(const int* cu_q, const int* cu_k, int n, int total_q, int total_k, void* plan, int64_t* positions,
-                          cudaStream_t stream) {
+MB_API int mb_packed_plan(const int* cu_q, const int* cu_k, int n, int total_q, int total_k, void* plan, cudaStream_t stream) {
   if (n < 0 || total_q < 0 || total_k < 0 || (reinterpret_cast<uintptr_t>(plan) & 15)) return -1;
   packed_plan_kernel<<<4 + (total_q + kThreads - 1) / kThreads, kThreads, 0, stream>>>(
-      cu_q, cu_k, n, total_q, total_k, static_cast<uint8_t*>(plan), positions);
+      cu_q, cu_k, n, total_q, total_k, static_cast<uint8_t*>(plan));
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }

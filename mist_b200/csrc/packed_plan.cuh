@@ -26,6 +26,23 @@ __host__ __device__ inline long packed_list_offset(long total_q, long total_k, l
   const long f = packed_list_bytes(packed_forward_items(total_q, n)), b = packed_list_bytes(packed_backward_items(total_k, n));
   return backward ? 2 * f + causal * b : causal * f;
 }
+// Behind the lists: every query row's place in its sequence (int64), then, a byte per row, whether at most one block of keys
+// is visible from the row's tile (bit 0: whole sequences visible, bit 1: causal).
+__host__ __device__ inline long packed_positions_offset(long total_q, long total_k, long n) {
+  return packed_list_offset(total_q, total_k, n, 1, 1) + packed_list_bytes(packed_backward_items(total_k, n));
+}
+__host__ __device__ inline long packed_single_offset(long total_q, long total_k, long n) {
+  return packed_positions_offset(total_q, total_k, n) + 8 * total_q;
+}
+// Blocks of 128 keys that a tile of 128 queries from q0 on sees, in a sequence of sq queries and sk keys.
+__host__ __device__ inline int packed_key_blocks(int q0, int sq, int sk, bool causal) {
+  int keys = sk;
+  if (causal) {
+    const int seen = q0 + 128 + sk - sq;
+    keys = seen < keys ? seen : keys;
+  }
+  return keys > 0 ? (keys + 127) / 128 : 0;
+}
 
 // Work items are dealt as they are asked for: a tile of a long sequence takes tens of times as long as one of a short
 // sequence, and dealing them in turn left a third of the chip idle at the end (16384 tokens in 14 documents, 32 heads of 128

@@ -86,8 +86,12 @@ def _unit_heads(q, k) -> int:
     the queries; it must not exceed a CTA's share of the whole (148 CTAs, half of the blocks visible), or the last
     CTA works alone.  What is not summed inside a CTA costs a pass over dK and dV afterwards."""
     b, sq, nh, _ = q.shape
-    g = nh // k.shape[2]
-    most = (k.shape[1] + 127) // 128 * nh * b // 296
+    return unit_heads(nh // k.shape[2], k.shape[1], nh * b)
+
+
+def unit_heads(g: int, sk: int, heads: int) -> int:
+    """:func:`_unit_heads` from the size of a group, the keys, and the query heads of all samples."""
+    most = (sk + 127) // 128 * heads // 296
     return max((u for u in range(1, g + 1) if g % u == 0 and u <= most), default=1)
 
 

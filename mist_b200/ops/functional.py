@@ -893,22 +893,17 @@ class _PackedAttnFn(torch.autograd.Function):
     produced as one packed tensor, so autograd never splits or re-concatenates q/k/v."""
 
     @staticmethod
-    def forward(ctx, qkv, cos, sin, rot, scale, causal, kv_heads, seqlens, packed):
-        ctx.kv_heads, ctx.seqlens, ctx.shape, ctx.packed = kv_heads, seqlens, qkv.shape, packed
+    def forward(ctx, qkv, cos, sin, rot, scale, causal, kv_heads, seqlens):
+        ctx.kv_heads, ctx.seqlens, ctx.shape = kv_heads, seqlens, qkv.shape
         if qkv.dim() == 5:
             qkv = qkv.reshape(*qkv.shape[:2], -1, qkv.shape[4])
-        if packed is not None:
-            qkv = qkv.reshape(1, -1, *qkv.shape[2:])
         if rot:
             qkv = _PackedAttnFn._rotate(qkv, cos, sin, rot, False, kv_heads)
         q, k, v = _PackedAttnFn._split(qkv, kv_heads)
-        if packed is not None:
-            o, lse = packed_attention.forward(q[0], k[0], v[0], packed, scale, causal)
-        else:
-            o, lse = attn_fwd(q, k, v, scale, causal, seqlens_q=seqlens, seqlens_k=seqlens)
+        o, lse = attn_fwd(q, k, v, scale, causal, seqlens_q=seqlens, seqlens_k=seqlens)
         ctx.rot, ctx.scale, ctx.causal = rot, scale, causal
         ctx.save_for_backward(qkv, o, lse, cos, sin)
-        return o if packed is None else o.view(*ctx.shape[:2], *o.shape[1:])
+        return o
 
     @staticmethod
     def _split(qkv, nkv):
@@ -931,16 +926,11 @@ class _PackedAttnFn(torch.autograd.Function):
         qkv, o, lse, cos, sin = ctx.saved_tensors
         from . import attention_bwd
         dqkv = torch.empty_like(qkv)
-        if ctx.packed is not None:
-            q, k, v, dq, dk, dv = (t[0] for x in (qkv, dqkv) for t in _PackedAttnFn._split(x, ctx.kv_heads))
-            packed_attention.backward(dout.reshape(o.shape), q, k, v, o, lse, ctx.packed, ctx.scale, ctx.causal,
-                                      out=(dq, dk, dv))
-        else:
-            attention_bwd.backward(dout, *_PackedAttnFn._split(qkv, ctx.kv_heads), o, lse, ctx.scale, ctx.causal,
-                                   out=_PackedAttnFn._split(dqkv, ctx.kv_heads), seqlens=(ctx.seqlens, ctx.seqlens))
+        attention_bwd.backward(dout, *_PackedAttnFn._split(qkv, ctx.kv_heads), o, lse, ctx.scale, ctx.causal,
+                               out=_PackedAttnFn._split(dqkv, ctx.kv_heads), seqlens=(ctx.seqlens, ctx.seqlens))
         if ctx.rot:
             dqkv = _PackedAttnFn._rotate(dqkv, cos, sin, ctx.rot, True, ctx.kv_heads)
-        return dqkv.view(ctx.shape), None, None, None, None, None, None, None, None
+        return dqkv.view(ctx.shape), None, None, None, None, None, None, None
 
 
 class _KVPackedAttnFn(torch.autograd.Function):
@@ -969,24 +959,15 @@ def attention_projected(qkv, kv_heads: int, scale: float, causal: bool, rotary=N
     ``seqlens``: as in :func:`attention`; ``rotary``: ``(cos, sin, rot_dim)``, rotated in place on the device.
     ``packed``: a :class:`PackedSequences` of the ``b * s`` tokens, each of which attends inside its sequence (then the
     tables of ``rotary`` have a row for every token: :meth:`PackedSequences.rotary`)."""
-    cos, sin, rot = rotary if rotary is not None else (None, None, 0)
     if packed is not None:
         if _elsewhere(qkv):
             with torch.cuda.device(qkv.device):
                 return attention_projected(qkv, kv_heads, scale, causal, rotary, seqlens, packed)
         if seqlens is not None:
             raise ValueError("packed sequences have no padding: seqlens cannot be given beside them")
-        rows, heads = qkv.flatten(0, 1), qkv.numel() // max(qkv.shape[0] * qkv.shape[1] * qkv.shape[-1], 1)
-        packed.check(rows, rows)
-        if not packed.same or (qkv.numel() and (heads <= 2 * kv_heads or (heads - 2 * kv_heads) % kv_heads)):
-            raise ValueError(f"self attention of {heads} heads in all, {kv_heads} of them for keys, over one packing expected")
-        if use_native(qkv):
-            packed_attention.check_kernel_types(qkv)
-            if not qkv.is_contiguous() or ptr(qkv) % 16:
-                if rot:
-                    raise ValueError("the rotation in place needs a contiguous projection output")
-                qkv = qkv.clone(memory_format=torch.contiguous_format)
-    return _PackedAttnFn.apply(qkv, cos, sin, int(rot), float(scale), bool(causal), int(kv_heads), seqlens, packed)
+        return packed_attention.projected_attention(qkv, kv_heads, packed, scale, causal, rotary)
+    cos, sin, rot = rotary if rotary is not None else (None, None, 0)
+    return _PackedAttnFn.apply(qkv, cos, sin, int(rot), float(scale), bool(causal), int(kv_heads), seqlens)
 
 
 def attention_kvpacked(q, kv, scale: float, causal: bool, seqlens_q=None, seqlens_k=None):

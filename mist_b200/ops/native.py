@@ -75,10 +75,12 @@ _SIGNATURES = {
     "mb_attn_bwd": ([_p] * 11 + [_i] * 7 + [_l] * 18 + [_f, _i, _p, _p, _p], _i),
     "mb_attn_sum_parts": ([_p] * 4 + [_i] * 5 + [_l] * 6 + [_p], _i),
     "mb_packed_plan_bytes": ([_i, _i, _i], _l),
-    "mb_packed_plan": ([_p, _p, _i, _i, _i, _p, _p, _p], _i),
+    "mb_packed_plan_positions": ([_i, _i, _i], _l),
+    "mb_packed_plan": ([_p, _p, _i, _i, _i, _p, _p], _i),
     "mb_attn_fwd_packed_counters": ([_i, _i, _i], _i),
     "mb_attn_fwd_packed": ([_p] * 7 + [_i] * 6 + [_l] * 8 + [_f, _i, _p], _i),
-    "mb_attn_bwd_packed": ([_p] * 13 + [_i] * 7 + [_l] * 12 + [_f, _i, _p], _i),
+    "mb_attn_bwd_packed_workspace": ([_i] * 6, _z),
+    "mb_attn_bwd_packed": ([_p] * 11 + [_i] * 7 + [_l] * 12 + [_f, _i, _p], _i),
     "mb_attn_fwd": ([_p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i] + [_l] * 12 + [_f, _i, _p, _p, _p], _i),
 }
 

@@ -20,7 +20,9 @@ def _offsets(cu, device):
         if cu.dim() != 1 or cu.numel() < 1 or cu.is_floating_point():
             raise ValueError(f"offsets: a vector of integers expected, got {tuple(cu.shape)} of {cu.dtype}")
         if cu.is_cuda:
-            return cu.to(device=device, dtype=torch.int32).contiguous(), None
+            if cu.dtype != torch.int32 or cu.device != device or not cu.is_contiguous():
+                cu = cu.to(device=device, dtype=torch.int32).contiguous()
+            return cu, None
     host = [int(x) for x in (cu.tolist() if isinstance(cu, torch.Tensor) else cu)]
     if not host or host[0] != 0 or any(b < a for a, b in zip(host, host[1:])):
         raise ValueError("offsets: they begin with 0 and do not fall")
@@ -38,8 +40,10 @@ class PackedSequences:
 
     def __init__(self, cu_seqlens, total: Optional[int] = None, cu_seqlens_k=None, total_k: Optional[int] = None, device=None):
         if device is None:
-            device = cu_seqlens.device if isinstance(cu_seqlens, torch.Tensor) else torch.device("cpu")
+            device = cu_seqlens.device if isinstance(cu_seqlens, torch.Tensor) else "cpu"
         device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
         self.same = cu_seqlens_k is None
         self.cu_q, self.host_q = _offsets(cu_seqlens, device)
         self.cu_k, self.host_k = (self.cu_q, self.host_q) if self.same else _offsets(cu_seqlens_k, device)
@@ -48,26 +52,32 @@ class PackedSequences:
         self.n = self.cu_q.numel() - 1
         self.total_q = self._total(total, self.host_q)
         self.total_k = self.total_q if self.same and total_k is None else self._total(total_k, self.host_k)
-        self.device = self.cu_q.device
+        self.device = device
         self._rotary = {}
-        self.plan = None
+        self._positions = self.plan = None
         if use_native(self.cu_q):
             size = native.kernels().mb_packed_plan_bytes(self.n, self.total_q, self.total_k)
-            self.plan = torch.empty(size, dtype=torch.uint8, device=self.device)
-            #: every query row's place in its sequence, int64 ``[total]``
-            self.positions = torch.empty(self.total_q, dtype=torch.int64, device=self.device)
-            if self.device.index == torch._C._cuda_getDevice():
+            self.plan = torch.empty(size, dtype=torch.uint8, device=device)
+            if device.index == torch._C._cuda_getDevice():
                 self._make_plan()
             else:
-                with torch.cuda.device(self.device):
+                with torch.cuda.device(device):
                     self._make_plan()
-        else:
-            at = torch.arange(self.total_q)
-            self.positions = at - self.cu_q.long()[torch.searchsorted(self.cu_q, at, right=True) - 1]
 
     def _make_plan(self):
-        call("mb_packed_plan", ptr(self.cu_q), ptr(self.cu_k), self.n, self.total_q, self.total_k, ptr(self.plan),
-             ptr(self.positions), stream())
+        call("mb_packed_plan", ptr(self.cu_q), ptr(self.cu_k), self.n, self.total_q, self.total_k, ptr(self.plan), stream())
+
+    @property
+    def positions(self):
+        """Every query row's place in its sequence, int64 ``[total]``."""
+        if self._positions is None:
+            if self.plan is not None:
+                at = native.kernels().mb_packed_plan_positions(self.n, self.total_q, self.total_k)
+                self._positions = self.plan[at:at + 8 * self.total_q].view(torch.int64)
+            else:
+                rows = torch.arange(self.total_q)
+                self._positions = rows - self.cu_q.long()[torch.searchsorted(self.cu_q, rows, right=True) - 1]
+        return self._positions
 
     @staticmethod
     def _total(total, host):
@@ -102,71 +112,57 @@ class PackedSequences:
 
 def _rows(t):
     """``t`` ``[rows, heads, d]`` as the kernels' copies can address it."""
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or ptr(t) % 16 or (t.shape[0] > 1 and t.stride(0) == 0) \
-            or (t.shape[1] > 1 and t.stride(1) == 0):
+    rows, heads, inner = t.stride()
+    if inner != 1 or rows % 8 or heads % 8 or ptr(t) % 16 or (rows == 0 and t.shape[0] > 1) or (heads == 0 and t.shape[1] > 1):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
-def forward(q, k, v, packed: PackedSequences, scale: float, causal: bool):
-    """Attention of ``q`` ``[total_q, heads, d]`` over ``k``, ``v`` ``[total_k, kv heads, d]`` inside each sequence:
-    ``(o, lse [heads, total_q])``."""
-    total, nh, d = q.shape
-    if not use_native(q):
-        from .functional import _ref_attention
-        o = torch.zeros_like(q, memory_format=torch.contiguous_format)
-        lse = torch.full((nh, total), float("-inf"), dtype=torch.float32)
-        for a, b in packed._each():
-            if a.stop > a.start and b.stop > b.start:
-                oi, li = _ref_attention(q[None, a], k[None, b], v[None, b], scale, causal)
-                o[a], lse[:, a] = oi[0], li[0]
-        return o, lse
-    o = torch.empty(total, nh, d, dtype=q.dtype, device=q.device)
-    lse = torch.empty(nh * total + 1, dtype=torch.float32, device=q.device)      # and the count of claimed work items
-    claimed = ptr(lse) + 4 * nh * total
-    lse = lse[:nh * total].view(nh, total)
-    call("mb_attn_fwd_packed", ptr(q), ptr(k), ptr(v), ptr(o), ptr(lse), ptr(packed.plan),
-         claimed if native.kernels().mb_attn_fwd_packed_counters(packed.n, total, nh) else 0, packed.n, total, k.shape[0], nh,
-         k.shape[1], d, q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), nh * d, d, scale,
-         int(causal), stream())
+def _reference_forward(q, k, v, packed, scale, causal):
+    from .functional import _ref_attention
+    o = torch.zeros(q.shape, dtype=q.dtype)
+    lse = torch.full((q.shape[1], q.shape[0]), float("-inf"), dtype=torch.float32)
+    for a, b in packed._each():
+        if a.stop > a.start and b.stop > b.start:
+            oi, li = _ref_attention(q[None, a], k[None, b], v[None, b], scale, causal)
+            o[a], lse[:, a] = oi[0], li[0]
     return o, lse
 
 
-def backward(dout, q, k, v, o, lse, packed: PackedSequences, scale: float, causal: bool, out=None):
-    """``(dq, dk, dv)``; with ``out`` written into those (possibly strided) tensors."""
-    from . import attention_bwd
-    if out is None:
-        out = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    dq, dk, dv = out
-    if not use_native(q):
-        for t in out:
-            t.zero_()
-        for a, b in packed._each():
-            if a.stop > a.start and b.stop > b.start:
-                for t, at, g in zip(out, (a, b, b), attention_bwd._reference(dout[None, a], q[None, a], k[None, b], v[None, b],
-                                                                            scale, causal)):
-                    t[at] = g[0]
-        return out
-    total, nh, d = q.shape
-    nkv = k.shape[1]
+def _reference_backward(dout, q, k, v, packed, scale, causal, out):
+    from .attention_bwd import _reference
+    for t in out:
+        t.zero_()
+    for a, b in packed._each():
+        if a.stop > a.start and b.stop > b.start:
+            grads = _reference(dout[None, a], q[None, a], k[None, b], v[None, b], scale, causal)
+            for t, at, g in zip(out, (a, b, b), grads):
+                t[at] = g[0]
+
+
+def _launch_forward(tensors, strides, o, heads, packed, scale, causal):
+    """``tensors``: addresses of q, k, v; ``strides``: of their rows and heads.  Returns lse, ``[heads, total]`` and one more
+    number behind (the count of claimed work items)."""
+    nh, nkv, d = heads
+    total = packed.total_q
+    lse = torch.empty(nh * total + 1, dtype=torch.float32, device=o.device)
+    claimed = ptr(lse) + 4 * nh * total if native.kernels().mb_attn_fwd_packed_counters(packed.n, total, nh) else 0
+    call("mb_attn_fwd_packed", *tensors, ptr(o), ptr(lse), ptr(packed.plan), claimed, packed.n, total, packed.total_k, nh, nkv,
+         d, *strides, nh * d, d, scale, int(causal), stream())
+    return lse
+
+
+def _launch_backward(dout, tensors, strides, o, lse, grads, grad_strides, heads, packed, scale, causal):
+    from .attention_bwd import unit_heads
+    nh, nkv, d = heads
     dout = dout.contiguous()
     if ptr(dout) % 16:
         dout = dout.clone()
-    unit = attention_bwd._unit_heads(q[None], k[None])
-    parts = nh // nkv // unit
-    gk, gv = dk, dv
-    if parts > 1:        # a CTA sums `unit` heads of a group; the rest is added from a copy per unit
-        gk, gv = (torch.empty(k.shape[0], nkv * parts, d, dtype=q.dtype, device=q.device) for _ in range(2))
-    delta = torch.empty(nh * total + 1, dtype=torch.float32, device=q.device)    # and the count of claimed work items
-    dq_acc = torch.empty(nh, total, d, dtype=torch.float32, device=q.device)
-    call("mb_attn_bwd_packed", ptr(dout), ptr(q), ptr(k), ptr(v), ptr(o), ptr(lse), ptr(delta), ptr(dq_acc),
-         ptr(delta) + 4 * nh * total, ptr(dq), ptr(gk), ptr(gv), ptr(packed.plan), packed.n, total, k.shape[0], nh, nkv, unit, d, q.stride(0), q.stride(1), k.stride(0),
-         k.stride(1), v.stride(0), v.stride(1), dq.stride(0), dq.stride(1), gk.stride(0), gk.stride(1), gv.stride(0),
-         gv.stride(1), scale, int(causal), stream())
-    if parts > 1:
-        call("mb_attn_sum_parts", ptr(gk), ptr(gv), ptr(dk), ptr(dv), 1, k.shape[0], nkv, parts, d, 0, dk.stride(0),
-             dk.stride(1), 0, dv.stride(0), dv.stride(1), stream())
-    return out
+    unit = unit_heads(nh // nkv, packed.total_k, nh)
+    size = native.kernels().mb_attn_bwd_packed_workspace(packed.total_q, packed.total_k, nh, nkv, unit, d)
+    workspace = torch.empty(size, dtype=torch.uint8, device=o.device)
+    call("mb_attn_bwd_packed", ptr(dout), *tensors, ptr(o), ptr(lse), *grads, ptr(packed.plan), ptr(workspace), packed.n,
+         packed.total_q, packed.total_k, nh, nkv, unit, d, *strides, *grad_strides, scale, int(causal), stream())
 
 
 def check_kernel_types(*tensors):
@@ -176,20 +172,87 @@ def check_kernel_types(*tensors):
 
 
 class _PackedSequencesAttnFn(torch.autograd.Function):
+    """q ``[total_q, heads, d]``, k and v ``[total_k, kv heads, d]``."""
+
     @staticmethod
     def forward(ctx, q, k, v, packed, scale, causal):
-        o, lse = forward(q, k, v, packed, scale, causal)
         ctx.packed, ctx.scale, ctx.causal = packed, scale, causal
+        if use_native(q):
+            o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            lse = _launch_forward((ptr(q), ptr(k), ptr(v)), (*q.stride()[:2], *k.stride()[:2], *v.stride()[:2]), o,
+                                  (q.shape[1], k.shape[1], q.shape[2]), packed, scale, causal)
+        else:
+            o, lse = _reference_forward(q, k, v, packed, scale, causal)
         ctx.save_for_backward(q, k, v, o, lse)
         return o
 
     @staticmethod
     def backward(ctx, dout):
-        dq, dk, dv = backward(dout, *ctx.saved_tensors, ctx.packed, ctx.scale, ctx.causal)
-        return dq, dk, dv, None, None, None
+        q, k, v, o, lse = ctx.saved_tensors
+        out = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        if use_native(q):
+            _launch_backward(dout, (ptr(q), ptr(k), ptr(v)), (*q.stride()[:2], *k.stride()[:2], *v.stride()[:2]), o, lse,
+                             tuple(ptr(t) for t in out), tuple(x for t in out for x in t.stride()[:2]),
+                             (q.shape[1], k.shape[1], q.shape[2]), ctx.packed, ctx.scale, ctx.causal)
+        else:
+            _reference_backward(dout, q, k, v, ctx.packed, ctx.scale, ctx.causal, out)
+        return (*out, None, None, None)
+
+
+class _ProjectedAttnFn(torch.autograd.Function):
+    """Rotary embedding and self attention on a projection output ``[b, s, q heads + 2 * kv heads, d]`` of packed sequences,
+    whose gradient is one tensor.  On the device the projection output is rotated in place."""
+
+    @staticmethod
+    def forward(ctx, qkv, cos, sin, rot, packed, kv_heads, scale, causal):
+        from .functional import _PackedAttnFn
+        b, s, n, d = qkv.shape
+        if rot:
+            qkv = _PackedAttnFn._rotate(qkv.view(1, b * s, n, d), cos, sin, rot, False, kv_heads)
+        ctx.args = rot, packed, kv_heads, scale, causal
+        ctx.shape = b, s, n, d
+        if use_native(qkv):
+            o = torch.empty(b, s, n - 2 * kv_heads, d, dtype=qkv.dtype, device=qkv.device)
+            lse = _launch_forward(_ProjectedAttnFn._parts(ptr(qkv), n, kv_heads, d), (n * d, d) * 3, o,
+                                  (n - 2 * kv_heads, kv_heads, d), packed, scale, causal)
+        else:
+            o, lse = _reference_forward(*_ProjectedAttnFn._split(qkv.view(b * s, n, d), kv_heads), packed, scale, causal)
+            o = o.view(b, s, n - 2 * kv_heads, d)
+        ctx.save_for_backward(qkv, o, lse, cos, sin)
+        return o
+
+    @staticmethod
+    def _parts(at, n, kv_heads, d):
+        """Addresses of the q, the k and the v heads of the first token."""
+        return at, at + 2 * d * (n - 2 * kv_heads), at + 2 * d * (n - kv_heads)
+
+    @staticmethod
+    def _split(t, kv_heads):
+        n = t.shape[1]
+        return t[:, :n - 2 * kv_heads], t[:, n - 2 * kv_heads:n - kv_heads], t[:, n - kv_heads:]
+
+    @staticmethod
+    def backward(ctx, dout):
+        from .functional import _PackedAttnFn
+        qkv, o, lse, cos, sin = ctx.saved_tensors
+        rot, packed, kv_heads, scale, causal = ctx.args
+        b, s, n, d = ctx.shape
+        dqkv = torch.empty(ctx.shape, dtype=qkv.dtype, device=qkv.device)
+        if use_native(qkv):
+            strides = (n * d, d) * 3
+            _launch_backward(dout, _ProjectedAttnFn._parts(ptr(qkv), n, kv_heads, d), strides, o, lse,
+                             _ProjectedAttnFn._parts(ptr(dqkv), n, kv_heads, d), strides, (n - 2 * kv_heads, kv_heads, d),
+                             packed, scale, causal)
+        else:
+            _reference_backward(dout.reshape(b * s, -1, d), *_ProjectedAttnFn._split(qkv.view(b * s, n, d), kv_heads), packed,
+                                scale, causal, _ProjectedAttnFn._split(dqkv.view(b * s, n, d), kv_heads))
+        if rot:
+            dqkv = _PackedAttnFn._rotate(dqkv.view(1, b * s, n, d), cos, sin, rot, True, kv_heads).view(ctx.shape)
+        return dqkv, None, None, None, None, None, None, None
 
 
 def attention(q, k, v, packed: PackedSequences, scale: float, causal: bool):
+    """Attention of ``q`` ``[total_q, heads, d]`` over ``k``, ``v`` ``[total_k, kv heads, d]`` inside each sequence."""
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2] or q.shape[1] % max(k.shape[1], 1):
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit")
     packed.check(q, k)
@@ -199,3 +262,25 @@ def attention(q, k, v, packed: PackedSequences, scale: float, causal: bool):
         check_kernel_types(q, k, v)
         q, k, v = _rows(q), _rows(k), _rows(v)
     return _PackedSequencesAttnFn.apply(q, k, v, packed, float(scale), bool(causal))
+
+
+def projected_attention(qkv, kv_heads: int, packed: PackedSequences, scale: float, causal: bool, rotary):
+    """Self attention on a projection output ``[b, s, q heads + 2 * kv heads, d]`` or ``[b, s, 3, kv heads, d]``."""
+    cos, sin, rot = rotary if rotary is not None else (None, None, 0)
+    if qkv.dim() == 5:
+        qkv = qkv.flatten(2, 3)
+    if qkv.dim() != 4 or qkv.shape[2] <= 2 * kv_heads or (qkv.shape[2] - 2 * kv_heads) % kv_heads or not packed.same:
+        raise ValueError(f"{tuple(qkv.shape)} with {kv_heads} key heads: self attention over one packing expected")
+    if qkv.shape[0] * qkv.shape[1] != packed.total_q or packed.total_k != packed.total_q:
+        raise ValueError(f"{tuple(qkv.shape[:2])} tokens, but the packing is of {packed.total_q}")
+    if qkv.device != packed.device:
+        raise ValueError(f"tensors on {qkv.device}, offsets on {packed.device}")
+    if use_native(qkv):
+        check_kernel_types(qkv)
+        if not qkv.is_contiguous() or ptr(qkv) % 16:
+            if rot:
+                raise ValueError("the rotation in place needs a contiguous projection output")
+            qkv = qkv.clone(memory_format=torch.contiguous_format)
+    elif not qkv.is_contiguous():
+        qkv = qkv.contiguous()
+    return _ProjectedAttnFn.apply(qkv, cos, sin, int(rot), packed, int(kv_heads), float(scale), bool(causal))

@@ -153,7 +153,8 @@ def _lists(seqs):
     """(backward, causal) -> items of a plan, as the kernels read them."""
     plan, n = seqs.plan.cpu(), seqs.n
     fwd, bwd = HEAD + ITEM * (seqs.total_q // 256 + n + 1), HEAD + ITEM * (seqs.total_k // 128 + n + 1)
-    assert plan.numel() == 2 * (fwd + bwd)
+    assert plan.numel() == 2 * (fwd + bwd) + 9 * seqs.total_q
+    single = plan[2 * (fwd + bwd) + 8 * seqs.total_q:].tolist()      # a byte per query row
     out, heads = {}, {}
     for backward in (0, 1):
         for causal in (0, 1):
@@ -164,7 +165,7 @@ def _lists(seqs):
             assert 0 <= count <= (size - HEAD) // ITEM
             out[backward, causal] = words[4:4 + 8 * count].view(-1, 8)[:, :5].tolist()
             heads[backward, causal] = words[:4].tolist()
-    return out, heads
+    return out, heads, single
 
 
 @pytest.mark.parametrize("lens_q,lens_k,extra", [(SHORT, SHORT, 0), (EDGES, EDGES, 7), ([], [], 10), ([5000], [5000], 0),
@@ -174,7 +175,13 @@ def test_plan_covers_every_row_once(lens_q, lens_k, extra):
     tq, tk = cu_q[-1] + extra, cu_k[-1] + extra
     seqs = F.PackedSequences(torch.tensor(cu_q, device=DEV), tq, torch.tensor(cu_k, device=DEV), tk)
     assert seqs.positions.tolist() == [i for n in lens_q for i in range(n)] + list(range(extra))
-    lists, heads = _lists(seqs)
+    lists, heads, single = _lists(seqs)
+    want = []
+    for n, m in [*zip(lens_q, lens_k), (extra, 0)]:         # at most one block of keys seen: whole (1), causal (2)
+        for i in range(n):
+            keys = min(m, i // 128 * 128 + 128 + m - n)
+            want.append((1 if m <= 128 else 0) + (2 if keys <= 128 else 0))
+    assert single == want
     for (backward, causal), items in lists.items():
         step, total = (128, tk) if backward else (256, tq)
         seen, costs = torch.zeros(total, dtype=torch.int32), []
