@@ -19,7 +19,7 @@ namespace {
 
 // ------------------------------------------------------------------------------------------------ lookup
 // One warp per token and slice of its row, `per_warp` vectors of 8 values, four rounds of loads in flight per lane.
-__global__ void __launch_bounds__(256, 6)
+__global__ void __launch_bounds__(256, 4)
 embed_fwd_kernel(const int64_t* __restrict__ ids, const int64_t* __restrict__ pos, const __nv_bfloat16* __restrict__ wte,
                  const __nv_bfloat16* __restrict__ wpe, __nv_bfloat16* __restrict__ out, int tokens, int seq, int h, int64_t v0,
                  int rows, int positions, float scale, int per_warp) {
@@ -38,11 +38,12 @@ embed_fwd_kernel(const int64_t* __restrict__ ids, const int64_t* __restrict__ po
   const mb::bf16x8* pe = reinterpret_cast<const mb::bf16x8*>(wpe + (p >= 0 ? p : 0) * h);
   mb::bf16x8* dst = reinterpret_cast<mb::bf16x8*>(out + static_cast<int64_t>(t) * h);
   for (int c0 = from + lane; c0 < to; c0 += 128) {
-    mb::bf16x8 a[4];
+    mb::bf16x8 a[4], b[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       memset(&a[u], 0, sizeof(a[u]));
       if (in && c0 + 32 * u < to) a[u] = we[c0 + 32 * u];
+      if (p >= 0 && c0 + 32 * u < to) b[u] = pe[c0 + 32 * u];
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -52,7 +53,7 @@ embed_fwd_kernel(const int64_t* __restrict__ ids, const int64_t* __restrict__ po
       mb::unpack8(a[u], f);
       if (p >= 0) {
         float g[8];
-        mb::unpack8(pe[c], g);
+        mb::unpack8(b[u], g);
 #pragma unroll
         for (int k = 0; k < 8; ++k) f[k] = in ? fmaf(f[k], scale, g[k]) : g[k];
       } else {
@@ -66,15 +67,15 @@ embed_fwd_kernel(const int64_t* __restrict__ ids, const int64_t* __restrict__ po
 
 // -------------------------------------------------------------------------------------------------- sort
 // Work area of one table's sort, 16-byte aligned arrays in a row: two buffers each of keys and tokens [tokens], counters
-// of the long rows, partial sums of the long rows.
-constexpr int kTile = 64;        // sorted tokens that are summed together where a row has more than that ("long" rows)
-constexpr int kCols = 512;       // columns of such a sum that one CTA takes
+// and partial sums of the rows whose tokens lie in several tiles.
+constexpr int kTile = 32;        // sorted tokens that a warp sums
+constexpr int kChunk = 256;      // columns of them
 
 struct Area {
   uint32_t* key[2];
   int* tok[2];
-  int* arrived;      // [tile][first, last long row of it][column slice]
-  float* part;       // [tile][first, last long row of it][h]
+  int* arrived;      // [tile][first, last row of it][column chunk]
+  float* part;       // [tile][first, last row of it][h]
 };
 
 struct Sort {
@@ -87,127 +88,221 @@ struct Sort {
 
 constexpr int kSortThreads = 1024;
 constexpr int kSortCluster = 8;
-constexpr int kHeld = 4;         // tokens that a lane keeps in registers over a pass
 
-// One cluster (or, for few tokens, one CTA) sorts one table's tokens, 8 bits of the key a pass.  A warp owns a stretch
-// of consecutive tokens; __match_any_sync ranks equal digits inside 32 of them, a histogram per warp counts those before.
-// The CTAs exchange their digit counts through distributed shared memory.  Latency is what it costs: about 2 us a pass
-//.
+// The sorts take 8 bits of the key a pass.  A warp owns a stretch of consecutive tokens; ballots over the bits rank equal
+// digits inside 32 of them (__match_any_sync takes 270 cycles of a scheduler), a histogram per warp counts those before.  Latency is all that they cost.
+struct SortSpace {
+  int hist[32][256];
+  int totals[256], base[256], warp_part[8], quarter[4][256];
+};
+
+// The digits of a pass have been counted, hist[warp][digit]; what stands there becomes the number of equal digits of this CTA
+// in the warps before, and base[digit] the place of the digit's first token of this CTA.  All(tid, own) adds up the CTAs:
+// {tokens of the digit in the CTAs before, in all}.
+template <typename All>
+__device__ __forceinline__ void sort_offsets(SortSpace& z, All&& all_of) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  __syncthreads();
+  // exclusive sum of a digit over the warps, a quarter of them per thread
+  int* column = &z.hist[8 * (tid >> 8)][tid & 255];
+  int sum = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const int n = column[256 * w];
+    column[256 * w] = sum;
+    sum += n;
+  }
+  z.quarter[tid >> 8][tid & 255] = sum;
+  __syncthreads();
+  const int2 counts = all_of(tid);
+  // exclusive sum over the digits
+  int upto = counts.y;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int n = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += n;
+  }
+  if (tid < 256 && lane == 31) z.warp_part[warp] = upto;
+  __syncthreads();
+  if (tid < 256) {
+    int start = upto - counts.y + counts.x;
+    for (int w = 0; w < warp; ++w) start += z.warp_part[w];
+    z.base[tid] = start;
+  }
+  __syncthreads();
+}
+__device__ __forceinline__ unsigned digit_of(uint32_t key, int shift, bool live) { return live ? (key >> shift) & 255u : 256u; }
+// Counts 32 tokens of the warp and returns the rank of the lane's among the warp's tokens of its digit.
+__device__ __forceinline__ int sort_count(SortSpace& z, unsigned digit) {
+  unsigned same = __ballot_sync(0xffffffffu, digit < 256);
+#pragma unroll
+  for (int b = 0; b < 8; ++b) {
+    const bool one = (digit >> b) & 1;
+    const unsigned ones = __ballot_sync(0xffffffffu, one);
+    same &= one ? ones : ~ones;
+  }
+  const int before = __popc(same & ((1u << (threadIdx.x & 31)) - 1u));
+  int* count = &z.hist[threadIdx.x >> 5][digit & 255];
+  int rank = 0;
+  if (digit < 256) rank = *count + before;
+  __syncwarp();
+  if (digit < 256 && before == 0) *count += __popc(same);
+  __syncwarp();
+  return rank;
+}
+// The place of a token of that rank, after sort_offsets.
+__device__ __forceinline__ int sort_place(const SortSpace& z, unsigned digit, int rank) {
+  const int warp = threadIdx.x >> 5;
+  int at = z.base[digit] + z.hist[warp][digit] + rank;
+  for (int q = 0; q < (warp >> 3); ++q) at += z.quarter[q][digit];
+  return at;
+}
+__device__ __forceinline__ uint32_t row_of(const Sort& s, int i) {
+  const int64_t r = s.ids[i] - s.v0;
+  return (r >= 0 && r < s.rows) ? static_cast<uint32_t>(r) : static_cast<uint32_t>(s.rows);
+}
+
+// Up to kBlockSort tokens: one CTA per table, everything in its shared memory between the passes.  (Of 16384 tokens a CTA
+// takes 51 us, a cluster 19.)
+constexpr int kHeld = 2;         // tokens of a lane
+constexpr int kBlockSort = kSortThreads * kHeld;
+constexpr int kBlockSortBytes = sizeof(SortSpace) + 8 * kBlockSort;
+__global__ void __launch_bounds__(kSortThreads)
+embed_sort_block_kernel(const __grid_constant__ Sort s0, const __grid_constant__ Sort s1, int tokens, int counters) {
+  extern __shared__ __align__(16) uint8_t sort_smem[];
+  SortSpace& z = *reinterpret_cast<SortSpace*>(sort_smem);
+  uint2* pairs = reinterpret_cast<uint2*>(sort_smem + sizeof(SortSpace));
+  const Sort& s = blockIdx.x ? s1 : s0;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+  const int per_warp = ((tokens + 31) / 32 + 31) & ~31, begin = warp * per_warp, end = min(begin + per_warp, tokens);
+  mb::let_next_kernel_start();      // the row sums wait for this kernel's end, but not for their launch
+  for (int i = tid; i < counters; i += kSortThreads) s.area.arrived[i] = 0;
+  uint32_t key[kHeld], tok[kHeld];      // tok: the token, and above it, once it is known, its rank
+  static_assert(kBlockSort <= 1 << 16 && kBlockSort / 32 <= 1 << 16, "token and rank share 32 bits");
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u) {
+    const int i = begin + 32 * u + lane;
+    tok[u] = i;
+    key[u] = i < end ? row_of(s, i) : 0u;
+  }
+  for (int pass = 0; pass < s.passes; ++pass) {
+    const int shift = 8 * pass;
+    for (int d = lane; d < 256; d += 32) z.hist[warp][d] = 0;
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u)
+      if (begin + 32 * u < end) tok[u] |= sort_count(z, digit_of(key[u], shift, begin + 32 * u + lane < end)) << 16;
+    sort_offsets(z, [&](int t) {
+      return make_int2(0, t < 256 ? z.quarter[0][t] + z.quarter[1][t] + z.quarter[2][t] + z.quarter[3][t] : 0);
+    });
+    const bool last = pass + 1 == s.passes;
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+      if (begin + 32 * u + lane < end) {
+        const int at = sort_place(z, digit_of(key[u], shift, true), tok[u] >> 16);
+        if (last) {
+          s.area.key[pass & 1][at] = key[u];
+          s.area.tok[pass & 1][at] = tok[u] & 0xffffu;
+        } else {
+          pairs[at] = make_uint2(key[u], tok[u] & 0xffffu);
+        }
+      }
+    }
+    if (last) break;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+      const int i = begin + 32 * u + lane;
+      if (i < end) {
+        const uint2 p = pairs[i];
+        key[u] = p.x;
+        tok[u] = p.y;
+      }
+    }
+  }
+}
+
+// More tokens: one cluster per table.  The CTAs exchange their digit counts through distributed shared memory.  HELD: a lane's
+// tokens fit its registers.
+constexpr int kClusterHeld = 4;
 template <bool HELD>
 __global__ void __launch_bounds__(kSortThreads)
-embed_sort_kernel(const __grid_constant__ Sort s0, const __grid_constant__ Sort s1, int tokens, int counters) {
-  __shared__ int hist[32][256];
-  __shared__ int totals[256], base[256], warp_part[8], quarter[4][256];
+embed_sort_cluster_kernel(const __grid_constant__ Sort s0, const __grid_constant__ Sort s1, int tokens, int counters) {
+  __shared__ SortSpace z;
   cg::cluster_group cluster = cg::this_cluster();
-  const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
+  constexpr int ctas = kSortCluster;
+  const int rank = cluster.block_rank();
   const Sort& s = (blockIdx.x / ctas) ? s1 : s0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
-  const unsigned below = (1u << lane) - 1u;
   const int warps = ctas * 32;
   const int per_warp = ((tokens + warps - 1) / warps + 31) & ~31;
   const long first = static_cast<long>(rank * 32 + warp) * per_warp;
   const int begin = static_cast<int>(first < tokens ? first : tokens);
   const int end = static_cast<int>(first + per_warp < tokens ? first + per_warp : tokens);
-
-  mb::let_next_kernel_start();      // the row sums wait for this kernel's end, but not for their launch
+  mb::let_next_kernel_start();
   for (int i = rank * kSortThreads + tid; i < counters; i += ctas * kSortThreads) s.area.arrived[i] = 0;
-
   for (int pass = 0; pass < s.passes; ++pass) {
     const int shift = 8 * pass;
     const uint32_t* src_key = s.area.key[(pass + 1) & 1];
     const int* src_tok = s.area.tok[(pass + 1) & 1];
-    uint32_t* dst_key = s.area.key[pass & 1];
-    int* dst_tok = s.area.tok[pass & 1];
-    auto key_at = [&](int i) -> uint32_t {
-      if (pass > 0) return __ldcg(src_key + i);
-      const int64_t r = s.ids[i] - s.v0;
-      return (r >= 0 && r < s.rows) ? static_cast<uint32_t>(r) : static_cast<uint32_t>(s.rows);
-    };
-    uint32_t key[kHeld];
-    int tok[kHeld];
+    auto key_at = [&](int i) -> uint32_t { return i >= end ? 0u : (pass > 0 ? __ldcg(src_key + i) : row_of(s, i)); };
+    uint32_t key[kClusterHeld];
+    int tok[kClusterHeld], rank_of[kClusterHeld];
     if (HELD) {
 #pragma unroll
-      for (int u = 0; u < kHeld; ++u) {
+      for (int u = 0; u < kClusterHeld; ++u) {
         const int i = begin + 32 * u + lane;
-        if (i < end) {
-          key[u] = key_at(i);
-          tok[u] = pass > 0 ? __ldcg(src_tok + i) : i;
+        key[u] = key_at(i);
+        tok[u] = pass > 0 && i < end ? __ldcg(src_tok + i) : i;
+      }
+    }
+    for (int d = lane; d < 256; d += 32) z.hist[warp][d] = 0;
+    __syncwarp();
+    if (HELD) {
+#pragma unroll
+      for (int u = 0; u < kClusterHeld; ++u)
+        if (begin + 32 * u < end) rank_of[u] = sort_count(z, digit_of(key[u], shift, begin + 32 * u + lane < end));
+    } else {
+      for (int i = begin + lane; i - lane < end; i += 32) sort_count(z, digit_of(key_at(i), shift, i < end));
+    }
+    sort_offsets(z, [&](int t) {
+      if (t < 256) z.totals[t] = z.quarter[0][t] + z.quarter[1][t] + z.quarter[2][t] + z.quarter[3][t];
+      cluster.sync();
+      int2 n = make_int2(0, 0);
+      if (t < 256) {
+        int x[ctas];
+#pragma unroll
+        for (int c = 0; c < ctas; ++c) x[c] = cluster.map_shared_rank(z.totals, c)[t];
+#pragma unroll
+        for (int c = 0; c < ctas; ++c) {
+          if (c < rank) n.x += x[c];
+          n.y += x[c];
         }
       }
-    }
-#pragma unroll
-    for (int d = lane; d < 256; d += 32) hist[warp][d] = 0;
-    __syncwarp();
-    auto count = [&](int i, uint32_t k) {
-      const unsigned digit = i < end ? (k >> shift) & 255u : 256u;
-      const unsigned same = __match_any_sync(0xffffffffu, digit);
-      if (digit < 256 && (same & below) == 0) hist[warp][digit] += __popc(same);
-      __syncwarp();
-    };
+      return n;
+    });
     if (HELD) {
 #pragma unroll
-      for (int u = 0; u < kHeld; ++u)
-        if (begin + 32 * u < end) count(begin + 32 * u + lane, key[u]);
-    } else {
-      for (int i = begin + lane; i - lane < end; i += 32) count(i, i < end ? key_at(i) : 0u);
-    }
-    __syncthreads();
-    // exclusive sum of a digit over the warps, a quarter of them per thread
-    int* column = &hist[8 * (tid >> 8)][tid & 255];
-    int sum = 0;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      const int n = column[256 * w];
-      column[256 * w] = sum;
-      sum += n;
-    }
-    quarter[tid >> 8][tid & 255] = sum;
-    __syncthreads();
-    if (tid < 256) totals[tid] = quarter[0][tid] + quarter[1][tid] + quarter[2][tid] + quarter[3][tid];
-    cluster.sync();
-    int before = 0, all = 0;
-    if (tid < 256) {
-      for (int c = 0; c < ctas; ++c) {
-        const int n = cluster.map_shared_rank(totals, c)[tid];
-        if (c < rank) before += n;
-        all += n;
+      for (int u = 0; u < kClusterHeld; ++u) {
+        if (begin + 32 * u + lane < end) {
+          const int at = sort_place(z, digit_of(key[u], shift, true), rank_of[u]);
+          s.area.key[pass & 1][at] = key[u];
+          s.area.tok[pass & 1][at] = tok[u];
+        }
       }
-    }
-    // exclusive sum of `all` over the digits
-    int upto = all;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int n = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += n;
-    }
-    if (tid < 256 && lane == 31) warp_part[warp] = upto;
-    __syncthreads();
-    if (tid < 256) {
-      int start = upto - all;
-      for (int w = 0; w < warp; ++w) start += warp_part[w];
-      base[tid] = start + before;
-    }
-    __syncthreads();
-    auto place = [&](int i, uint32_t k, int t) {
-      const unsigned digit = i < end ? (k >> shift) & 255u : 256u;
-      const unsigned same = __match_any_sync(0xffffffffu, digit);
-      if (digit < 256) {
-        int at = base[digit] + hist[warp][digit] + __popc(same & below);
-        for (int q = 0; q < (warp >> 3); ++q) at += quarter[q][digit];
-        dst_key[at] = k;
-        dst_tok[at] = t;
-      }
-      __syncwarp();
-      if (digit < 256 && (same & below) == 0) hist[warp][digit] += __popc(same);
-      __syncwarp();
-    };
-    if (HELD) {
-#pragma unroll
-      for (int u = 0; u < kHeld; ++u)
-        if (begin + 32 * u < end) place(begin + 32 * u + lane, key[u], tok[u]);
     } else {
-      for (int i = begin + lane; i - lane < end; i += 32)
-        place(i, i < end ? key_at(i) : 0u, (pass > 0 && i < end) ? __ldcg(src_tok + i) : i);
+      // counted once more, now from the offsets on: sort_count's rank is then the place inside the CTA's share
+      for (int i = begin + lane; i - lane < end; i += 32) {
+        const uint32_t key = key_at(i);
+        const unsigned digit = digit_of(key, shift, i < end);
+        const int rank = sort_count(z, digit);
+        if (i < end) {
+          int at = z.base[digit] + rank;
+          for (int q = 0; q < (warp >> 3); ++q) at += z.quarter[q][digit];
+          s.area.key[pass & 1][at] = key;
+          s.area.tok[pass & 1][at] = pass > 0 ? __ldcg(src_tok + i) : i;
+        }
+      }
     }
     cluster.sync();      // the next pass reads what other CTAs wrote; nobody reads totals any more
   }
@@ -221,7 +316,6 @@ struct Table {
   float* part;
   void* out;             // [rows][h]
   int rows, stride;
-  int fp32, accumulate;
   float scale;
 };
 
@@ -249,14 +343,18 @@ __device__ __forceinline__ void add8(float* acc, const mb::bf16x8& v) {
   for (int k = 0; k < 8; ++k) acc[k] += f[k];
 }
 
+// How a table is written; a template parameter, because all four in every place cost registers and a third of the time.
+enum Mode : int { kBf16 = 0, kBf16Add = 1, kF32 = 2, kF32Add = 3 };
+
 // out[0..8) (+)= scale * acc, rounded once
+template <int MODE>
 __device__ __forceinline__ void write8(const Table& t, long at, const float* acc) {
   float f[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) f[k] = acc[k] * t.scale;
-  if (t.fp32) {
+  if (MODE >= kF32) {
     float4* dst = reinterpret_cast<float4*>(static_cast<float*>(t.out) + at);
-    if (t.accumulate) {
+    if (MODE == kF32Add) {
       const float4 x = dst[0], y = dst[1];
       f[0] += x.x; f[1] += x.y; f[2] += x.z; f[3] += x.w;
       f[4] += y.x; f[5] += y.y; f[6] += y.z; f[7] += y.w;
@@ -265,172 +363,182 @@ __device__ __forceinline__ void write8(const Table& t, long at, const float* acc
     dst[1] = make_float4(f[4], f[5], f[6], f[7]);
   } else {
     mb::bf16x8* dst = reinterpret_cast<mb::bf16x8*>(static_cast<__nv_bfloat16*>(t.out) + at);
-    if (t.accumulate) add8(f, *dst);
+    if (MODE == kBf16Add) add8(f, *dst);
     *dst = mb::pack8(f);
   }
 }
 
-constexpr int kRows = 8;         // table rows of a CTA
 constexpr int kSumThreads = 256;
+constexpr int kZeroRows = 16;
 
-// Rows of up to kTile tokens (and rows without any): one thread per 8 columns of a row.
-__device__ __forceinline__ void sum_rows(const Table& t, const __nv_bfloat16* dout, int tokens, int h, int block) {
-  __shared__ int start[kRows + 1];
-  const int warp = threadIdx.x >> 5;
-  const int r0 = block * kRows, nrows = min(kRows, t.rows - r0), vpr = h >> 3;
-  if (t.key) {
-    if (warp < 2) {
-      const int at = warp_lower_bound(t.key, tokens, static_cast<uint32_t>(warp ? r0 + nrows : r0));
-      if ((threadIdx.x & 31) == 0) start[warp ? nrows : 0] = at;
-    }
-    __syncthreads();
-    if (threadIdx.x > 0 && threadIdx.x < nrows) {
-      int lo = start[0], hi = start[nrows];
-      const uint32_t x = r0 + threadIdx.x;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (t.key[mid] < x) lo = mid + 1;
-        else hi = mid;
-      }
-      start[threadIdx.x] = lo;
-    }
-    __syncthreads();
+// A part of a row that lies in several tiles has been written: the warp that counts the last one adds all in order.
+// [a, b): the row's sorted tokens.
+template <int MODE>
+__device__ __noinline__ void count_part(const Table& t, int h, int chunk, int chunks, uint32_t row, int a, int b) {
+  const int lane = threadIdx.x & 31, c = chunk * 32 + lane;
+  const int tile0 = a / kTile, parts = (b - 1) / kTile - tile0 + 1;
+  const int slot0 = 2 * tile0 + (a % kTile != 0);      // in the row's first tile; in the others the row is the first
+  __threadfence();
+  __syncwarp();
+  int last = 0;
+  if (lane == 0) last = atomicAdd(&t.arrived[slot0 * chunks + chunk], 1) == parts - 1;
+  if (!__shfl_sync(0xffffffffu, last, 0)) return;
+  __threadfence();
+  if (c >= (h >> 3)) return;
+  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int q = 0; q < parts; ++q) {
+    const float4* src = reinterpret_cast<const float4*>(t.part + static_cast<long>(q ? 2 * (tile0 + q) : slot0) * h + 8 * c);
+    const float4 x = __ldcg(src), y = __ldcg(src + 1);
+    sum[0] += x.x; sum[1] += x.y; sum[2] += x.z; sum[3] += x.w;
+    sum[4] += y.x; sum[5] += y.y; sum[6] += y.z; sum[7] += y.w;
   }
-  for (int i = threadIdx.x; i < nrows * vpr; i += kSumThreads) {
-    const int r = i / vpr, c = (i - r * vpr) * 8;
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (t.key) {
-      const int a = start[r], b = start[r + 1];
-      if (b - a > kTile || (a == b && t.accumulate)) continue;      // summed by sum_long; nothing to add
-      for (int j = a; j < b; j += 4) {
-        mb::bf16x8 v[4];
+  write8<MODE>(t, static_cast<long>(row) * h + 8 * c, sum);
+}
+
+// One warp: the columns of a chunk, of the rows whose tokens are in a tile of kTile sorted ones.  However the ids are
+// distributed, a warp has the same work.  A row that lies in several tiles leaves a part in each.
+template <int MODE>
+__device__ __forceinline__ void sum_tile(const Table& t, const __nv_bfloat16* dout, int tokens, int h, int tile, int chunk,
+                                         int chunks) {
+  const int lane = threadIdx.x & 31, vpr = h >> 3, c = chunk * 32 + lane;
+  const bool live = c < vpr;
+  const int p0 = tile * kTile, all = min(kTile, tokens - p0);
+  const uint32_t key = lane < all ? t.key[p0 + lane] : 0xffffffffu;
+  const int tok = lane < all ? t.tok[p0 + lane] : 0;
+  const int n = __popc(__ballot_sync(0xffffffffu, key < static_cast<uint32_t>(t.rows)));      // tokens of no row come last
+  if (n == 0) return;
+  const uint32_t before = p0 > 0 ? t.key[p0 - 1] : 0xffffffffu;
+  const uint32_t after = n == all && p0 + n < tokens ? t.key[p0 + n] : 0xffffffffu;
+  uint32_t left = __shfl_up_sync(0xffffffffu, key, 1);
+  if (lane == 0) left = before;
+  // bit j: token j is the first of its row
+  const unsigned starts = __ballot_sync(0xffffffffu, lane < n && key != left);
+  const bool begun = !(starts & 1u), goes_on = after == __shfl_sync(0xffffffffu, key, n - 1);
+  float acc[8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (j + u < b) v[u] = *reinterpret_cast<const mb::bf16x8*>(dout + static_cast<long>(t.tok[j + u]) * h + c);
+  for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+  auto store_part = [&](int slot) {
+    if (!live) return;
+    float4* dst = reinterpret_cast<float4*>(t.part + (2l * tile + slot) * h + 8 * c);
+    dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+  };
+  int from = 0, first_end = n;                     // first token of the row in hand; end of the tile's first row
+  for (int j = 0; j < n; j += 8) {
+    mb::bf16x8 v[8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (j + u < b) add8(acc, v[u]);
+    for (int u = 0; u < 8; ++u) {
+      const long at = __shfl_sync(0xffffffffu, tok, (j + u) & 31);
+      if (live && j + u < n) v[u] = *reinterpret_cast<const mb::bf16x8*>(dout + at * h + 8 * c);
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (j + u < n) {
+        if (j + u > 0 && ((starts >> (j + u)) & 1u)) {
+          const long row = __shfl_sync(0xffffffffu, key, from);
+          if (from == 0) first_end = j + u;
+          if (from == 0 && begun) store_part(0);
+          else if (live) write8<MODE>(t, row * h + 8 * c, acc);
+          from = j + u;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+        }
+        add8(acc, v[u]);
       }
+    }
+  }
+  const uint32_t row = __shfl_sync(0xffffffffu, key, from), row0 = __shfl_sync(0xffffffffu, key, 0);
+  if (goes_on || (from == 0 && begun)) store_part(from != 0);
+  else if (live) write8<MODE>(t, static_cast<long>(row) * h + 8 * c, acc);
+  if (begun) {
+    const int a = warp_lower_bound(t.key, tokens, row0);
+    const int b = first_end == n && goes_on ? warp_lower_bound(t.key, tokens, row0 + 1) : p0 + first_end;
+    count_part<MODE>(t, h, chunk, chunks, row0, a, b);
+  }
+  if (goes_on && (from != 0 || !begun))
+    count_part<MODE>(t, h, chunk, chunks, row, p0 + from, warp_lower_bound(t.key, tokens, row + 1));
+}
+
+// Rows that get no token, where the table is stored.
+template <int MODE>
+__device__ __forceinline__ void zero_rows(const Table& t, int tokens, int h, int block) {
+  __shared__ uint8_t used[kZeroRows];
+  __shared__ int range[2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r0 = block * kZeroRows, nrows = min(kZeroRows, t.rows - r0);
+  if (threadIdx.x < kZeroRows) used[threadIdx.x] = 0;
+  if (warp < 2) {
+    const int at = warp_lower_bound(t.key, tokens, static_cast<uint32_t>(warp ? r0 + nrows : r0));
+    if (lane == 0) range[warp] = at;
+  }
+  __syncthreads();
+  for (int i = range[0] + threadIdx.x; i < range[1]; i += kSumThreads) used[t.key[i] - r0] = 1;
+  __syncthreads();
+  const int bytes = h * (MODE >= kF32 ? 4 : 2);
+  uint8_t* out = static_cast<uint8_t*>(t.out) + static_cast<long>(r0) * bytes;
+  const bool wide = ((reinterpret_cast<uintptr_t>(t.out) | bytes) & 31) == 0;      // whole sectors
+  for (int r = warp; r < nrows; r += kSumThreads / 32) {
+    if (used[r]) continue;
+    uint8_t* row = out + static_cast<long>(r) * bytes;
+    if (wide) {
+      for (int at = 32 * lane; at < bytes; at += 1024)
+        asm volatile("st.global.v8.b32 [%0], {%1, %1, %1, %1, %1, %1, %1, %1};\n" ::"l"(row + at), "r"(0) : "memory");
     } else {
-      if (r0 + r >= t.stride && t.accumulate) continue;
-      if (r0 + r < t.stride)
-        for (long j = r0 + r; j < tokens; j += t.stride) add8(acc, *reinterpret_cast<const mb::bf16x8*>(dout + j * h + c));
-    }
-    write8(t, static_cast<long>(r0 + r) * h + c, acc);
-  }
-}
-
-// Rows of more than kTile tokens: a CTA adds the tokens that such a row has among kTile sorted ones; a tile touches two
-// of these rows at most, the row of its first token and that of its last.  The CTA that counts the last part of a row adds
-// the parts in order.
-__device__ void sum_long(const Table& t, const __nv_bfloat16* dout, int tokens, int h, int tile, int slice, int slices) {
-  __shared__ int seg[2];
-  __shared__ float red[3][kCols];
-  __shared__ int last;
-  const int warp = threadIdx.x >> 5, tid = threadIdx.x;
-  const int p0 = tile * kTile, p1 = min(p0 + kTile, tokens) - 1;
-  const int group = tid >> 6, c = slice * kCols + (tid & 63) * 8;      // 4 groups of tokens x 64 vectors
-  for (int w = 0; w < 2; ++w) {
-    const uint32_t k = t.key[w ? p1 : p0];
-    if (k >= static_cast<uint32_t>(t.rows) || (w && k == t.key[p0])) continue;
-    // more than kTile equal keys in a row reach kTile - (tokens of this tile) further on one side
-    const int left = w ? p0 : max(0, p0 - kTile), right = min(tokens - 1, p1 + kTile);
-    __syncthreads();
-    if (warp < 2) {
-      const int at = warp_lower_bound(t.key + left, right + 1 - left, k + warp) + left;
-      if ((tid & 31) == 0) seg[warp] = at;
-    }
-    __syncthreads();
-    if (seg[1] - seg[0] <= kTile) continue;
-    __syncthreads();
-    if (warp < 2) {
-      const int at = warp_lower_bound(t.key, tokens, k + warp);
-      if ((tid & 31) == 0) seg[warp] = at;
-    }
-    __syncthreads();
-    const int a = seg[0], b = seg[1];
-    const int from = max(a, p0), to = min(b, p1 + 1), n = to - from;
-    const int j0 = from + n * group / 4, j1 = from + n * (group + 1) / 4;
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (c < h) {
-      for (int j = j0; j < j1; j += 4) {
-        mb::bf16x8 v[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (j + u < j1) v[u] = *reinterpret_cast<const mb::bf16x8*>(dout + static_cast<long>(t.tok[j + u]) * h + c);
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (j + u < j1) add8(acc, v[u]);
-      }
-      if (group > 0)
-#pragma unroll
-        for (int u = 0; u < 8; ++u) red[group - 1][(tid & 63) * 8 + u] = acc[u];
-    }
-    __syncthreads();
-    if (group == 0 && c < h) {
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int x = (tid & 63) * 8 + u;
-        acc[u] += red[0][x] + (red[1][x] + red[2][x]);
-      }
-      float4* dst = reinterpret_cast<float4*>(t.part + (2l * tile + w) * h + c);
-      dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-    }
-    __threadfence();
-    __syncthreads();
-    const int tile0 = a / kTile, parts = (b - 1) / kTile - tile0 + 1;
-    const int slot0 = 2 * tile0 + (a % kTile != 0);      // of the row's first tile; later tiles begin inside the row
-    if (tid == 0) last = atomicAdd(&t.arrived[slot0 * slices + slice], 1) == parts - 1;
-    __syncthreads();
-    if (!last) continue;
-    __threadfence();
-    if (group == 0 && c < h) {
-      float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      for (int q = 0; q < parts; q += 4) {
-        float4 x[4][2];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (q + u >= parts) break;
-          const float4* src = reinterpret_cast<const float4*>(t.part + static_cast<long>(q + u ? 2 * (tile0 + q + u) : slot0) * h + c);
-          x[u][0] = __ldcg(src);
-          x[u][1] = __ldcg(src + 1);
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (q + u >= parts) break;
-          sum[0] += x[u][0].x; sum[1] += x[u][0].y; sum[2] += x[u][0].z; sum[3] += x[u][0].w;
-          sum[4] += x[u][1].x; sum[5] += x[u][1].y; sum[6] += x[u][1].z; sum[7] += x[u][1].w;
-        }
-      }
-      write8(t, static_cast<long>(k) * h + c, sum);
+      for (int at = 16 * lane; at < bytes; at += 512) *reinterpret_cast<uint4*>(row + at) = make_uint4(0, 0, 0, 0);
     }
   }
 }
 
-// blocks: [long rows of table 0][of table 1][rows of table 0][of table 1]
-__global__ void __launch_bounds__(kSumThreads, 6)
-embed_sum_kernel(const __grid_constant__ Table t0, const __grid_constant__ Table t1, const __nv_bfloat16* dout, int tokens, int h, int long0, int long1,
-                 int rows0, int slices) {
+// A row of positions by place: token r of every sample.  One warp: a row's columns of a chunk.
+__device__ __forceinline__ void sum_stride(const Table& t, const __nv_bfloat16* dout, int tokens, int h, int row, int chunk) {
+  const int c = chunk * 32 + (threadIdx.x & 31);
+  if (c >= (h >> 3)) return;
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (row < t.stride) {
+#pragma unroll 4
+    for (long j = row; j < tokens; j += t.stride) add8(acc, *reinterpret_cast<const mb::bf16x8*>(dout + j * h + 8 * c));
+  }
+  write8<kBf16>(t, static_cast<long>(row) * h + 8 * c, acc);
+}
+
+// What the blocks do: items of sum_tile (or rows of sum_stride), one per warp, of table 0 and of table 1, then rows without a
+// token of table 0 and of table 1.  The sums wait for memory, the zeros fill its queues behind them.
+struct Blocks {
+  int sums0, sums1, zeros0;      // numbers of blocks; the rest are the zeros of table 1
+};
+template <int MODE>
+__global__ void __launch_bounds__(kSumThreads, 4)
+embed_sum_kernel(const __grid_constant__ Table t0, const __grid_constant__ Table t1, const __nv_bfloat16* dout, int tokens,
+                 int h, int chunks, const Blocks blocks) {
   mb::wait_for_previous_kernel();
   int b = blockIdx.x;
-  if (b < long0 + long1) {
-    const bool second = b >= long0;
-    if (second) b -= long0;
-    sum_long(second ? t1 : t0, dout, tokens, h, b / slices, b % slices, slices);
+  if (b < blocks.sums0 + blocks.sums1) {
+    const bool second = b >= blocks.sums0;
+    if (second) b -= blocks.sums0;
+    const long item = static_cast<long>(b) * (kSumThreads / 32) + (threadIdx.x >> 5);
+    const int at = static_cast<int>(item / chunks), chunk = static_cast<int>(item - static_cast<long>(at) * chunks);
+    const bool inside = static_cast<long>(at) * kTile < tokens;
+    if (!second) {      // (a reference to one of the two would put both in local memory)
+      if (inside) sum_tile<MODE>(t0, dout, tokens, h, at, chunk, chunks);
+    } else if (t1.key) {
+      if (inside) sum_tile<kBf16>(t1, dout, tokens, h, at, chunk, chunks);
+    } else if (at < t1.rows) {
+      sum_stride(t1, dout, tokens, h, at, chunk);
+    }
     return;
   }
-  b -= long0 + long1;
-  if (b < rows0) sum_rows(t0, dout, tokens, h, b);
-  else sum_rows(t1, dout, tokens, h, b - rows0);
+  b -= blocks.sums0 + blocks.sums1;
+  if (b < blocks.zeros0) zero_rows<MODE & ~1>(t0, tokens, h, b);
+  else zero_rows<kBf16>(t1, tokens, h, b - blocks.zeros0);
 }
 
 size_t up16(size_t n) { return (n + 15) & ~static_cast<size_t>(15); }
-int tiles_of(int tokens) { return tokens > kTile ? (tokens + kTile - 1) / kTile : 0; }
-int slices_of(int h) { return (h + kCols - 1) / kCols; }
+int tiles_of(int tokens) { return static_cast<int>((tokens + static_cast<long>(kTile) - 1) / kTile); }
+int chunks_of(int h) { return (h + kChunk - 1) / kChunk; }
 
 size_t area_bytes(int tokens, int h) {
-  return 4 * up16(4ul * tokens) + up16(8ul * tiles_of(tokens) * slices_of(h)) + up16(8ul * tiles_of(tokens) * h);
+  return 4 * up16(4ul * tokens) + up16(8ul * tiles_of(tokens) * chunks_of(h)) + up16(8ul * tiles_of(tokens) * h);
 }
 Area make_area(uint8_t* at, int tokens, int h) {
   Area a;
@@ -440,7 +548,7 @@ Area make_area(uint8_t* at, int tokens, int h) {
     a.tok[i] = reinterpret_cast<int*>(at + (2 * i + 1) * n);
   }
   a.arrived = reinterpret_cast<int*>(at + 4 * n);
-  a.part = reinterpret_cast<float*>(at + 4 * n + up16(8ul * tiles_of(tokens) * slices_of(h)));
+  a.part = reinterpret_cast<float*>(at + 4 * n + up16(8ul * tiles_of(tokens) * chunks_of(h)));
   return a;
 }
 Sort make_sort(const int64_t* ids, int64_t v0, int rows, uint8_t* at, int tokens, int h) {
@@ -453,7 +561,7 @@ Sort make_sort(const int64_t* ids, int64_t v0, int rows, uint8_t* at, int tokens
   s.area = make_area(at, tokens, h);
   return s;
 }
-Table make_table(const Sort& s, void* out, int fp32, int accumulate, float scale) {
+Table make_table(const Sort& s, void* out, float scale) {
   Table t;
   t.key = s.area.key[(s.passes + 1) & 1];
   t.tok = s.area.tok[(s.passes + 1) & 1];
@@ -462,8 +570,6 @@ Table make_table(const Sort& s, void* out, int fp32, int accumulate, float scale
   t.out = out;
   t.rows = s.rows;
   t.stride = 0;
-  t.fp32 = fp32;
-  t.accumulate = accumulate;
   t.scale = scale;
   return t;
 }
@@ -509,41 +615,65 @@ MB_API int mb_embed_bwd(const int64_t* ids, const int64_t* pos, const void* dout
   memset(t, 0, sizeof(t));
   if (sort0) {
     s[nsort] = make_sort(ids, v0, rows, at, tokens, h);
-    t[0] = make_table(s[nsort++], dwte, dwte_fp32, accumulate, scale);
+    t[0] = make_table(s[nsort++], dwte, scale);
   }
   if (sort1) {
     s[nsort] = make_sort(pos, 0, positions, at + nsort * area_bytes(tokens, h), tokens, h);
-    t[1] = make_table(s[nsort++], dwpe, 0, 0, 1.f);
+    t[1] = make_table(s[nsort++], dwpe, 1.f);
   } else if (dwpe) {
     t[1].out = dwpe;
     t[1].rows = positions;
     t[1].stride = seq;
     t[1].scale = 1.f;
   }
-  const int slices = slices_of(h), tiles = tiles_of(tokens);
+  const int chunks = chunks_of(h), tiles = tiles_of(tokens);
   if (nsort && tokens > 0) {
-    // one CTA up to 2048 tokens: a cluster's exchange costs more than the shorter stretches of its warps save
-    cudaLaunchConfig_t cfg;
-    memset(&cfg, 0, sizeof(cfg));
-    const int ctas = tokens <= 2048 ? 1 : kSortCluster;
-    cfg.gridDim = dim3(ctas * nsort);
-    cfg.blockDim = dim3(kSortThreads);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ctas;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const bool held = tokens <= ctas * kSortThreads * kHeld;
-    if (cudaLaunchKernelEx(&cfg, held ? embed_sort_kernel<true> : embed_sort_kernel<false>, s[0], s[1], tokens, 2 * tiles * slices) != cudaSuccess) return -4;
+    const long counters64 = 2l * tiles * chunks;
+    if (counters64 > 0x7fffffffl) return -1;
+    const int counters = static_cast<int>(counters64);
+    if (tokens <= kBlockSort) {
+      int dev = 0;
+      static bool configured[64] = {};
+      if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -3;
+      if (!configured[dev]) {
+        if (cudaFuncSetAttribute(embed_sort_block_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBlockSortBytes) !=
+            cudaSuccess)
+          return -3;
+        configured[dev] = true;
+      }
+      embed_sort_block_kernel<<<nsort, kSortThreads, kBlockSortBytes, stream>>>(s[0], s[1], tokens, counters);
+      if (cudaGetLastError() != cudaSuccess) return -4;
+    } else {
+      cudaLaunchConfig_t cfg;
+      memset(&cfg, 0, sizeof(cfg));
+      cfg.gridDim = dim3(kSortCluster * nsort);
+      cfg.blockDim = dim3(kSortThreads);
+      cfg.stream = stream;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = kSortCluster;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      const bool held = tokens <= kSortCluster * kSortThreads * kClusterHeld;
+      if (cudaLaunchKernelEx(&cfg, held ? embed_sort_cluster_kernel<true> : embed_sort_cluster_kernel<false>, s[0], s[1], tokens,
+                             counters) != cudaSuccess)
+        return -4;
+    }
   }
-  const long rows0 = sort0 ? (rows + kRows - 1) / kRows : 0, rows1 = dwpe ? (positions + kRows - 1) / kRows : 0;
-  const long long0 = sort0 ? static_cast<long>(tiles) * slices : 0, long1 = sort1 ? static_cast<long>(tiles) * slices : 0;
-  const long blocks = rows0 + rows1 + long0 + long1;
+  auto groups = [](long n, int per) { return (n + per - 1) / per; };
+  const long sums0 = sort0 ? groups(static_cast<long>(tiles) * chunks, kSumThreads / 32) : 0;
+  const long sums1 = sort1 ? groups(static_cast<long>(tiles) * chunks, kSumThreads / 32)
+                           : (dwpe ? groups(static_cast<long>(positions) * chunks, kSumThreads / 32) : 0);
+  const long zeros0 = sort0 && !accumulate ? groups(rows, kZeroRows) : 0, zeros1 = sort1 ? groups(positions, kZeroRows) : 0;
+  const long blocks = sums0 + sums1 + zeros0 + zeros1;
   if (blocks == 0) return 0;
   if (blocks > 0x7fffffffl) return -1;
+  Blocks of;
+  of.sums0 = static_cast<int>(sums0);
+  of.sums1 = static_cast<int>(sums1);
+  of.zeros0 = static_cast<int>(zeros0);
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
@@ -554,8 +684,10 @@ MB_API int mb_embed_bwd(const int64_t* ids, const int64_t* pos, const void* dout
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = nsort && tokens > 0 ? 1 : 0;
-  if (cudaLaunchKernelEx(&cfg, embed_sum_kernel, t[0], t[1], static_cast<const __nv_bfloat16*>(dout), tokens, h,
-                         static_cast<int>(long0), static_cast<int>(long1), static_cast<int>(rows0), slices) != cudaSuccess)
+  const auto kernel = dwte_fp32 ? (accumulate ? embed_sum_kernel<kF32Add> : embed_sum_kernel<kF32>)
+                                : (accumulate ? embed_sum_kernel<kBf16Add> : embed_sum_kernel<kBf16>);
+  if (cudaLaunchKernelEx(&cfg, kernel, t[0], t[1], static_cast<const __nv_bfloat16*>(dout), tokens, h, chunks, of) !=
+      cudaSuccess)
     return -4;
   return 0;
 }

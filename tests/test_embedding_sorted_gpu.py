@@ -30,7 +30,7 @@ def _ids(kind, b, s, v, start):
 
 @pytest.mark.parametrize("kind", ["uniform", "one", "none", "ends", "skewed"])
 @pytest.mark.parametrize("b,s,h,v", [(1, 1, 8, 3), (2, 65, 24, 255), (1, 64, 128, 256), (3, 777, 520, 1003),
-                                     (1, 5003, 1024, 70001), (4, 2048, 64, 300)])
+                                     (1, 5003, 1024, 70001), (4, 2048, 64, 300), (2, 17001, 16, 500)])
 @pytest.mark.parametrize("positions", ["none", "row", "given"])
 def test_forward_and_gradients(kind, b, s, h, v, positions):
     torch.manual_seed(7)
