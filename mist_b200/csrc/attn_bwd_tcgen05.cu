@@ -425,23 +425,10 @@ constexpr int kDeltaRows = 4;
 __host__ __device__ inline unsigned delta_first_row(unsigned block, unsigned thread) {
   return (block * 16u + (thread >> 4)) * kDeltaRows;
 }
-// What the backward pass of packed sequences also needs: the count of claimed work items set to 0, the fp32 dQ of tiles that
-// more than one block of keys sees set to 0, and dQ itself where no key is visible.
-struct DeltaExtras {
-  int* claimed;
-  float* dq_acc;
-  const uint8_t* single;
-  int single_bit;
-  const float* lse;
-  __nv_bfloat16* dq;
-  long dq_ts, dq_hs;
-};
-template <bool PACKED>
 __global__ void __launch_bounds__(256)
 attn_delta_kernel(const __nv_bfloat16* __restrict__ dout, const __nv_bfloat16* __restrict__ o,
                   float* __restrict__ delta, int batch, int sq, int nh, int d, long do_bs,
-                  long do_ts, long do_hs, long o_bs, long o_ts, long o_hs, const DeltaExtras e) {
-  if (PACKED && blockIdx.x == 0 && threadIdx.x == 0) *e.claimed = 0;
+                  long do_ts, long do_hs, long o_bs, long o_ts, long o_hs) {
   const unsigned first = delta_first_row(blockIdx.x, threadIdx.x);
   const int sub = threadIdx.x & 15;
   const unsigned total = static_cast<unsigned>(batch) * sq * nh;
@@ -470,15 +457,58 @@ attn_delta_kernel(const __nv_bfloat16* __restrict__ dout, const __nv_bfloat16* _
 #pragma unroll
     for (int m = 8; m > 0; m >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, m);
     if (sub == 0 && first + u < total) delta[at[u]] = acc;
-    if (PACKED && sub * 8 < d && first + u < total) {
-      const unsigned q = at[u] % sq, h = at[u] / sq;
-      if (!(e.single[q] & e.single_bit)) {
-        float4* dst = reinterpret_cast<float4*>(e.dq_acc + static_cast<size_t>(at[u]) * d + sub * 8);
-        dst[0] = dst[1] = make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      if (e.lse[at[u]] == -INFINITY)
-        *reinterpret_cast<uint4*>(e.dq + q * e.dq_ts + h * e.dq_hs + sub * 8) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// The same of packed sequences, [total][nh][d] -> delta [nh][total], and what their backward pass also needs: the count of
+// claimed work items set to 0, the fp32 dQ [nh][total][d] of tiles that more than one block of keys sees (rows whose `single`
+// lacks the bit) set to 0, and dQ itself where no key is visible.  A lane has 8 values; a warp takes as many rows as fit it and
+// does so four times at once (16 lanes per row, of which 10 worked, took 45 us for 8192 x 32 heads of 80).
+__global__ void __launch_bounds__(256)
+attn_delta_packed_kernel(const __nv_bfloat16* __restrict__ dout, const __nv_bfloat16* __restrict__ o,
+                         float* __restrict__ delta, int total, int nh, int d, const float* __restrict__ lse, int* claimed,
+                         float* __restrict__ dq_acc, const uint8_t* __restrict__ single, int single_bit,
+                         __nv_bfloat16* __restrict__ dq, long dq_ts, long dq_hs) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) *claimed = 0;
+  const int vpr = d >> 3, lane = threadIdx.x & 31, per_warp = 32 / vpr, sub = lane % vpr, mine = lane / vpr;
+  const long rows = static_cast<long>(total) * nh;
+  const long first = (blockIdx.x * 8l + (threadIdx.x >> 5)) * per_warp * kDeltaRows + mine;
+  const bool works = mine < per_warp;
+  mb::bf16x8 x[kDeltaRows], y[kDeltaRows];
+#pragma unroll
+  for (int u = 0; u < kDeltaRows; ++u) {
+    const long row = first + u * per_warp;
+    if (works && row < rows) {
+      x[u] = reinterpret_cast<const mb::bf16x8*>(dout)[row * vpr + sub];
+      y[u] = reinterpret_cast<const mb::bf16x8*>(o)[row * vpr + sub];
     }
+  }
+#pragma unroll
+  for (int u = 0; u < kDeltaRows; ++u) {
+    const long row = first + u * per_warp;
+    const bool live = works && row < rows;
+    float acc = 0.f;
+    if (live) {
+      float f[8], g[8];
+      mb::unpack8(x[u], f);
+      mb::unpack8(y[u], g);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) acc += f[k] * g[k];
+    }
+#pragma unroll
+    for (int m = 8; m > 0; m >>= 1) {
+      const float other = __shfl_down_sync(0xffffffffu, acc, m);
+      if (sub + m < vpr) acc += other;
+    }
+    if (!live) continue;
+    const int t = static_cast<int>(row / nh), h = static_cast<int>(row - static_cast<long>(t) * nh);
+    const long at = static_cast<long>(h) * total + t;
+    if (sub == 0) delta[at] = acc;
+    if (!(single[t] & single_bit)) {
+      float4* dst = reinterpret_cast<float4*>(dq_acc + at * d + sub * 8);
+      dst[0] = dst[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    if (lse[at] == -INFINITY) *reinterpret_cast<uint4*>(dq + t * dq_ts + h * dq_hs + sub * 8) = make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -622,9 +652,9 @@ MB_API int mb_attn_bwd(const void* dout, const void* q, const void* k, const voi
     long rows = static_cast<long>(batch) * sq * nh;
     if (rows > 0x7fffffff) return -1;
     long blocks = (rows + 16 * kDeltaRows - 1) / (16 * kDeltaRows);
-    attn_delta_kernel<false><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
+    attn_delta_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
         reinterpret_cast<const __nv_bfloat16*>(dout), reinterpret_cast<const __nv_bfloat16*>(o), delta, batch, sq,
-        nh, d, o_bs, o_ts, d, o_bs, o_ts, d, DeltaExtras());
+        nh, d, o_bs, o_ts, d, o_bs, o_ts, d);
   }
   if (cudaMemsetAsync(dq_acc, 0, sizeof(float) * batch * nh * static_cast<size_t>(sq) * d, stream) != cudaSuccess)
     return -4;
@@ -748,17 +778,11 @@ MB_API int mb_attn_bwd_packed(const void* dout, const void* q, const void* k, co
   float* dq_acc = reinterpret_cast<float*>(at + area.dq_acc);
   int* claimed = reinterpret_cast<int*>(at + area.claimed);
   if (total_q > 0) {
-    DeltaExtras e;
-    e.claimed = claimed;
-    e.dq_acc = dq_acc;
-    e.single = static_cast<const uint8_t*>(plan) + packed_single_offset(total_q, total_k, n);
-    e.single_bit = causal ? 2 : 1;
-    e.lse = lse;
-    e.dq = reinterpret_cast<__nv_bfloat16*>(dq);
-    e.dq_ts = dq_ts; e.dq_hs = dq_hs;
-    attn_delta_kernel<true><<<static_cast<unsigned>((rows + 16 * kDeltaRows - 1) / (16 * kDeltaRows)), 256, 0, stream>>>(
-        reinterpret_cast<const __nv_bfloat16*>(dout), reinterpret_cast<const __nv_bfloat16*>(o), delta, 1, total_q, nh, d,
-        rows * d, static_cast<long>(nh) * d, d, rows * d, static_cast<long>(nh) * d, d, e);
+    const long per_block = 8l * (32 / (d / 8)) * kDeltaRows;
+    attn_delta_packed_kernel<<<static_cast<unsigned>((rows + per_block - 1) / per_block), 256, 0, stream>>>(
+        reinterpret_cast<const __nv_bfloat16*>(dout), reinterpret_cast<const __nv_bfloat16*>(o), delta, total_q, nh, d, lse,
+        claimed, dq_acc, static_cast<const uint8_t*>(plan) + packed_single_offset(total_q, total_k, n), causal ? 2 : 1,
+        reinterpret_cast<__nv_bfloat16*>(dq), dq_ts, dq_hs);
   } else if (cudaMemsetAsync(claimed, 0, sizeof(int), stream) != cudaSuccess) {
     return -4;
   }

@@ -171,18 +171,22 @@ def check_kernel_types(*tensors):
             raise ValueError(f"the attention kernels take bf16 and head sizes of 16, 32, ... 128, not {t.dtype} of {t.shape[-1]}")
 
 
+def _forward(q, k, v, packed, scale, causal):
+    if not use_native(q):
+        return _reference_forward(q, k, v, packed, scale, causal)
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = _launch_forward((ptr(q), ptr(k), ptr(v)), (*q.stride()[:2], *k.stride()[:2], *v.stride()[:2]), o,
+                          (q.shape[1], k.shape[1], q.shape[2]), packed, scale, causal)
+    return o, lse
+
+
 class _PackedSequencesAttnFn(torch.autograd.Function):
     """q ``[total_q, heads, d]``, k and v ``[total_k, kv heads, d]``."""
 
     @staticmethod
     def forward(ctx, q, k, v, packed, scale, causal):
         ctx.packed, ctx.scale, ctx.causal = packed, scale, causal
-        if use_native(q):
-            o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            lse = _launch_forward((ptr(q), ptr(k), ptr(v)), (*q.stride()[:2], *k.stride()[:2], *v.stride()[:2]), o,
-                                  (q.shape[1], k.shape[1], q.shape[2]), packed, scale, causal)
-        else:
-            o, lse = _reference_forward(q, k, v, packed, scale, causal)
+        o, lse = _forward(q, k, v, packed, scale, causal)
         ctx.save_for_backward(q, k, v, o, lse)
         return o
 
@@ -261,6 +265,8 @@ def attention(q, k, v, packed: PackedSequences, scale: float, causal: bool):
     if use_native(q):
         check_kernel_types(q, k, v)
         q, k, v = _rows(q), _rows(k), _rows(v)
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        return _forward(q, k, v, packed, float(scale), bool(causal))[0]
     return _PackedSequencesAttnFn.apply(q, k, v, packed, float(scale), bool(causal))
 
 
