@@ -1134,6 +1134,11 @@ def _flat_positions(position_ids, ids):
     return position_ids.expand(ids.shape).long().contiguous()
 
 
+@functools.lru_cache(maxsize=1024)
+def _embed_workspace(tokens: int, h: int, with_positions: int) -> int:
+    return native.kernels().mb_embed_bwd_workspace(tokens, h, with_positions)
+
+
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, wte, wpe, v0, scale, pos):
@@ -1191,8 +1196,7 @@ class _EmbeddingFn(torch.autograd.Function):
         dout = dout.contiguous()
         if ptr(dout) % 16:
             dout = dout.clone()
-        area = native.kernels().mb_embed_bwd_workspace(b * s, h, int(want_wpe and pos is not None))
-        workspace = torch.empty(area, dtype=torch.uint8, device=wte.device)
+        workspace = torch.empty(_embed_workspace(b * s, h, int(want_wpe and pos is not None)), dtype=torch.uint8, device=wte.device)
         call("mb_embed_bwd", ptr(ids), ptr(pos), ptr(dout), ptr(dwte), ptr(dwpe), b * s, s, h, ctx.v0, wte.shape[0],
              wpe.shape[0] if want_wpe else 0, ctx.scale, int(dwte is not None and dwte.dtype == torch.float32),
              int(direct and accumulate), ptr(workspace), stream())
@@ -1223,9 +1227,9 @@ def embedding(ids, wte, wpe=None, vocab_start: int = 0, scale: float = 1.0, posi
         raise ValueError(f"{ids.shape[1]} positions, but the table has {wpe.shape[0]}")
     pos = _flat_positions(position_ids, ids) if wpe is not None else None
     if use_native(wte):
-        for name, t in (("wte", wte), ("wpe", wpe)):
-            if t is not None and (t.dtype != torch.bfloat16 or not t.is_contiguous() or t.shape[1] != wte.shape[1]
-                                  or t.shape[1] % 8 or t.device != ids.device):
+        for name, t in (("wte", wte),) if wpe is None else (("wte", wte), ("wpe", wpe)):
+            if (t.dtype != torch.bfloat16 or not t.is_contiguous() or t.shape[1] != wte.shape[1]
+                    or t.shape[1] % 8 or t.device != ids.device):
                 raise ValueError(f"{name}: contiguous bf16 rows of a multiple of 8 values on the device of the ids expected")
         ids = ids.long().contiguous()
     return _EmbeddingFn.apply(ids, wte, wpe, int(vocab_start), float(scale), pos)

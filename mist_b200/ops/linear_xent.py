@@ -8,7 +8,7 @@ followed by mist/modules/losses.py:48-176, which hold ``[tokens, vocabulary]`` l
 """
 from __future__ import annotations
 
-from typing import Optional
+import functools
 
 import torch
 
@@ -31,6 +31,12 @@ def piece_columns(rows: int, vocab: int) -> int:
     most = max(256, F.Settings.xent_piece_bytes // (2 * max(rows, 1)) // 256 * 256)
     pieces = -(-vocab // most)
     return min(vocab, -(-(-(-vocab // pieces)) // 256) * 256)
+
+
+@functools.lru_cache(maxsize=1024)
+def _backward_bytes(*sizes):
+    """Workspace of the backward pass: a function of the sizes alone."""
+    return native.kernels().mb_xent_linear_bwd_workspace(*sizes)
 
 
 def _combine_over_group(stats, labels, ignore_index, group):
@@ -108,7 +114,7 @@ class _LinearXentFn(torch.autograd.Function):
         elif use_native(x2):
             w2, piece, ctas = _rows(weight, k), piece_columns(rows, vocab), F.Settings.gemm_max_ctas
             fp32 = int(dw is not None and dw.dtype == torch.float32)
-            area = native.kernels().mb_xent_linear_bwd_workspace(rows, vocab, k, piece, want_x, want_w, want_b, fp32, add, ctas)
+            area = _backward_bytes(rows, vocab, k, piece, want_x, want_w, want_b, fp32, add, ctas)
             workspace = torch.empty(area, dtype=torch.uint8, device=x2.device)
             call("mb_xent_linear_bwd", ptr(x2), ptr(w2), ptr(bias), ptr(labels), ptr(lse), ptr(gloss), ptr(dx), ptr(dw), ptr(db),
                  rows, vocab, k, x2.stride(0), w2.stride(0), 0 if dw is None else dw.stride(0), fp32, add, 0, ctx.v0, ctx.ignore,

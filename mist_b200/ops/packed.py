@@ -6,12 +6,32 @@ nothing is read back to the host (reference: csrc/flash_attn/flash_api.cpp:427, 
 with offsets that mist/modules/mha.py:1233-1243 derives from a padding mask)."""
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
 
 from . import native
 from .native import call, ptr, stream, use_native
+
+
+# what the library says of sizes alone
+@functools.lru_cache(maxsize=1024)
+def _plan_bytes(n, total_q, total_k):
+    return native.kernels().mb_packed_plan_bytes(n, total_q, total_k)
+
+
+@functools.lru_cache(maxsize=1024)
+def _counters(n, total_q, heads):
+    return native.kernels().mb_attn_fwd_packed_counters(n, total_q, heads)
+
+
+@functools.lru_cache(maxsize=1024)
+def _backward_sizes(total_q, total_k, nh, nkv, d):
+    """Query heads of a group that a CTA sums, bytes of workspace."""
+    from .attention_bwd import unit_heads
+    unit = unit_heads(nh // nkv, total_k, nh)
+    return unit, native.kernels().mb_attn_bwd_packed_workspace(total_q, total_k, nh, nkv, unit, d)
 
 
 def _offsets(cu, device):
@@ -39,11 +59,12 @@ class PackedSequences:
     on the stream that is current then."""
 
     def __init__(self, cu_seqlens, total: Optional[int] = None, cu_seqlens_k=None, total_k: Optional[int] = None, device=None):
-        if device is None:
-            device = cu_seqlens.device if isinstance(cu_seqlens, torch.Tensor) else "cpu"
-        device = torch.device(device)
-        if device.type == "cuda" and device.index is None:
-            device = torch.device("cuda", torch.cuda.current_device())
+        if device is None and isinstance(cu_seqlens, torch.Tensor):
+            device = cu_seqlens.device
+        else:
+            device = torch.device("cpu" if device is None else device)
+            if device.type == "cuda" and device.index is None:
+                device = torch.device("cuda", torch.cuda.current_device())
         self.same = cu_seqlens_k is None
         self.cu_q, self.host_q = _offsets(cu_seqlens, device)
         self.cu_k, self.host_k = (self.cu_q, self.host_q) if self.same else _offsets(cu_seqlens_k, device)
@@ -56,8 +77,7 @@ class PackedSequences:
         self._rotary = {}
         self._positions = self.plan = None
         if use_native(self.cu_q):
-            size = native.kernels().mb_packed_plan_bytes(self.n, self.total_q, self.total_k)
-            self.plan = torch.empty(size, dtype=torch.uint8, device=device)
+            self.plan = torch.empty(_plan_bytes(self.n, self.total_q, self.total_k), dtype=torch.uint8, device=device)
             if device.index == torch._C._cuda_getDevice():
                 self._make_plan()
             else:
@@ -146,20 +166,18 @@ def _launch_forward(tensors, strides, o, heads, packed, scale, causal):
     nh, nkv, d = heads
     total = packed.total_q
     lse = torch.empty(nh * total + 1, dtype=torch.float32, device=o.device)
-    claimed = ptr(lse) + 4 * nh * total if native.kernels().mb_attn_fwd_packed_counters(packed.n, total, nh) else 0
+    claimed = ptr(lse) + 4 * nh * total if _counters(packed.n, total, nh) else 0
     call("mb_attn_fwd_packed", *tensors, ptr(o), ptr(lse), ptr(packed.plan), claimed, packed.n, total, packed.total_k, nh, nkv,
          d, *strides, nh * d, d, scale, int(causal), stream())
     return lse
 
 
 def _launch_backward(dout, tensors, strides, o, lse, grads, grad_strides, heads, packed, scale, causal):
-    from .attention_bwd import unit_heads
     nh, nkv, d = heads
     dout = dout.contiguous()
     if ptr(dout) % 16:
         dout = dout.clone()
-    unit = unit_heads(nh // nkv, packed.total_k, nh)
-    size = native.kernels().mb_attn_bwd_packed_workspace(packed.total_q, packed.total_k, nh, nkv, unit, d)
+    unit, size = _backward_sizes(packed.total_q, packed.total_k, nh, nkv, d)
     workspace = torch.empty(size, dtype=torch.uint8, device=o.device)
     call("mb_attn_bwd_packed", ptr(dout), *tensors, ptr(o), ptr(lse), *grads, ptr(packed.plan), ptr(workspace), packed.n,
          packed.total_q, packed.total_k, nh, nkv, unit, d, *strides, *grad_strides, scale, int(causal), stream())
