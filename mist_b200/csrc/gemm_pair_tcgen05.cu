@@ -881,6 +881,7 @@ int xent_gemm(const void* x, const void* w, void* dlogits, int ldd, XentParams& 
   p.status = mb_status_device_ptr();
   p.splits = 1;
   max_ctas = clamp_ctas(max_ctas);
+  if (max_ctas < 2) max_ctas = 2;      // a pair
   return dlogits ? launch<false, false, kXentGrad>(ta, tb, tc, tx, p, max_ctas, stream)
                  : launch<false, false, kXentStats>(ta, tb, tc, tx, p, max_ctas, stream);
 }
@@ -981,8 +982,9 @@ MB_API int mb_xent_linear_bwd(const void* x, const void* w, const void* bias, co
   float* dx32 = reinterpret_cast<float*>(at + area.dlogits + area.col_sums);
   void* gemm_area = area.gemm ? at + area.dlogits + area.col_sums + area.dx32 : nullptr;
   auto gemm = [&](const void* a, const void* b, void* c, int m, int n, int k, int lda, int ldb, int ldc, int a_mn, int flags) {
-    const int rc = mb_gemm_pair_split_bf16(a, b, c, m, n, k, lda, ldb, ldc, a_mn, 1, flags, nullptr, nullptr, 1.f, max_ctas,
-                                           gemm_area, stream);
+    const int rc = max_ctas == 1 ? 1      // no pair
+                                 : mb_gemm_pair_split_bf16(a, b, c, m, n, k, lda, ldb, ldc, a_mn, 1, flags, nullptr, nullptr,
+                                                           1.f, max_ctas, gemm_area, stream);
     return rc != 1 ? rc : mb_gemm_bf16(a, b, c, m, n, k, lda, ldb, ldc, a_mn, 1, flags, nullptr, nullptr, 1.f, 0, max_ctas,
                                        stream);
   };

@@ -1159,7 +1159,7 @@ class _EmbeddingFn(torch.autograd.Function):
                 out = out + wpe[pos.clamp(0, wpe.shape[0] - 1)].float() * known[..., None].float()
             return out.to(wte.dtype)
         out = torch.empty(b, s, h, dtype=wte.dtype, device=wte.device)
-        call("mb_embed_fwd", ptr(ids), ptr(pos), ptr(wte), ptr(wpe), ptr(out), b * s, s, h, v0, wte.shape[0],
+        call("mb_embed_fwd", ptr(ids), ptr(pos), ptr(wte), ptr(wpe), ptr(out), b * s, max(s, 1), h, v0, wte.shape[0],
              0 if wpe is None else wpe.shape[0], scale, stream())
         return out
 
@@ -1197,7 +1197,7 @@ class _EmbeddingFn(torch.autograd.Function):
         if ptr(dout) % 16:
             dout = dout.clone()
         workspace = torch.empty(_embed_workspace(b * s, h, int(want_wpe and pos is not None)), dtype=torch.uint8, device=wte.device)
-        call("mb_embed_bwd", ptr(ids), ptr(pos), ptr(dout), ptr(dwte), ptr(dwpe), b * s, s, h, ctx.v0, wte.shape[0],
+        call("mb_embed_bwd", ptr(ids), ptr(pos), ptr(dout), ptr(dwte), ptr(dwpe), b * s, max(s, 1), h, ctx.v0, wte.shape[0],
              wpe.shape[0] if want_wpe else 0, ctx.scale, int(dwte is not None and dwte.dtype == torch.float32),
              int(direct and accumulate), ptr(workspace), stream())
         if bucket is None:

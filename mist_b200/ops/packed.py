@@ -119,9 +119,10 @@ class PackedSequences:
         """``(cos, sin, rot_dim)`` with a row for each packed token, that of its position."""
         key = (rot_dim, base)
         if key not in self._rotary:
-            from .functional import rope_tables
-            cos, sin = rope_tables(max(self.total_q, 1), rot_dim, base, self.device)
-            self._rotary[key] = (cos[self.positions].contiguous(), sin[self.positions].contiguous(), rot_dim)
+            # the angles of functional.rope_tables; what it keeps is by length, and packings come in every length
+            inv = 1.0 / (base ** (torch.arange(0, rot_dim, 2, dtype=torch.float32, device=self.device) / rot_dim))
+            angles = torch.outer(self.positions.float(), inv)
+            self._rotary[key] = (angles.cos(), angles.sin(), rot_dim)
         return self._rotary[key]
 
     def _each(self):

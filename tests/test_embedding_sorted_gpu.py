@@ -154,6 +154,29 @@ def test_other_integer_types_and_strides():
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("shape", [(0, 5), (3, 0)])
+@pytest.mark.parametrize("given", [False, True])
+def test_no_tokens(shape, given):
+    wte, wpe = (torch.randn(n, 16, device=DEV).bfloat16().requires_grad_(True) for n in (20, 9))
+    ids = torch.zeros(shape, device=DEV, dtype=torch.long)
+    out = F.embedding(ids, wte, wpe, position_ids=ids if given else None)
+    assert out.shape == (*shape, 16)
+    assert all(not g.any() for g in torch.autograd.grad(out.sum(), (wte, wpe)))
+
+
+@pytest.mark.parametrize("given", [False, True])
+def test_one_table_frozen(given):
+    torch.manual_seed(8)
+    ids, pos = torch.randint(0, 40, (2, 90), device=DEV), torch.randint(0, 90, (2, 90), device=DEV) if given else None
+    g = torch.randn(2, 90, 24, device=DEV).bfloat16()
+    tables = [torch.randn(n, 24, device=DEV).bfloat16() for n in (40, 90)]
+    both = [t.clone().requires_grad_(True) for t in tables]
+    want = torch.autograd.grad(F.embedding(ids, *both, position_ids=pos), both, g)
+    for k in range(2):
+        only = [t.clone().requires_grad_(i == k) for i, t in enumerate(tables)]
+        assert torch.equal(torch.autograd.grad(F.embedding(ids, *only, position_ids=pos), only[k], g)[0], want[k])
+
+
 @pytest.mark.parametrize("case", ["type", "width", "stride", "device"])
 def test_refusals(case):
     wte = torch.zeros(10, 16, device=DEV, dtype=torch.bfloat16)

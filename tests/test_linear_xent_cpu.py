@@ -128,3 +128,41 @@ def test_vocabulary_slices_on_two_ranks():
         assert torch.allclose(ret[r][2], dw[19 * r:19 * r + 19], atol=1e-5)
         assert torch.allclose(ret[r][3], db[19 * r:19 * r + 19], atol=1e-5)
     assert torch.allclose(ret[0][1] + ret[1][1], dx, atol=1e-5)
+
+
+def _head_worker(rank, port, tied, ret):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE="2")
+    dist.init_process_group("gloo", rank=rank, world_size=2)
+    try:
+        from mist_b200.models.language_model import LMHead
+        ret[rank] = _head_step(LMHead, dist.group.WORLD, rank, 2, tied)
+    finally:
+        dist.destroy_process_group()
+
+
+def _head_step(LMHead, group, rank, world, tied):
+    from mist_b200.config import ModelConfig
+    cfg = ModelConfig(name="gpt2-t", hidden_size=16, num_hidden_layers=1, num_attention_heads=2, max_position_embeddings=8,
+                      vocab_size=40, params_dtype="float32", add_encoder=True, add_decoder=False,
+                      encoder_attn_mask_type="causal", fused_lm_loss=True)
+    x, w, _, labels, _ = _case(rows=12, v=40, bias=False)
+    labels = labels.clamp(min=0)
+    head = LMHead(cfg, group)
+    part = w.detach().chunk(world)[rank].clone().requires_grad_(True)
+    if not tied:
+        with torch.no_grad():
+            head.proj.weight.copy_(part)
+        part = head.proj.weight
+    loss = head(x.view(2, 6, 16), labels.view(2, 6), part if tied else None)
+    return [t.detach() for t in (loss, *torch.autograd.grad(loss, (x, part)))]
+
+
+@pytest.mark.parametrize("tied", [False, True])
+def test_head_on_two_ranks(tied):
+    from mist_b200.models.language_model import LMHead
+    ret = mp.Manager().dict()
+    mp.spawn(_head_worker, args=(free_port(), tied, ret), nprocs=2)
+    loss, dx, dw = _head_step(LMHead, None, 0, 1, tied)
+    for r in range(2):
+        assert torch.allclose(ret[r][0], loss, atol=1e-5) and torch.allclose(ret[r][1], dx, atol=1e-5)
+        assert torch.allclose(ret[r][2], dw.chunk(2)[r], atol=1e-5)

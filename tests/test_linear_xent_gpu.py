@@ -155,6 +155,28 @@ def test_only_what_is_asked_for():
         assert torch.equal(torch.autograd.grad(loss, leaf, g)[0], both[k])
 
 
+def test_an_ignored_word_and_a_limit_on_the_ctas(monkeypatch):
+    """The ignored label may be a word of the vocabulary; few CTAs, down to one, give the same."""
+    x, w, b, labels, g = _case(300, 128, 600, True, ignored=0.0)
+    labels[::3] = 5
+    kept = labels.masked_fill(labels == 5, -100)
+    leaves = (x, w, b)
+
+    def once(labels, ignore):
+        loss = F.linear_cross_entropy(x, w, labels, b, ignore_index=ignore)
+        return [loss, *torch.autograd.grad(loss, leaves, g)]
+
+    want = once(kept, -100)
+    assert all(torch.equal(a, c) for a, c in zip(once(labels, 5), want))
+    for ctas in (1, 2, 7, 64):
+        monkeypatch.setattr(F.Settings, "gemm_max_ctas", ctas)
+        got = once(kept, -100)
+        assert torch.equal(got[0], want[0])
+        exact = _Exact(x, w, b, kept, g)
+        exact.check(got[0], got[1:])
+    native.check_status()
+
+
 def test_strided_inputs_and_one_gradient_value():
     x, w, b, labels, _ = _case(64, 128, 500, False)
     loss = F.linear_cross_entropy(x, w, labels)
