@@ -170,11 +170,15 @@ class TrainingSession:
         ``micro_batch * G`` samples along dimension 0; used for the encoder-only and
         encoder-decoder families whose forward takes more than ids and labels."""
         self._beat()
+        # (a list or tuple holds one value per micro batch: the packings of batches of packed sequences)
+        listed = {k for k, v in batch.items() if isinstance(v, (list, tuple))}
+        for k in listed:
+            if len(batch[k]) != self.G:
+                raise ValueError(f"{k}: {len(batch[k])} values for {self.G} micro batches")
         if self.G == 1:
-            batches = [dict(batch)]
+            batches = [{k: v[0] if k in listed else v for k, v in batch.items()}]
         else:
-            # (a list or tuple holds one value per micro batch: the packings of batches of packed sequences)
-            parts = {k: v if isinstance(v, (list, tuple)) else v.chunk(self.G) for k, v in batch.items()}
+            parts = {k: v if k in listed else v.chunk(self.G) for k, v in batch.items()}
             batches = [{k: parts[k][i] for k in batch} for i in range(self.G)]
         if self.pipeline is not None:
             return self.pipeline.train_step(batches)

@@ -693,11 +693,13 @@ template <bool A_MN, bool B_MN, int KIND>
 int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const CUtensorMap& tx,
            const typename ParamsOf<KIND>::type& p, int max_ctas, cudaStream_t stream) {
   constexpr int smem = Layout<staged_tiles(KIND) == 4>::kTotal + 1024;
-  static bool configured = false;
+  static bool configured[64] = {};      // of each device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
   auto kern = gemm_pair_kernel<A_MN, B_MN, KIND>;
-  if (!configured) {
+  if (!configured[dev]) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -3;
-    configured = true;
+    configured[dev] = true;
   }
   int tiles = ((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + BN - 1) / BN);
   int pairs = max_ctas / 2;

@@ -471,12 +471,14 @@ int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, 
            const GemmParams& p, int max_ctas, cudaStream_t stream) {
   using L = SmemLayout<BN, STAGES>;
   constexpr int smem = L::kTotal + 1024;
-  static bool configured = false;
+  static bool configured[64] = {};      // of each device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
   auto kern = gemm_bf16_kernel<BN, STAGES, A_MN, B_MN>;
-  if (!configured) {
+  if (!configured[dev]) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return -3;
-    configured = true;
+    configured[dev] = true;
   }
   int num_tiles = ((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
   int grid = num_tiles < max_ctas ? num_tiles : max_ctas;

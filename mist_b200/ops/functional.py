@@ -870,7 +870,8 @@ def attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k=None, scale: Optional[f
     :class:`PackedSequences` in the place of ``cu_seqlens_q``.  One launch covers all sequences, in the forward pass and
     in the backward pass; offsets on the device are not read back.  A causal query sees the keys up to its own place, the
     sequences aligned at their ends.  Queries without a key, and rows behind the last sequence, give zeros.
-    Returns ``[total_q, nh, d]``, or where the offsets are known on the host as many rows as they say (the interface of the
+    Returns ``[total_q, nh, d]``, or where the offsets are known on the host as many rows as they say (all, of zeros, where they say
+    none) (the interface of the
     reference's ``flash_attn_varlen`` entry points, csrc/flash_attn/flash_api.cpp ``varlen_fwd`` / ``varlen_bwd``)."""
     if _elsewhere(q):
         with torch.cuda.device(q.device):
@@ -881,7 +882,8 @@ def attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k=None, scale: Optional[f
         return packed_attention.attention(q, k, v, cu_seqlens_q, scale, causal)
     seqs = PackedSequences(cu_seqlens_q, q.shape[0], cu_seqlens_k, k.shape[0], device=q.device)
     out = packed_attention.attention(q, k, v, seqs, scale, causal)
-    return out if seqs.host_q is None or seqs.host_q[-1] == q.shape[0] else out[:seqs.host_q[-1]]
+    rows = seqs.host_q[-1] if seqs.host_q is not None else 0
+    return out if rows in (0, q.shape[0]) else out[:rows]
 
 
 class _PackedAttnFn(torch.autograd.Function):

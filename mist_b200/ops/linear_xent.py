@@ -67,7 +67,8 @@ class _LinearXentFn(torch.autograd.Function):
             inside = (at >= 0) & (at < vocab)
             top = logits.max(-1).values
             target = torch.where(inside, logits.gather(1, at.clamp(0, vocab - 1)[:, None])[:, 0], torch.zeros_like(top))
-            total = torch.exp(logits - top[:, None]).sum(-1)
+            # (a slice that is all -inf adds nothing: the others may have more)
+            total = torch.exp(logits - top.masked_fill(top == float("-inf"), 0.0)[:, None]).sum(-1)
             if split:
                 loss, lse = _combine_over_group(torch.stack([top, total, target], 1), labels, ignore_index, group)
             else:
@@ -98,6 +99,8 @@ class _LinearXentFn(torch.autograd.Function):
         bucket = getattr(ctx.param, "grad_bucket", None) if want_w else None
         accumulate = bucket is not None and bool(getattr(ctx.param, "grad_accumulate", False))
         direct = bucket is not None and bucket.dtype in (torch.float32, weight.dtype) and bucket.stride(1) == 1
+        if direct and use_native(x2):      # what the products' stores can address
+            direct = bucket.stride(0) % 8 == 0 and bucket.stride(0) >= k and ptr(bucket) % 16 == 0
         dw = None
         if direct:
             dw = bucket
@@ -149,7 +152,7 @@ def _reference_backward(x2, weight, bias, labels, lse, gloss, v0, ignore, dx, dw
 def linear_cross_entropy(x, weight, labels, bias=None, vocab_start: int = 0, group=None, ignore_index: int = -100):
     """Loss (fp32) of every row of ``x`` ``[..., hidden]`` against ``labels`` ``[...]``: the cross entropy of the logits
     ``x @ weight.T + bias``, which are computed in fp32 and not kept.  Rows labelled ``ignore_index`` have loss 0 and
-    give no gradient.
+    give no gradient.  A label outside the vocabulary counts as one whose logit is 0; no one checks for it.
 
     ``weight`` ``[vocab, hidden]`` (and ``bias`` ``[vocab]``) may be this rank's slice of the vocabulary, starting at
     ``vocab_start``; ``group`` is then the group of the slices, and ``x`` is the same on every rank of it (its gradient is

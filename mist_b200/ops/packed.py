@@ -116,14 +116,19 @@ class PackedSequences:
             raise ValueError(f"tensors on {q.device}, offsets on {self.device}")
 
     def rotary(self, rot_dim: int, base: float):
-        """``(cos, sin, rot_dim)`` with a row for each packed token, that of its position."""
+        """``(cos, sin, rot_dim)`` with a row for each packed token, that of its position; made on the stream of the first call
+        and kept, or made for the graph alone while one is captured."""
         key = (rot_dim, base)
-        if key not in self._rotary:
+        tables = self._rotary.get(key)
+        if tables is None:
             # the angles of functional.rope_tables; what it keeps is by length, and packings come in every length
             inv = 1.0 / (base ** (torch.arange(0, rot_dim, 2, dtype=torch.float32, device=self.device) / rot_dim))
             angles = torch.outer(self.positions.float(), inv)
-            self._rotary[key] = (angles.cos(), angles.sin(), rot_dim)
-        return self._rotary[key]
+            tables = (angles.cos(), angles.sin(), rot_dim)
+            # (tables that a graph being captured computes belong to it: outside it nobody has computed them)
+            if self.plan is None or not torch.cuda.is_current_stream_capturing():
+                self._rotary[key] = tables
+        return tables
 
     def _each(self):
         """``(queries, keys)`` slices of every sequence (reference path: reads the offsets)."""

@@ -166,3 +166,36 @@ def test_head_on_two_ranks(tied):
     for r in range(2):
         assert torch.allclose(ret[r][0], loss, atol=1e-5) and torch.allclose(ret[r][1], dx, atol=1e-5)
         assert torch.allclose(ret[r][2], dw.chunk(2)[r], atol=1e-5)
+
+
+def _masked_slice_worker(rank, port, ret):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE="2")
+    dist.init_process_group("gloo", rank=rank, world_size=2)
+    try:
+        x, w, b, labels, g = _masked_case()
+        half = w.detach()[rank * 19:(rank + 1) * 19].clone().requires_grad_(True)
+        hb = b.detach()[rank * 19:(rank + 1) * 19].clone()
+        loss = F.linear_cross_entropy(x, half, labels, hb, vocab_start=19 * rank, group=dist.group.WORLD)
+        ret[rank] = [t.detach() for t in (loss, *torch.autograd.grad(loss, (x, half), g))]
+    finally:
+        dist.destroy_process_group()
+
+
+def _masked_case():
+    """All of the second rank's words (the padding of a vocabulary) have the logit -inf."""
+    x, w, b, labels, g = _case(v=38)
+    with torch.no_grad():
+        b[19:] = float("-inf")
+    return x, w, b, torch.where(labels >= 0, labels % 19, labels), g
+
+
+def test_a_slice_of_words_that_are_masked():
+    ret = mp.Manager().dict()
+    mp.spawn(_masked_slice_worker, args=(free_port(), ret), nprocs=2)
+    x, w, b, labels, g = _masked_case()
+    want = _plain(x, w, b, labels)
+    dx, dw = torch.autograd.grad(want, (x, w), g)
+    for r in range(2):
+        assert torch.allclose(ret[r][0], want, atol=1e-5)
+        assert torch.allclose(ret[r][2], dw[19 * r:19 * r + 19], atol=1e-5)
+    assert torch.allclose(ret[0][1] + ret[1][1], dx, atol=1e-5)

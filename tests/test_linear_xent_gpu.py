@@ -250,3 +250,21 @@ def test_refusals(case):
         labels = labels.cpu()
     with pytest.raises(ValueError):
         F.linear_cross_entropy(x, w, labels)
+
+
+@pytest.mark.parametrize("dtype,start", [(torch.float32, 1), (torch.bfloat16, 4)])
+def test_bucket_off_the_stores_alignment(dtype, start):
+    """A bucket that the kernels' stores cannot address gets the gradient by way of another tensor."""
+    torch.manual_seed(9)
+    x = torch.randn(40, 64, device=DEV).bfloat16()
+    w = torch.nn.Parameter(torch.randn(96, 64, device=DEV).bfloat16())
+    labels = torch.randint(0, 96, (40,), device=DEV)
+    want, = torch.autograd.grad(F.linear_cross_entropy(x, w, labels).sum(), w)
+    flat = torch.zeros(96 * 64 + 8, device=DEV, dtype=dtype)
+    w.grad_bucket = flat[start:start + 96 * 64].view(96, 64)
+    for n in (1, 2):
+        F.linear_cross_entropy(x, w, labels).sum().backward()
+        # an fp32 bucket holds what the bf16 gradient was before its rounding; a second step adds one rounding
+        tol = 2 ** -8 * n * want.float().abs() * (1 + n) + 1e-6
+        assert ((w.grad_bucket.float() - n * want.float()).abs() <= tol).all()
+    assert not flat[:start].any() and not flat[start + 96 * 64:].any()

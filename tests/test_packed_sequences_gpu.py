@@ -313,3 +313,26 @@ def test_refusals(case):
         cu = F.PackedSequences(cu, 11)
     with pytest.raises(ValueError):
         F.attention_varlen(x, x, x, cu)
+
+
+def test_rotary_tables_of_a_captured_graph_stay_in_it():
+    """Tables that a graph computes are not there for anyone before it is replayed."""
+    seqs = F.PackedSequences([0, 30, 70], device=DEV)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        F.PackedSequences([0, 30, 70], device=DEV).rotary(32, 10000.0)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inside = seqs.rotary(32, 10000.0)
+    at = torch.cat([torch.arange(30), torch.arange(40)]).double()
+    angles = torch.outer(at, 10000.0 ** (-torch.arange(0, 32, 2).double() / 32))
+    outside = seqs.rotary(32, 10000.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    for cos, sin, rot in (outside, inside):
+        assert rot == 32
+        # angles up to 40 in fp32: half a step is 2^-19, three roundings of it on the way
+        assert (cos.double().cpu() - angles.cos()).abs().max() < 2 ** -17
+        assert (sin.double().cpu() - angles.sin()).abs().max() < 2 ** -17

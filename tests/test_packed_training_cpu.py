@@ -108,3 +108,28 @@ def test_refusals():
         ParallelMHA(32, 4, causal=True, rotary_emb_dim=8, rotary_emb_interleaved=True)(x, attention_mask=seqs)
     with pytest.raises(ValueError):
         ParallelMHA(32, 4, causal=True)(x, attention_mask=F.PackedSequences([0, 7]))
+
+
+@pytest.mark.parametrize("micro", [1, 2])
+def test_a_session_takes_one_packing_per_micro_batch(micro):
+    from mist_b200.api import TrainingSession
+    from mist_b200.config import load_config
+    vec = "[1,1,1,0,0,0,0,0,0,0]"
+    cfg, _ = load_config("config", [
+        "experiment=gpt2-1.3b", "model=gpt2/1.3b", "model.params_dtype=float32", "training.params_dtype=float32",
+        "hardware.num_gpus_per_node=1", "model.hidden_size=32", "model.intermediate_size=64", "model.num_attention_heads=4",
+        "model.num_heads_kv=4", "model.num_hidden_layers=1", "model.vocab_size=256", "training.vocab_size=256",
+        "training.max_sequence_length=24", f"training.global_batch_size={micro}", "strategy.layer_partitions=[1]",
+        "strategy.device_assignment=[[1,1]]", "strategy.gradient_checkpointing=[0]",
+        f"strategy.gradient_accumulation_steps={micro}", f"strategy.stage_strategies=[{vec}]",
+        f"strategy.pre_post_strategy_array={vec}"], check_world_size=False)
+    sess = TrainingSession(cfg, seed=3, device=torch.device("cpu"), hp=dict(lr=1e-3))
+    ids = torch.randint(0, 256, (micro, 24), generator=torch.Generator().manual_seed(2))
+    packings = [F.PackedSequences(cu, 24) for cu in ([0, 5, 24], [0, 24])]
+    with torch.no_grad():
+        want = sum(sess.model(ids[i:i + 1], attention_mask=packings[i], labels=ids[i:i + 1]) for i in range(micro)) / micro
+    with pytest.raises(ValueError, match="micro batches"):
+        sess.step_on_device_batch(dict(input_ids=ids, labels=ids, attention_mask=packings * 2))
+    got = sess.step_on_device_batch(dict(input_ids=ids, labels=ids, attention_mask=packings[:micro]))
+    sess.finish()
+    assert abs(float(got) - float(want)) < 1e-5
