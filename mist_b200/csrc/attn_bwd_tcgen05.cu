@@ -462,31 +462,38 @@ attn_delta_kernel(const __nv_bfloat16* __restrict__ dout, const __nv_bfloat16* _
 
 // The same of packed sequences, [total][nh][d] -> delta [nh][total], and what their backward pass also needs: the count of
 // claimed work items set to 0, the fp32 dQ [nh][total][d] of tiles that more than one block of keys sees (rows whose `single`
-// lacks the bit) set to 0, and dQ itself where no key is visible.  A lane has 8 values; a warp takes as many rows as fit it and
-// does so four times at once (16 lanes per row, of which 10 worked, took 45 us for 8192 x 32 heads of 80).
-__global__ void __launch_bounds__(256)
+// lacks the bit) set to 0, and dQ itself where no key is visible.  A lane has 8 values; a warp takes consecutive tokens of one
+// head, as many as fit it and that twice, so that what it reads and writes per row has its neighbours beside it.  Bound by memory:
+// 16384 x 32 heads of 128, dQ of nearly all rows set to 0, 80 us at 6.6 TB/s (98 with consecutive heads per warp).
+constexpr int kPackedRows = 2;
+__global__ void __launch_bounds__(256, 6)
 attn_delta_packed_kernel(const __nv_bfloat16* __restrict__ dout, const __nv_bfloat16* __restrict__ o,
-                         float* __restrict__ delta, int total, int nh, int d, const float* __restrict__ lse, int* claimed,
-                         float* __restrict__ dq_acc, const uint8_t* __restrict__ single, int single_bit,
+                         float* __restrict__ delta, unsigned total, unsigned nh, unsigned d, const float* __restrict__ lse,
+                         int* claimed, float* __restrict__ dq_acc, const uint8_t* __restrict__ single, int single_bit,
                          __nv_bfloat16* __restrict__ dq, long dq_ts, long dq_hs) {
   if (blockIdx.x == 0 && threadIdx.x == 0) *claimed = 0;
-  const int vpr = d >> 3, lane = threadIdx.x & 31, per_warp = 32 / vpr, sub = lane % vpr, mine = lane / vpr;
-  const long rows = static_cast<long>(total) * nh;
-  const long first = (blockIdx.x * 8l + (threadIdx.x >> 5)) * per_warp * kDeltaRows + mine;
+  const unsigned vpr = d >> 3, lane = threadIdx.x & 31, per_warp = 32 / vpr, mine = lane / vpr, sub = lane - mine * vpr;
+  const unsigned w = blockIdx.x * 8 + (threadIdx.x >> 5), tile = w / nh, h = w - tile * nh;
+  const unsigned t0 = tile * per_warp * kPackedRows + mine;
   const bool works = mine < per_warp;
-  mb::bf16x8 x[kDeltaRows], y[kDeltaRows];
+  mb::bf16x8 x[kPackedRows], y[kPackedRows];
+  float l[kPackedRows];
+  bool many[kPackedRows];
 #pragma unroll
-  for (int u = 0; u < kDeltaRows; ++u) {
-    const long row = first + u * per_warp;
-    if (works && row < rows) {
-      x[u] = reinterpret_cast<const mb::bf16x8*>(dout)[row * vpr + sub];
-      y[u] = reinterpret_cast<const mb::bf16x8*>(o)[row * vpr + sub];
+  for (int u = 0; u < kPackedRows; ++u) {
+    const unsigned t = t0 + u * per_warp;
+    if (works && t < total) {
+      const size_t at = (static_cast<size_t>(t) * nh + h) * vpr + sub;
+      x[u] = reinterpret_cast<const mb::bf16x8*>(dout)[at];
+      y[u] = reinterpret_cast<const mb::bf16x8*>(o)[at];
+      l[u] = lse[static_cast<size_t>(h) * total + t];
+      many[u] = !(single[t] & single_bit);
     }
   }
 #pragma unroll
-  for (int u = 0; u < kDeltaRows; ++u) {
-    const long row = first + u * per_warp;
-    const bool live = works && row < rows;
+  for (int u = 0; u < kPackedRows; ++u) {
+    const unsigned t = t0 + u * per_warp;
+    const bool live = works && t < total;
     float acc = 0.f;
     if (live) {
       float f[8], g[8];
@@ -501,22 +508,32 @@ attn_delta_packed_kernel(const __nv_bfloat16* __restrict__ dout, const __nv_bflo
       if (sub + m < vpr) acc += other;
     }
     if (!live) continue;
-    const int t = static_cast<int>(row / nh), h = static_cast<int>(row - static_cast<long>(t) * nh);
-    const long at = static_cast<long>(h) * total + t;
+    const size_t at = static_cast<size_t>(h) * total + t;
     if (sub == 0) delta[at] = acc;
-    if (!(single[t] & single_bit)) {
+    if (many[u]) {
       float4* dst = reinterpret_cast<float4*>(dq_acc + at * d + sub * 8);
       dst[0] = dst[1] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    if (lse[at] == -INFINITY) *reinterpret_cast<uint4*>(dq + t * dq_ts + h * dq_hs + sub * 8) = make_uint4(0, 0, 0, 0);
+    if (l[u] == -INFINITY) *reinterpret_cast<uint4*>(dq + t * dq_ts + h * dq_hs + sub * 8) = make_uint4(0, 0, 0, 0);
   }
 }
 
-// dq[b][q][h][:] = bf16(scale * dq_acc[b][h][q][:]); PACKED: but for the rows whose `single` has the bit
-template <bool PACKED>
+// dq[t][h][:] = bf16(scale * acc[h][t][:]) but for the rows whose `single` has the bit; blockIdx.y: head.
+__global__ void __launch_bounds__(256)
+attn_convert_dq_packed_kernel(const float* __restrict__ acc, __nv_bfloat16* __restrict__ dq, unsigned total, unsigned d, long dq_ts,
+                              long dq_hs, float scale, const uint8_t* __restrict__ single, int single_bit) {
+  const unsigned vpr = d >> 3, i = blockIdx.x * 256 + threadIdx.x;
+  const unsigned t = i / vpr, v = i - t * vpr, h = blockIdx.y;
+  if (t >= total || (single[t] & single_bit)) return;
+  const float4* src = reinterpret_cast<const float4*>(acc + (static_cast<size_t>(h) * total + t) * d + 8 * v);
+  const float4 x = src[0], y = src[1];
+  const float f[8] = {x.x * scale, x.y * scale, x.z * scale, x.w * scale, y.x * scale, y.y * scale, y.z * scale, y.w * scale};
+  *reinterpret_cast<mb::bf16x8*>(dq + t * dq_ts + h * dq_hs + 8 * v) = mb::pack8(f);
+}
+
+// dq[b][q][h][:] = bf16(scale * dq_acc[b][h][q][:])
 __global__ void attn_convert_dq_kernel(const float* __restrict__ acc, __nv_bfloat16* __restrict__ dq, int batch,
-                                       int sq, int nh, int d, long dq_bs, long dq_ts, long dq_hs, float scale,
-                                       const uint8_t* single, int single_bit) {
+                                       int sq, int nh, int d, long dq_bs, long dq_ts, long dq_hs, float scale) {
   const int vpr = d >> 3;
   const long nvec = static_cast<long>(batch) * nh * sq * vpr;
   for (long i = static_cast<long>(blockIdx.x) * blockDim.x + threadIdx.x; i < nvec;
@@ -524,7 +541,6 @@ __global__ void attn_convert_dq_kernel(const float* __restrict__ acc, __nv_bfloa
     const int v = static_cast<int>(i % vpr);
     long t = i / vpr;
     const int q = static_cast<int>(t % sq);
-    if (PACKED && (single[q] & single_bit)) continue;
     t /= sq;
     const int h = static_cast<int>(t % nh);
     const int b = static_cast<int>(t / nh);
@@ -718,8 +734,8 @@ MB_API int mb_attn_bwd(const void* dout, const void* q, const void* k, const voi
     long nvec = static_cast<long>(batch) * nh * sq * (d / 8);
     long blocks = (nvec + 255) / 256;
     if (blocks > 148 * 16) blocks = 148 * 16;
-    attn_convert_dq_kernel<false><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
-        dq_acc, reinterpret_cast<__nv_bfloat16*>(dq), batch, sq, nh, d, dq_bs, dq_ts, dq_hs, pipelined ? scale : 1.f, nullptr, 0);
+    attn_convert_dq_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
+        dq_acc, reinterpret_cast<__nv_bfloat16*>(dq), batch, sq, nh, d, dq_bs, dq_ts, dq_hs, pipelined ? scale : 1.f);
   }
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
@@ -771,15 +787,15 @@ MB_API int mb_attn_bwd_packed(const void* dout, const void* q, const void* k, co
     return -1;
   const long rows = static_cast<long>(total_q) * nh, units = nh / unit_heads;
   const long most = packed_backward_items(total_k, n) * units;
-  if (rows > 0x7fffffff || most > 0x3fffffff) return -1;
+  if (rows > 0x7fffffff || most > 0x3fffffff || nh > 65535 || static_cast<long>(total_q) * (d / 8) > 0x7fffffff) return -1;
   const PackedArea area = packed_area(total_q, total_k, nh, nh_kv, unit_heads, d);
   uint8_t* at = static_cast<uint8_t*>(workspace);
   float* delta = reinterpret_cast<float*>(at + area.delta);
   float* dq_acc = reinterpret_cast<float*>(at + area.dq_acc);
   int* claimed = reinterpret_cast<int*>(at + area.claimed);
   if (total_q > 0) {
-    const long per_block = 8l * (32 / (d / 8)) * kDeltaRows;
-    attn_delta_packed_kernel<<<static_cast<unsigned>((rows + per_block - 1) / per_block), 256, 0, stream>>>(
+    const long tokens = (32 / (d / 8)) * kPackedRows, warps = (total_q + tokens - 1) / tokens * nh;
+    attn_delta_packed_kernel<<<static_cast<unsigned>((warps + 7) / 8), 256, 0, stream>>>(
         reinterpret_cast<const __nv_bfloat16*>(dout), reinterpret_cast<const __nv_bfloat16*>(o), delta, total_q, nh, d, lse,
         claimed, dq_acc, static_cast<const uint8_t*>(plan) + packed_single_offset(total_q, total_k, n), causal ? 2 : 1,
         reinterpret_cast<__nv_bfloat16*>(dq), dq_ts, dq_hs);
@@ -843,11 +859,10 @@ MB_API int mb_attn_bwd_packed(const void* dout, const void* q, const void* k, co
   sch.group = static_cast<int>(group < 1 ? 1 : (group < units ? group : units));
   kern<<<most < 148 ? static_cast<int>(most) : 148, wide::kThreads, wide::kSmem, stream>>>(tq, tk, tv, tdo, tdq, p, sch);
   if (queries) {
-    long blocks = (rows * (d / 8) + 255) / 256;
-    if (blocks > 148 * 16) blocks = 148 * 16;
-    attn_convert_dq_kernel<true><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
-        dq_acc, p.dq, 1, total_q, nh, d, 0, dq_ts, dq_hs, scale,
-        static_cast<const uint8_t*>(plan) + packed_single_offset(total_q, total_k, n), causal ? 2 : 1);
+    attn_convert_dq_packed_kernel<<<dim3(static_cast<unsigned>((static_cast<long>(total_q) * (d / 8) + 255) / 256), nh), 256, 0,
+                                    stream>>>(dq_acc, p.dq, total_q, d, dq_ts, dq_hs, scale,
+                                              static_cast<const uint8_t*>(plan) + packed_single_offset(total_q, total_k, n),
+                                              causal ? 2 : 1);
   }
   if (cudaGetLastError() != cudaSuccess) return -4;
   return parts > 1 ? mb_attn_sum_parts(part_k, part_v, dk, dv, 1, total_k, nh_kv, parts, d, 0, dk_ts, dk_hs, 0, dv_ts, dv_hs,
