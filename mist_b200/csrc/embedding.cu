@@ -7,6 +7,8 @@
 // tokens of a row keep their order), then every row of the table is summed in fp32 by the threads that write it: each
 // row of dout is read once, each row of the table is written once in its own type, and the sums have one order, so
 // results repeat bit for bit.  The traffic that stays is that of the definition; it is bound by memory.
+// Measured: 16384 tokens of 2560, tables of 50304 and 2048 rows: lookup 40 us, sort 16, sums 67 (390 MB, 5.8 TB/s); 8192
+// tokens of 4096, 32000 rows: 25, 11, 51.  (A scatter with atomics into fp32 tables and a cast of those took 1300 us.)
 //
 // Reference counterpart: the embedding modules of mist/modules/embedding.py:207-281 (gradient by torch's scatter-add).
 #include "common.cuh"
@@ -18,7 +20,8 @@ namespace cg = cooperative_groups;
 namespace {
 
 // ------------------------------------------------------------------------------------------------ lookup
-// One warp per token and slice of its row, `per_warp` vectors of 8 values, four rounds of loads in flight per lane.
+// One warp per token and slice of its row, `per_warp` vectors of 8 values, four rounds of loads in flight per lane (and
+// registers for four CTAs per SM: 16384 x 2560 with positions 76 -> 40 us).
 __global__ void __launch_bounds__(256, 4)
 embed_fwd_kernel(const int64_t* __restrict__ ids, const int64_t* __restrict__ pos, const __nv_bfloat16* __restrict__ wte,
                  const __nv_bfloat16* __restrict__ wpe, __nv_bfloat16* __restrict__ out, int tokens, int seq, int h, int64_t v0,
@@ -90,7 +93,8 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortCluster = 8;
 
 // The sorts take 8 bits of the key a pass.  A warp owns a stretch of consecutive tokens; ballots over the bits rank equal
-// digits inside 32 of them (__match_any_sync takes 270 cycles of a scheduler), a histogram per warp counts those before.  Latency is all that they cost.
+// digits inside 32 of them (__match_any_sync takes 270 cycles of a scheduler), a histogram per warp counts those before.
+// Latency is all that they cost: 8 us a pass of 16384 tokens, most of it the exchange between the CTAs and the scatter.
 struct SortSpace {
   int hist[32][256];
   int totals[256], base[256], warp_part[8], quarter[4][256];
