@@ -1133,7 +1133,9 @@ def _flat_positions(position_ids, ids):
         return None
     if position_ids.is_floating_point() or position_ids.device != ids.device:
         raise ValueError("position_ids: integers on the device of the ids expected")
-    return position_ids.expand(ids.shape).long().contiguous()
+    if position_ids.shape != ids.shape:
+        position_ids = position_ids.expand(ids.shape)
+    return position_ids.long().contiguous()
 
 
 @functools.lru_cache(maxsize=1024)

@@ -19,7 +19,8 @@ from .native import call, ptr, stream, use_native
 
 def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
     """``t`` as ``[rows, cols]`` that the kernels' copies can address: unit stride, rows on 16 bytes."""
-    t = t.reshape(-1, cols)
+    if t.dim() != 2:
+        t = t.reshape(-1, cols)
     if t.stride(1) != 1 or t.stride(0) % 8 or t.stride(0) < cols or ptr(t) % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
@@ -128,7 +129,9 @@ class _LinearXentFn(torch.autograd.Function):
             if not direct:
                 bucket.add_(dw) if accumulate else bucket.copy_(dw)      # any type and order
             ctx.param.grad_accumulate = True
-        return (None if dx is None else dx.reshape(ctx.x_shape), dw if bucket is None else None, db, None, None, None, None)
+        if dx is not None and dx.shape != ctx.x_shape:
+            dx = dx.reshape(ctx.x_shape)
+        return (dx, dw if bucket is None else None, db, None, None, None, None)
 
 
 def _reference_backward(x2, weight, bias, labels, lse, gloss, v0, ignore, dx, dw, accumulate, db):
@@ -174,5 +177,6 @@ def linear_cross_entropy(x, weight, labels, bias=None, vocab_start: int = 0, gro
             raise ValueError("the kernels take bf16 of a hidden size that is a multiple of 8")
         if bias is not None and not bias.is_contiguous():
             bias = bias.contiguous()
-    labels = labels.reshape(-1).long().contiguous()
-    return _LinearXentFn.apply(x, weight, bias, labels, int(vocab_start), group, int(ignore_index)).reshape(x.shape[:-1])
+    flat = labels if labels.dim() == 1 else labels.reshape(-1)
+    loss = _LinearXentFn.apply(x, weight, bias, flat.long().contiguous(), int(vocab_start), group, int(ignore_index))
+    return loss if labels.dim() == 1 else loss.reshape(labels.shape)
