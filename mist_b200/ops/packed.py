@@ -299,12 +299,18 @@ def projected_attention(qkv, kv_heads: int, packed: PackedSequences, scale: floa
     cos, sin, rot = rotary if rotary is not None else (None, None, 0)
     if qkv.dim() == 5:
         qkv = qkv.flatten(2, 3)
-    if qkv.dim() != 4 or qkv.shape[2] <= 2 * kv_heads or (qkv.shape[2] - 2 * kv_heads) % kv_heads or not packed.same:
+    if qkv.dim() != 4 or kv_heads < 1 or qkv.shape[2] <= 2 * kv_heads or (qkv.shape[2] - 2 * kv_heads) % kv_heads or not packed.same:
         raise ValueError(f"{tuple(qkv.shape)} with {kv_heads} key heads: self attention over one packing expected")
     if qkv.shape[0] * qkv.shape[1] != packed.total_q or packed.total_k != packed.total_q:
         raise ValueError(f"{tuple(qkv.shape[:2])} tokens, but the packing is of {packed.total_q}")
     if qkv.device != packed.device:
         raise ValueError(f"tensors on {qkv.device}, offsets on {packed.device}")
+    if rot:
+        for t in (cos, sin):
+            if t.shape != (packed.total_q, rot // 2) or t.dtype != torch.float32 or not t.is_contiguous() or t.device != qkv.device:
+                raise ValueError(f"rotary tables: fp32 {(packed.total_q, rot // 2)} on {qkv.device} expected, a row for every token")
+        if rot % 2 or rot > qkv.shape[3]:
+            raise ValueError(f"{rot} rotated values of heads of {qkv.shape[3]}")
     if use_native(qkv):
         check_kernel_types(qkv)
         if not qkv.is_contiguous() or ptr(qkv) % 16:

@@ -84,3 +84,24 @@ def test_tensors_that_do_not_fit():
         F.attention_projected(q[None], 1, 0.25, True, seqlens=torch.tensor([18]), packed=seqs)
     with pytest.raises(ValueError):
         F.attention_projected(q[None], 2, 0.25, True, packed=seqs)
+
+
+@pytest.mark.parametrize("case", ["rows", "width", "type", "strided", "more than a head"])
+def test_rotary_tables_that_do_not_fit_are_refused(case):
+    """Each token has a row; a table of positions, as the batched form takes it, is too short."""
+    seqs = F.PackedSequences([0, 5, 12])
+    qkv = torch.randn(1, 12, 3, 2, 16)
+    cos, sin, rot = seqs.rotary(16, 10000.0)
+    F.attention_projected(qkv, 2, 0.25, True, (cos, sin, rot), packed=seqs)
+    if case == "rows":
+        cos, sin = cos[:7].contiguous(), sin[:7].contiguous()
+    elif case == "width":
+        rot = 8
+    elif case == "type":
+        cos = cos.double()
+    elif case == "strided":
+        sin = torch.cat([sin, sin], 1)[:, ::2]
+    else:
+        cos, sin, rot = seqs.rotary(32, 10000.0)
+    with pytest.raises(ValueError):
+        F.attention_projected(qkv, 2, 0.25, True, (cos, sin, rot), packed=seqs)
