@@ -70,26 +70,47 @@ __device__ __forceinline__ void report(int* status, int code) {
 
 // What a kernel's epilogue does beside the common part.  The split form is a kernel of its own: its second source of the
 // products cost the others 4 - 9 % where the epilogue is the bound (13760 x 6664 x 128: 81.7 us against 87.4).
-enum Kind : int { kPlain = 0, kAux = 1, kSplit = 2, kXentStats = 3, kXentGrad = 4 };
+enum Kind : int { kPlain = 0, kAux = 1, kSplit = 2, kXentStats = 3, kXentGrad = 4, kXentKeep = 5 };
 
 // Vocabulary projection with cross entropy: C, the logits, is never stored.  The statistics' epilogue hides behind the
 // products (4096 x 2048, vocabulary 50304 with bias: 496 us, 1.70 PFLOP/s, tensor pipe 97 % busy), the gradient's almost (25344
-// columns of the same: 259 us, 1.64 PFLOP/s, 88 %).  Of both passes, 8 T H V operations, 6.6 ms at 8192 x 2560 x 50304 are
-// bound by the power cap (1.28 PFLOP/s).  Keeping the logits instead of computing them again would save a quarter of the
-// operations and cost T V 16-bit numbers, 824 MB there.  A struct of its own, because a parameter
+// columns of the same: 259 us, 1.64 PFLOP/s, 88 %).  Long runs of
+// both passes are bound by the power cap: 8192 x 2560 x 50304 6.4 ms for 8 T H V operations, 5.1 where kXentKeep spares the
+// backward pass the logits (its own 1440 us against 1290: 824 MB more to write, one stage less).  A struct of its own, because a parameter
 // more changes the code of the other kinds (registers of the split one 238 -> 164).
 struct XentParams : PairParams {
   const int64_t* labels;      // [M]; the label's column is labels[m] - v0
   int64_t v0, ignore;
   int segments;               // parts of K whose sums are added in registers
-  float2* stats;              // kXentStats: [column tile][M] {maximum * log2(e), sum of 2^(x * log2(e) - that)}
-  float* target;              // kXentStats: [M], written where the label's column is among these
+  float2* stats;              // kXentStats: [column tile][M] {maximum * log2(e), sum of 2^(x * log2(e) - that)}; kXentKeep: of
+                              // every 128 columns
+  float* target;              // kXentStats, kXentKeep: [M], written where the label's column is among these
   const float *lse, *gloss;   // kXentGrad: [M]
   float* col_sums;            // kXentGrad: [32 rows][N], column sums of what is stored, or null
 };
 template <int KIND> struct ParamsOf { using type = PairParams; };
 template <> struct ParamsOf<kXentStats> { using type = XentParams; };
 template <> struct ParamsOf<kXentGrad> { using type = XentParams; };
+template <> struct ParamsOf<kXentKeep> { using type = XentParams; };
+
+// What kXentKeep stores of a logit: how far it is below the greatest of its row's 128 columns, in 16 bits of 2^-10 octaves.
+// The probability it stands for is right to 2^-11 octaves, 3.4e-4 of itself, a sixth of the rounding of the gradient to bf16,
+// whatever its size (fp16 would lose the small ones, bf16 has a coarser step); 64 octaves below count as 0.
+constexpr float kKeptStep = 1024.f;
+constexpr uint32_t kKeptZero = 65535u;
+// Two logits; `top` is the greatest in the same units.  2^23 is added instead of a conversion, which the unit of the
+// exponentials would do; a NaN becomes 0 here and is one again by its row's sum.
+__device__ __forceinline__ uint32_t kept_code2(float a, float b, float top) {
+  constexpr float kScale = -1.4426950408889634f * kKeptStep, kMost = static_cast<float>(kKeptZero);
+  const uint32_t x = __float_as_uint(fminf(fmaxf(fmaf(a, kScale, top), 0.f), kMost) + 8388608.f);
+  const uint32_t y = __float_as_uint(fminf(fmaxf(fmaf(b, kScale, top), 0.f), kMost) + 8388608.f);
+  return __byte_perm(x, y, 0x5410);
+}
+// The way back: 2^13 + code * 2^-10 has the code in its low half.
+__device__ __forceinline__ float kept_below(uint32_t pair, int which) {
+  static_assert(kKeptStep == 1024.f, "the step is 2^-10");
+  return __uint_as_float(__byte_perm(pair, 0x46000000u, which ? 0x7632 : 0x7610)) - 8192.f;
+}
 
 // The bias of N columns, what the sums of their logits start from.
 template <int N>
@@ -131,16 +152,16 @@ __device__ __forceinline__ float2 xent_row_stats(const XentParams& p, float* v, 
 }
 
 // Threads of a kind's CTA: the epilogues of cross entropy have two warps for each 32 rows.
-__host__ __device__ constexpr bool is_xent(int kind) { return kind == kXentStats || kind == kXentGrad; }
+__host__ __device__ constexpr bool is_xent(int kind) { return kind >= kXentStats; }
 __host__ __device__ constexpr int threads_of(int kind) { return is_xent(kind) ? 320 : kThreads; }
-__host__ __device__ constexpr int staged_tiles(int kind) { return kind == kAux || kind == kXentGrad ? 4 : 2; }
+__host__ __device__ constexpr int staged_tiles(int kind) { return kind == kAux || kind == kXentGrad || kind == kXentKeep ? 4 : 2; }
 
 template <bool A_MN, bool B_MN, int KIND>
 __global__ void __launch_bounds__(threads_of(KIND), 1)
 gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                  const __grid_constant__ CUtensorMap tma_c, const __grid_constant__ CUtensorMap tma_aux,
                  const typename ParamsOf<KIND>::type p) {
-  constexpr bool AUX = KIND == kAux, SPLIT = KIND == kSplit, XENT = is_xent(KIND), STATS = KIND == kXentStats;
+  constexpr bool AUX = KIND == kAux, SPLIT = KIND == kSplit, XENT = is_xent(KIND), KEEP = KIND == kXentKeep, STATS = KIND == kXentStats || KEEP;
   using L = Layout<staged_tiles(KIND) == 4>;
   constexpr int STAGES = L::kStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -375,6 +396,33 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
         const int lab = label_at(live, row, col0, 128);
         float target = 0.f;
         float2 mine = xent_row_stats(p, v, col0, lab, target);
+        if (lab >= 0) p.target[row] = target;
+        if constexpr (KEEP) {
+          if (live) p.stats[(2 * static_cast<size_t>(n0 / BN) + half) * p.M + row] = mine;
+          const float top = mine.x == -INFINITY ? 0.f : mine.x * kKeptStep;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            if (col0 + 64 * u >= p.N) break;
+            uint8_t* stg = smem + L::kStagingOffset + (2 * half + (stored & 1)) * L::kStagingBytes;
+            if (leader) tma_wait_read<1>();
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+              uint32_t c[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) c[i] = kept_code2(v[64 * u + 8 * g + 2 * i], v[64 * u + 8 * g + 2 * i + 1], top);
+              *reinterpret_cast<uint4*>(stg + r * 128 + ((g ^ (r & 7)) << 4)) = make_uint4(c[0], c[1], c[2], c[3]);
+            }
+            fence_async_smem();
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+            if (leader) {
+              tma_store_2d(&tma_c, stg, col0 + 64 * u, m0);
+              tma_commit();
+            }
+            ++stored;
+          }
+          continue;
+        }
         if (half) meet[parity * BM + r] = mine;
         asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
         if (!half) {
@@ -383,7 +431,6 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
           mine = make_float2(m, mine.y * mb::fast_exp2(mine.x - use) + other.y * mb::fast_exp2(other.x - use));
           if (live) p.stats[static_cast<size_t>(n0 / BN) * p.M + row] = mine;
         }
-        if (lab >= 0) p.target[row] = target;
       } else {
         // (softmax - [label]) * gradient of the loss, 0 in an ignored row; 64 columns at a time through staging
         const bool skipped = !live || p.labels[row] == p.ignore;
@@ -874,9 +921,96 @@ xent_bias_grad_kernel(const float* __restrict__ sums, void* __restrict__ out, in
   else static_cast<__nv_bfloat16*>(out)[c] = __float2bfloat16(a);
 }
 
+// Gradient of a piece of the logits from what kXentKeep stored: 32 rows x 512 columns per block, 8 columns of 8 rows per thread.
+// The label's column is computed from the logit itself, so that a row whose label is all but certain keeps its small gradient.
+// Bound by memory: 8192 x 12800 72 us, 5.8 TB/s (146 with conversions between integers and floats, which share the unit of the
+// exponentials, and every check per element).
+template <bool SUMS>
+__global__ void __launch_bounds__(256)
+xent_kept_grad_kernel(const uint16_t* __restrict__ kept, int ldk, const float2* __restrict__ stats, const float* __restrict__ target,
+                      const int64_t* __restrict__ labels, const float* __restrict__ lse, const float* __restrict__ gloss,
+                      __nv_bfloat16* __restrict__ out, int ldd, float* __restrict__ col_sums, int rows, int c0, int cols,
+                      int64_t v0, int64_t ignore) {
+  constexpr float kLog2e = 1.4426950408889634f;
+  __shared__ float top[4][32], grad[32], hit[32], part[3][SUMS ? 512 : 1];
+  __shared__ int at[32];
+  __shared__ bool skip[32];
+  const int tid = threadIdx.x, r0 = blockIdx.y * 32, col = blockIdx.x * 512 + 8 * (tid & 63), line = tid >> 6;
+  uint4 c[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int row = r0 + 4 * k + line;
+    if (col < cols && row < rows) c[k] = *reinterpret_cast<const uint4*>(kept + static_cast<size_t>(row) * ldk + c0 + col);
+  }
+  if (tid < 32) {
+    const int row = r0 + tid;
+    const bool none = row >= rows || labels[row] == ignore;
+    const int64_t a = none ? -1 : labels[row] - v0 - c0;
+    const bool here = a >= 0 && a < cols;
+    skip[tid] = none;
+    grad[tid] = none ? 0.f : gloss[row];
+    hit[tid] = here ? mb::fast_exp2(kLog2e * target[row] - kLog2e * lse[row]) - 1.f : 0.f;
+    at[tid] = here ? static_cast<int>(a) : -8;
+  } else if (tid >= 64 && tid < 192) {
+    const int q = (tid - 64) >> 5, row = r0 + (tid & 31), first = blockIdx.x * 512 + 128 * q;
+    if (row < rows && first < cols)
+      top[q][tid & 31] = stats[static_cast<size_t>((c0 + first) / 128) * rows + row].x - kLog2e * lse[row];
+  }
+  __syncthreads();
+  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (col < cols) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int in = 4 * k + line, row = r0 + in;
+      if (row >= rows) break;
+      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (!skip[in]) {
+        const float t = top[(tid & 63) >> 4][in], g = grad[in];
+        const uint32_t w[4] = {c[k].x, c[k].y, c[k].z, c[k].w};
+        uint32_t zeros = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) zeros |= (~w[i] - 0x00010001u) & w[i] & 0x80008000u;      // halves that are all ones
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = g * mb::fast_exp2(t - kept_below(w[i >> 1], i & 1));
+        const int label = at[in] - col;
+        if (zeros || static_cast<unsigned>(label) < 8u || col + 8 > cols) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (((w[i >> 1] >> (16 * (i & 1))) & 0xffffu) == kKeptZero) f[i] = 0.f;
+            if (i == label) f[i] = g * hit[in];
+            if (col + i >= cols) f[i] = 0.f;
+          }
+        }
+      }
+      const mb::bf16x8 packed = mb::pack8(f);
+      *reinterpret_cast<mb::bf16x8*>(out + static_cast<size_t>(row) * ldd + col) = packed;
+      if (SUMS) {
+        float s[8];
+        mb::unpack8(packed, s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] += s[i];
+      }
+    }
+  }
+  if (!SUMS) return;
+  if (line) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) part[line - 1][8 * (tid & 63) + i] = sum[i];
+  }
+  __syncthreads();
+  if (line || col >= cols) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (col + i < cols)
+      col_sums[static_cast<size_t>(blockIdx.y) * cols + col + i] =
+          (sum[i] + part[0][8 * tid + i]) + (part[1][8 * tid + i] + part[2][8 * tid + i]);
+  }
+}
+
 // Both operands K-major, the vocabulary on the B side; no rule on the number of tiles: there is one kernel for all sizes.
+// out: the gradient of the logits (kXentGrad), what is kept of them (kXentKeep), or nothing.
 int xent_gemm(const void* x, const void* w, void* dlogits, int ldd, XentParams& p, int ldx, int ldw, int max_ctas,
-              cudaStream_t stream) {
+              cudaStream_t stream, bool keep = false) {
   CUtensorMap ta, tb, tc, tx;
   memset(&tc, 0, sizeof(tc));
   memset(&tx, 0, sizeof(tx));
@@ -888,6 +1022,7 @@ int xent_gemm(const void* x, const void* w, void* dlogits, int ldd, XentParams& 
   p.splits = 1;
   max_ctas = clamp_ctas(max_ctas);
   if (max_ctas < 2) max_ctas = 2;      // a pair
+  if (keep) return launch<false, false, kXentKeep>(ta, tb, tc, tx, p, max_ctas, stream);
   return dlogits ? launch<false, false, kXentGrad>(ta, tb, tc, tx, p, max_ctas, stream)
                  : launch<false, false, kXentStats>(ta, tb, tc, tx, p, max_ctas, stream);
 }
@@ -938,10 +1073,13 @@ MB_API int mb_xent_linear_tiles(int V) { return (V + BN - 1) / BN; }
 // fp32, workspaces of this call.  out_stats null: loss [M] (0 where the label is `ignore`) and lse [M], natural logarithms;
 // a label outside [v0, v0 + V) has the logit 0.  out_stats [M][3]: {maximum, sum of exponentials relative to it, label's
 // logit (0 outside)} instead, which a group of vocabulary slices combines.  K and the leading dimensions multiples of 8.
-MB_API int mb_xent_linear_fwd(const void* x, const void* w, const void* bias, const int64_t* labels, float* stats,
-                              float* target, float* loss, float* lse, float* out_stats, int M, int V, int K, int ldx,
-                              int ldw, int64_t v0, int64_t ignore, int max_ctas, cudaStream_t stream) {
+// The first form also keeps 16 bits of every logit, kept [M][ldk] (ldk >= V, a multiple of 8), for the backward pass, which then
+// needs stats, [2 * tiles][M][2] here, and target as well.
+MB_API int mb_xent_linear_fwd_keep(const void* x, const void* w, const void* bias, const int64_t* labels, float* stats,
+                                   float* target, float* loss, float* lse, float* out_stats, void* kept, int ldk, int M, int V,
+                                   int K, int ldx, int ldw, int64_t v0, int64_t ignore, int max_ctas, cudaStream_t stream) {
   if (!xent_args_ok(x, w, M, V, K, ldx, ldw)) return -1;
+  if (kept && (ldk < V || ldk % 8 || (reinterpret_cast<uintptr_t>(kept) & 15))) return -1;
   if (M == 0) return 0;
   XentParams p;
   memset(&p, 0, sizeof(p));
@@ -953,11 +1091,17 @@ MB_API int mb_xent_linear_fwd(const void* x, const void* w, const void* bias, co
   p.segments = (K + 1023) / 1024;
   p.stats = reinterpret_cast<float2*>(stats);
   p.target = target;
-  const int rc = xent_gemm(x, w, nullptr, 0, p, ldx, ldw, max_ctas, stream);
+  const int rc = xent_gemm(x, w, kept, ldk, p, ldx, ldw, max_ctas, stream, kept != nullptr);
   if (rc != 0) return rc;
   xent_combine_kernel<<<(M + 31) / 32, 512, 0, stream>>>(p.stats, target, labels, loss, lse, out_stats, M,
-                                                         mb_xent_linear_tiles(V), V, v0, ignore);
+                                                         mb_xent_linear_tiles(V) * (kept ? 2 : 1), V, v0, ignore);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
+}
+MB_API int mb_xent_linear_fwd(const void* x, const void* w, const void* bias, const int64_t* labels, float* stats,
+                              float* target, float* loss, float* lse, float* out_stats, int M, int V, int K, int ldx,
+                              int ldw, int64_t v0, int64_t ignore, int max_ctas, cudaStream_t stream) {
+  return mb_xent_linear_fwd_keep(x, w, bias, labels, stats, target, loss, lse, out_stats, nullptr, 0, M, V, K, ldx, ldw, v0, ignore,
+                                 max_ctas, stream);
 }
 
 // Bytes of workspace of mb_xent_linear_bwd, which holds the gradient of `piece` columns of logits at a time.
@@ -971,12 +1115,14 @@ MB_API size_t mb_xent_linear_bwd_workspace(int M, int V, int K, int piece, int w
 // Gradients of the loss, gloss [M] being what it is differentiated by: with d[t,v] = (exp(logit - lse) - [label]) * gloss
 // (rows whose label is `ignore`: 0), computed again piece by piece and rounded to bf16, dx [M][K] = d w (bf16), dw [V][K]
 // (+)= d^T x (bf16 or fp32, row stride lddw), dbias [V] = column sums of d (bf16 or fp32).  dx, dw and dbias may be null.
-// piece: a multiple of 256, or V.
-MB_API int mb_xent_linear_bwd(const void* x, const void* w, const void* bias, const int64_t* labels, const float* lse,
-                              const float* gloss, void* dx, void* dw, void* dbias, int M, int V, int K, int ldx, int ldw,
-                              int lddw, int dw_fp32, int accumulate, int dbias_fp32, int64_t v0, int64_t ignore, int piece,
-                              int max_ctas, void* workspace, cudaStream_t stream) {
+// piece: a multiple of 256, or V.  The first form takes what the forward pass kept instead of computing the logits again.
+MB_API int mb_xent_linear_bwd_kept(const void* x, const void* w, const void* bias, const int64_t* labels, const float* lse,
+                                   const float* gloss, void* dx, void* dw, void* dbias, const void* kept, int ldk,
+                                   const float* stats, const float* target, int M, int V, int K, int ldx, int ldw, int lddw,
+                                   int dw_fp32, int accumulate, int dbias_fp32, int64_t v0, int64_t ignore, int piece,
+                                   int max_ctas, void* workspace, cudaStream_t stream) {
   if (!xent_args_ok(x, w, M, V, K, ldx, ldw) || M == 0 || piece <= 0) return -1;
+  if (kept && (ldk < V || ldk % 8 || (reinterpret_cast<uintptr_t>(kept) & 15) || (M + 31) / 32 > 65535)) return -1;
   if (piece >= V) piece = V;
   else if (piece % 256) return -1;
   if ((reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(workspace)) & 15) return -1;
@@ -1009,7 +1155,15 @@ MB_API int mb_xent_linear_bwd(const void* x, const void* w, const void* bias, co
     p.gloss = gloss;
     p.segments = 1;
     p.col_sums = sums;
-    int rc = xent_gemm(x, wp, dl, ldd, p, ldx, ldw, max_ctas, stream);
+    int rc = 0;
+    if (kept) {
+      (sums ? xent_kept_grad_kernel<true> : xent_kept_grad_kernel<false>)<<<dim3((n + 511) / 512, (M + 31) / 32), 256, 0, stream>>>(
+          static_cast<const uint16_t*>(kept), ldk, reinterpret_cast<const float2*>(stats), target, labels, lse, gloss,
+          static_cast<__nv_bfloat16*>(dl), ldd, sums, M, c0, n, v0, ignore);
+      if (cudaGetLastError() != cudaSuccess) rc = -4;
+    } else {
+      rc = xent_gemm(x, wp, dl, ldd, p, ldx, ldw, max_ctas, stream);
+    }
     if (rc == 0 && dbias) {
       void* dst = static_cast<uint8_t*>(dbias) + static_cast<size_t>(c0) * (dbias_fp32 ? 4 : 2);
       xent_bias_grad_kernel<<<(n + 31) / 32, 256, 0, stream>>>(sums, dst, (M + 31) / 32, n, dbias_fp32);
@@ -1024,6 +1178,13 @@ MB_API int mb_xent_linear_bwd(const void* x, const void* w, const void* bias, co
     if (rc != 0) return rc;
   }
   return dx && piece < V ? mb_cast_f32_to_bf16(dx32, dx, static_cast<size_t>(M) * K, 1.f, stream) : 0;
+}
+MB_API int mb_xent_linear_bwd(const void* x, const void* w, const void* bias, const int64_t* labels, const float* lse,
+                              const float* gloss, void* dx, void* dw, void* dbias, int M, int V, int K, int ldx, int ldw,
+                              int lddw, int dw_fp32, int accumulate, int dbias_fp32, int64_t v0, int64_t ignore, int piece,
+                              int max_ctas, void* workspace, cudaStream_t stream) {
+  return mb_xent_linear_bwd_kept(x, w, bias, labels, lse, gloss, dx, dw, dbias, nullptr, 0, nullptr, nullptr, M, V, K, ldx, ldw, lddw,
+                                 dw_fp32, accumulate, dbias_fp32, v0, ignore, piece, max_ctas, workspace, stream);
 }
 
 MB_API int mb_gemm_pair_bf16(const void* A, const void* B, void* C, int M, int N, int K, int lda, int ldb, int ldc,

@@ -55,6 +55,9 @@ class Settings:
     gemm_max_ctas = 0             # >0 leaves SMs free for a concurrent communication kernel
     # bytes of the bf16 gradient of the logits that linear_cross_entropy's backward pass holds at a time
     xent_piece_bytes = 256 << 20
+    # bytes that linear_cross_entropy may keep from the forward to the backward pass, 16 bits per logit; where that is not
+    # enough the logits are computed twice (0: always)
+    xent_keep_bytes = 2 << 30
     gemm_pair = True              # large GEMMs on CTA pairs (256 x 256 tiles, tcgen05 cta_group::2)
     fuse_mlp_gelu = True          # GELU MLP as one autograd node (gelu' folded into a dgrad GEMM epilogue)
     tp_backend = "nccl"           # "nccl" | "fused": sequence-parallel linears on the GEMM+collective kernels

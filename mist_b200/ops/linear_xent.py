@@ -1,9 +1,11 @@
-"""Vocabulary projection and cross entropy as one operator that never holds the logits.
+"""Vocabulary projection and cross entropy as one operator that holds neither the logits nor their gradient.
 
 ``loss[t] = log sum_v exp(x_t . w_v + b_v) - (x_t . w_label + b_label)``.  The forward pass is one GEMM whose epilogue
-keeps a maximum and a sum per row and tile; it stores two numbers per row for the backward pass.  That computes the
-logits again, a piece of the vocabulary at a time, turns them into their gradient in the GEMM's epilogue and multiplies
-the piece into the gradients of ``x`` and of the weight (reference: the projection of mist/modules/fused_dense.py:221-327
+keeps a maximum and a sum per row and tile.  The backward pass goes over the vocabulary piece by piece, gets the gradient
+of a piece's logits and multiplies it into the gradients of ``x`` and of the weight.  It has the logits from the forward
+pass, which keeps 16 bits of each while they take no more than ``Settings.xent_keep_bytes`` and the hidden size makes it
+worth while, or computes them again (8192 tokens of 2560, vocabulary 50304, both passes: 5.1 ms with 824 MB kept, 6.4 ms
+with two numbers per row) (reference: the projection of mist/modules/fused_dense.py:221-327
 followed by mist/modules/losses.py:48-176, which hold ``[tokens, vocabulary]`` logits between the two).
 """
 from __future__ import annotations
@@ -15,6 +17,10 @@ import torch
 from . import functional as F
 from . import native
 from .native import call, ptr, stream, use_native
+
+# Hidden sizes from which a logit is kept and not computed again.  Both passes of 4096 tokens, vocabulary 50304 (kept, twice, us):
+# hidden 2048 2329, 2664; 1024 1448, 1552; 512 963, 978; 256 771, 717; vocabulary 8192: 1024 217, 232; 512 187, 174.
+KEEP_FROM = 1024
 
 
 def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
@@ -32,6 +38,11 @@ def piece_columns(rows: int, vocab: int) -> int:
     most = max(256, F.Settings.xent_piece_bytes // (2 * max(rows, 1)) // 256 * 256)
     pieces = -(-vocab // most)
     return min(vocab, -(-(-(-vocab // pieces)) // 256) * 256)
+
+
+def keeps_logits(rows: int, vocab: int, k: int) -> bool:
+    """Whether the forward pass keeps 16 bits of every logit for the backward pass instead of computing the logits twice."""
+    return k >= KEEP_FROM and rows <= 2 ** 20 and 2 * rows * (-(-vocab // 8) * 8) <= F.Settings.xent_keep_bytes
 
 
 @functools.lru_cache(maxsize=1024)
@@ -53,13 +64,14 @@ def _combine_over_group(stats, labels, ignore_index, group):
 
 class _LinearXentFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, labels, v0, group, ignore_index):
+    def forward(ctx, x, weight, bias, labels, v0, group, ignore_index, backward):
         ctx.v0, ctx.ignore, ctx.x_shape = v0, ignore_index, x.shape
         ctx.param = F._bucket_owner(weight)
         vocab, k = weight.shape
         x2, w2 = _rows(x, k), weight
         rows = x2.shape[0]
         split = group is not None and torch.distributed.get_world_size(group) > 1
+        kept = None, None
         if not use_native(x2):
             logits = x2.float() @ weight.float().t()
             if bias is not None:
@@ -78,21 +90,26 @@ class _LinearXentFn(torch.autograd.Function):
         else:
             w2 = _rows(weight, k)
             tiles = native.kernels().mb_xent_linear_tiles(vocab)
-            # [tile][row] statistics, labels' logits, and per row: loss and lse, or what the group combines
-            work = torch.empty((2 * tiles + 1) * rows, dtype=torch.float32, device=x.device)
+            keeps = backward and keeps_logits(rows, vocab, k)
+            # [tile, or half of one][row] statistics, labels' logits, and per row: loss and lse, or what the group combines
+            entries = tiles * (2 if keeps else 1)
+            work = torch.empty((2 * entries + 1) * rows, dtype=torch.float32, device=x.device)
             out = torch.empty(3 if split else 2, rows, dtype=torch.float32, device=x.device)
             loss, lse = out[0], out[1]
-            call("mb_xent_linear_fwd", ptr(x2), ptr(w2), ptr(bias), ptr(labels), ptr(work), ptr(work) + 8 * tiles * rows,
-                 ptr(loss), ptr(lse), ptr(out) if split else 0, rows, vocab, k, x2.stride(0), w2.stride(0), v0, ignore_index,
-                 F.Settings.gemm_max_ctas, stream())
+            if keeps:
+                wide = -(-vocab // 8) * 8
+                kept = torch.empty(rows, wide, dtype=torch.int16, device=x.device), work
+            call("mb_xent_linear_fwd_keep", ptr(x2), ptr(w2), ptr(bias), ptr(labels), ptr(work), ptr(work) + 8 * entries * rows,
+                 ptr(loss), ptr(lse), ptr(out) if split else 0, ptr(kept[0]), wide if keeps else 0, rows, vocab, k, x2.stride(0),
+                 w2.stride(0), v0, ignore_index, F.Settings.gemm_max_ctas, stream())
             if split:
                 loss, lse = _combine_over_group(out.view(rows, 3), labels, ignore_index, group)
-        ctx.save_for_backward(x2, weight, bias, labels, lse)
+        ctx.save_for_backward(x2, weight, bias, labels, lse, *kept)
         return loss
 
     @staticmethod
     def backward(ctx, gloss):
-        x2, weight, bias, labels, lse = ctx.saved_tensors
+        x2, weight, bias, labels, lse, kept, stats = ctx.saved_tensors
         rows, k = x2.shape
         vocab = weight.shape[0]
         want_x, want_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
@@ -120,8 +137,9 @@ class _LinearXentFn(torch.autograd.Function):
             fp32 = int(dw is not None and dw.dtype == torch.float32)
             area = _backward_bytes(rows, vocab, k, piece, want_x, want_w, want_b, fp32, add, ctas)
             workspace = torch.empty(area, dtype=torch.uint8, device=x2.device)
-            call("mb_xent_linear_bwd", ptr(x2), ptr(w2), ptr(bias), ptr(labels), ptr(lse), ptr(gloss), ptr(dx), ptr(dw), ptr(db),
-                 rows, vocab, k, x2.stride(0), w2.stride(0), 0 if dw is None else dw.stride(0), fp32, add, 0, ctx.v0, ctx.ignore,
+            wide, target = (0, 0) if kept is None else (kept.shape[1], ptr(stats) + 4 * (stats.numel() - rows))
+            call("mb_xent_linear_bwd_kept", ptr(x2), ptr(w2), ptr(bias), ptr(labels), ptr(lse), ptr(gloss), ptr(dx), ptr(dw),
+                 ptr(db), ptr(kept), wide, ptr(stats), target, rows, vocab, k, x2.stride(0), w2.stride(0), 0 if dw is None else dw.stride(0), fp32, add, 0, ctx.v0, ctx.ignore,
                  piece, ctas, ptr(workspace), stream())
         else:
             _reference_backward(x2, weight, bias, labels, lse, gloss, ctx.v0, ctx.ignore, dx, dw, add, db)
@@ -131,7 +149,7 @@ class _LinearXentFn(torch.autograd.Function):
             ctx.param.grad_accumulate = True
         if dx is not None and dx.shape != ctx.x_shape:
             dx = dx.reshape(ctx.x_shape)
-        return (dx, dw if bucket is None else None, db, None, None, None, None)
+        return (dx, dw if bucket is None else None, db, None, None, None, None, None)
 
 
 def _reference_backward(x2, weight, bias, labels, lse, gloss, v0, ignore, dx, dw, accumulate, db):
@@ -178,5 +196,6 @@ def linear_cross_entropy(x, weight, labels, bias=None, vocab_start: int = 0, gro
         if bias is not None and not bias.is_contiguous():
             bias = bias.contiguous()
     flat = labels if labels.dim() == 1 else labels.reshape(-1)
-    loss = _LinearXentFn.apply(x, weight, bias, flat.long().contiguous(), int(vocab_start), group, int(ignore_index))
+    loss = _LinearXentFn.apply(x, weight, bias, flat.long().contiguous(), int(vocab_start), group, int(ignore_index),
+                               torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)))
     return loss if labels.dim() == 1 else loss.reshape(labels.shape)

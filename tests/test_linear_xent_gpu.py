@@ -26,6 +26,18 @@ def _case(rows, k, v, bias, ignored=0.2, seed=0):
     return x, w, b, labels, (torch.rand(rows, device=DEV) + 0.5) / rows
 
 
+
+@pytest.fixture(autouse=True, params=["kept", "computed twice"])
+def logits(request, monkeypatch):
+    """Every test with the logits kept for the backward pass, and with logits that are computed again.  What is kept is
+    right to 2^-11 octaves, 3.4e-4 of a probability: a sixth of half a step of bf16, which the bounds below count."""
+    from mist_b200.ops import linear_xent
+    monkeypatch.setattr(linear_xent, "KEEP_FROM", 0)
+    if request.param != "kept":
+        monkeypatch.setattr(F.Settings, "xent_keep_bytes", 0)
+    return request.param
+
+
 class _Exact:
     def __init__(self, x, w, b, labels, g):
         xd, wd = x.detach().double(), w.detach().double()
@@ -268,3 +280,68 @@ def test_bucket_off_the_stores_alignment(dtype, start):
         tol = 2 ** -8 * n * want.float().abs() * (1 + n) + 1e-6
         assert ((w.grad_bucket.float() - n * want.float()).abs() <= tol).all()
     assert not flat[:start].any() and not flat[start + 96 * 64:].any()
+
+
+def test_a_label_that_is_all_but_certain():
+    """Its gradient is the small rest to 1, which what is kept of the logit alone would get wrong by a tenth."""
+    torch.manual_seed(12)
+    rows, k, v = 96, 256, 1000
+    w = (torch.randn(v, k, device=DEV) / k ** 0.5).bfloat16().requires_grad_(True)
+    labels = torch.arange(rows, device=DEV) * 7
+    x = (12.5 * w.detach()[labels].float()).bfloat16().requires_grad_(True)
+    g = torch.rand(rows, device=DEV) + 0.5
+    exact = _Exact(x, w, None, labels, g)
+    rest = -exact.dl.gather(1, labels[:, None])[:, 0] / g
+    assert 1e-4 < rest.median() < 2e-2
+    loss = F.linear_cross_entropy(x, w, labels)
+    grads = torch.autograd.grad(loss, (x, w), g)
+    exact.check(loss, grads)
+    # row by row: dx of a row is what its own column of dl gives; bf16 of dl (2^-8 of each entry) and of dx
+    dl = exact.dl
+    for got, want, spread in zip(grads[0].double(), dl @ w.double(), (dl.square() @ w.double().square()).sum(1)):
+        assert (got - want).norm() <= BF * (2 * spread.sqrt() + want.norm())
+
+
+def test_a_second_backward_pass_gets_the_same(logits):
+    x, w, b, labels, g = _case(130, 72, 700, True)
+    loss = F.linear_cross_entropy(x, w, labels, b)
+    first = torch.autograd.grad(loss, (x, w, b), g, retain_graph=True)
+    again = torch.autograd.grad(loss, (x, w, b), g)
+    assert all(torch.equal(p, q) for p, q in zip(first, again))
+
+
+def test_what_is_kept(logits, monkeypatch):
+    """16 bits per logit, and not without need: no gradient wanted, or more than the limit."""
+    x, w, _, labels, g = _case(256, 64, 4096, False)
+
+    def held(fn):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        out = fn()
+        return torch.cuda.memory_allocated() - before, out
+
+    size = 2 * 256 * 4096
+    small = 4 * 256 * 16 * 8
+    n, loss = held(lambda: F.linear_cross_entropy(x, w, labels))
+    assert (size <= n <= size + small) if logits == "kept" else n <= small
+    del loss
+    with torch.no_grad():
+        n, loss = held(lambda: F.linear_cross_entropy(x, w, labels))
+    assert n <= small
+    monkeypatch.setattr(F.Settings, "xent_keep_bytes", size - 1)
+    n, loss = held(lambda: F.linear_cross_entropy(x, w, labels))
+    assert n <= small
+
+
+def test_rows_that_are_not_numbers():
+    """An ignored row of NaN has the loss 0 and no gradient of its own; a row of NaN with a label is NaN, the others are not."""
+    x, w, b, labels, g = _case(70, 64, 600, True, ignored=0.0)
+    with torch.no_grad():
+        x[5] = float("nan")
+        x[9] = float("nan")
+    labels[5] = -100
+    loss = F.linear_cross_entropy(x, w, labels, b)
+    dx, = torch.autograd.grad(loss, (x,), g)
+    assert loss[5] == 0 and not dx[5].any() and torch.isnan(loss[9]) and torch.isnan(dx[9]).all()
+    others = [i for i in range(70) if i not in (5, 9)]
+    assert torch.isfinite(loss[others]).all() and torch.isfinite(dx[others]).all()
