@@ -5,6 +5,8 @@ Tolerances.  A logit is a sum of k products in fp32, taken as off by at most k *
 gradient of a logit is rounded to bf16, off by at most 2^-8 of it; the gradients of x and of the weight sum those with
 signs that have nothing to do with one another, so the 2-norm of their error is held to 2^-8 of the root of the sum of
 the squared terms, and 2^-8 of the gradient itself for its own rounding."""
+import gc
+
 import pytest
 import torch
 
@@ -314,11 +316,15 @@ def test_what_is_kept(logits, monkeypatch):
     """16 bits per logit, and not without need: no gradient wanted, or more than the limit."""
     x, w, _, labels, g = _case(256, 64, 4096, False)
 
+    def asked():              # (a block that the allocator hands out may be larger)
+        return torch.cuda.memory_stats()["requested_bytes.all.current"]
+
     def held(fn):
+        gc.collect()              # what earlier tests left
         torch.cuda.synchronize()
-        before = torch.cuda.memory_allocated()
+        before = asked()
         out = fn()
-        return torch.cuda.memory_allocated() - before, out
+        return asked() - before, out
 
     size = 2 * 256 * 4096
     small = 4 * 256 * 16 * 8
@@ -345,3 +351,34 @@ def test_rows_that_are_not_numbers():
     assert loss[5] == 0 and not dx[5].any() and torch.isnan(loss[9]) and torch.isnan(dx[9]).all()
     others = [i for i in range(70) if i not in (5, 9)]
     assert torch.isfinite(loss[others]).all() and torch.isfinite(dx[others]).all()
+
+
+def test_slices_that_join_with_logits_kept():
+    """As above for slices of the vocabulary, each keeping its own logits; the log-sum-exp is that of all of them."""
+    rows, k, v, cut = 150, 128, 900, 333
+    x, w, b, labels, g = _case(rows, k, v, True)
+    exact = _Exact(x, w, b, labels, g)
+    lib, held, outs = native.kernels(), [], []
+    p = native.ptr
+    for a, e in ((0, cut), (cut, v)):
+        wide = (e - a + 7) // 8 * 8
+        stats, target = torch.empty(2 * lib.mb_xent_linear_tiles(e - a), rows, 2, device=DEV), torch.empty(rows, device=DEV)
+        kept, out = torch.empty(rows, wide, device=DEV, dtype=torch.int16), torch.full((rows, 3), float("nan"), device=DEV)
+        wa, ba = w.detach()[a:e].contiguous(), b.detach()[a:e].contiguous()
+        native.call("mb_xent_linear_fwd_keep", p(x), p(wa), p(ba), p(labels), p(stats), p(target), 0, 0, p(out), p(kept), wide, rows,
+                    e - a, k, k, k, a, -100, 0, native.stream())
+        held.append((a, e, wa, ba, stats, target, kept, wide))
+        outs.append(out)
+    top = torch.maximum(outs[0][:, 0], outs[1][:, 0])
+    lse = sum(o[:, 1] * torch.exp(o[:, 0] - top) for o in outs).log() + top
+    loss = torch.where(labels == -100, torch.zeros_like(lse), lse - outs[0][:, 2] - outs[1][:, 2])
+    parts = []
+    for a, e, wa, ba, stats, target, kept, wide in held:
+        dw, db = torch.empty(e - a, k, device=DEV, dtype=torch.bfloat16), torch.empty(e - a, device=DEV)
+        dx = torch.empty(rows, k, device=DEV, dtype=torch.bfloat16)
+        work = torch.empty(lib.mb_xent_linear_bwd_workspace(rows, e - a, k, 256, 1, 1, 1, 0, 0, 0), dtype=torch.uint8, device=DEV)
+        native.call("mb_xent_linear_bwd_kept", p(x), p(wa), p(ba), p(labels), p(lse), p(g), p(dx), p(dw), p(db), p(kept), wide,
+                    p(stats), p(target), rows, e - a, k, k, k, k, 0, 0, 1, a, -100, 256, 0, p(work), native.stream())
+        parts.append((dx.double(), dw, db))
+    native.check_status()
+    exact.check(loss, (parts[0][0] + parts[1][0], torch.cat([q[1] for q in parts]), torch.cat([q[2] for q in parts])))
