@@ -7,8 +7,8 @@
 // tokens of a row keep their order), then every row of the table is summed in fp32 by the threads that write it: each
 // row of dout is read once, each row of the table is written once in its own type, and the sums have one order, so
 // results repeat bit for bit.  The traffic that stays is that of the definition; it is bound by memory.
-// Measured: 16384 tokens of 2560, tables of 50304 and 2048 rows: lookup 40 us, sort 16, sums 67 (390 MB, 5.8 TB/s); 8192
-// tokens of 4096, 32000 rows: 25, 11, 51.  (A scatter with atomics into fp32 tables and a cast of those took 1300 us.)
+// Measured: 16384 tokens of 2560, tables of 50304 and 2048 rows: lookup 35 us, sort 16, sums 67 (390 MB, 5.8 TB/s); 8192
+// tokens of 4096, 32000 rows: 19, 11, 51.  (A scatter with atomics into fp32 tables and a cast of those took 1300 us.)
 //
 // Reference counterpart: the embedding modules of mist/modules/embedding.py:207-281 (gradient by torch's scatter-add).
 #include "common.cuh"
@@ -20,16 +20,41 @@ namespace cg = cooperative_groups;
 namespace {
 
 // ------------------------------------------------------------------------------------------------ lookup
-// One warp per token and slice of its row, `per_warp` vectors of 8 values, four rounds of loads in flight per lane (and
-// registers for four CTAs per SM: 16384 x 2560 with positions 76 -> 40 us).
+// N words of two values each, in one access of 16 or 32 bytes.
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t* w, const uint32_t* p) {
+  if (N == 8) {
+    asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[N - 4]), "=r"(w[N - 3]), "=r"(w[N - 2]), "=r"(w[N - 1])
+                 : "l"(p));
+  } else {
+    const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
+    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+  }
+}
+template <int N>
+__device__ __forceinline__ void store_words(uint32_t* p, const uint32_t* w) {
+  if (N == 8) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[N - 4]), "r"(w[N - 3]), "r"(w[N - 2]), "r"(w[N - 1]) : "memory");
+  } else {
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// One warp per token and slice of its row, `per_warp` vectors of 2 N values, 64 bytes of each table in flight per lane.  (In
+// accesses of 32 bytes 16384 x 2560 with positions take 34.8 us and 8192 x 4096 19.4, of 16 bytes 39.4 and 24.7; more CTAs per
+// SM with less in flight 36 - 50.)
+template <int N>
 __global__ void __launch_bounds__(256, 4)
-embed_fwd_kernel(const int64_t* __restrict__ ids, const int64_t* __restrict__ pos, const __nv_bfloat16* __restrict__ wte,
-                 const __nv_bfloat16* __restrict__ wpe, __nv_bfloat16* __restrict__ out, int tokens, int seq, int h, int64_t v0,
-                 int rows, int positions, float scale, int per_warp) {
+embed_fwd_kernel(const int64_t* __restrict__ ids, const int64_t* __restrict__ pos, const uint32_t* __restrict__ wte,
+                 const uint32_t* __restrict__ wpe, uint32_t* __restrict__ out, int tokens, int seq, int h, int64_t v0, int rows,
+                 int positions, float scale, int per_warp) {
+  constexpr int kRounds = 16 / N;
   const int lane = threadIdx.x & 31;
   const int t = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (t >= tokens) return;
-  const int vpr = h >> 3, from = blockIdx.y * per_warp, to = min(vpr, from + per_warp);
+  const int from = blockIdx.y * per_warp, to = min(h / (2 * N), from + per_warp);
   const int64_t row = ids[t] - v0;
   const bool in = row >= 0 && row < rows;
   int64_t p = -1;
@@ -37,33 +62,38 @@ embed_fwd_kernel(const int64_t* __restrict__ ids, const int64_t* __restrict__ po
     p = pos ? pos[t] : t % seq;
     if (p >= positions) p = -1;
   }
-  const mb::bf16x8* we = reinterpret_cast<const mb::bf16x8*>(wte + (in ? row : 0) * h);
-  const mb::bf16x8* pe = reinterpret_cast<const mb::bf16x8*>(wpe + (p >= 0 ? p : 0) * h);
-  mb::bf16x8* dst = reinterpret_cast<mb::bf16x8*>(out + static_cast<int64_t>(t) * h);
-  for (int c0 = from + lane; c0 < to; c0 += 128) {
-    mb::bf16x8 a[4], b[4];
+  const int64_t words = h >> 1;
+  const uint32_t* we = wte + (in ? row : 0) * words;
+  const uint32_t* pe = wpe + (p >= 0 ? p : 0) * words;
+  uint32_t* dst = out + t * words;
+  for (int c0 = from + lane; c0 < to; c0 += 32 * kRounds) {
+    uint32_t a[kRounds][N], b[kRounds][N];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      memset(&a[u], 0, sizeof(a[u]));
-      if (in && c0 + 32 * u < to) a[u] = we[c0 + 32 * u];
-      if (p >= 0 && c0 + 32 * u < to) b[u] = pe[c0 + 32 * u];
+    for (int u = 0; u < kRounds; ++u) {
+      memset(a[u], 0, sizeof(a[u]));
+      if (in && c0 + 32 * u < to) load_words<N>(a[u], we + static_cast<int64_t>(c0 + 32 * u) * N);
+      if (p >= 0 && c0 + 32 * u < to) load_words<N>(b[u], pe + static_cast<int64_t>(c0 + 32 * u) * N);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kRounds; ++u) {
       const int c = c0 + 32 * u;
       if (c >= to) break;
-      float f[8];
-      mb::unpack8(a[u], f);
-      if (p >= 0) {
-        float g[8];
-        mb::unpack8(b[u], g);
+      uint32_t o[N];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] = in ? fmaf(f[k], scale, g[k]) : g[k];
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] = in ? f[k] * scale : 0.f;
+      for (int k = 0; k < N; ++k) {
+        float x = __uint_as_float(a[u][k] << 16), y = __uint_as_float(a[u][k] & 0xffff0000u);
+        if (p >= 0) {
+          const float gx = __uint_as_float(b[u][k] << 16), gy = __uint_as_float(b[u][k] & 0xffff0000u);
+          x = in ? fmaf(x, scale, gx) : gx;
+          y = in ? fmaf(y, scale, gy) : gy;
+        } else {
+          x = in ? x * scale : 0.f;
+          y = in ? y * scale : 0.f;
+        }
+        const __nv_bfloat162 both = __floats2bfloat162_rn(x, y);
+        o[k] = *reinterpret_cast<const uint32_t*>(&both);
       }
-      dst[c] = mb::pack8(f);
+      store_words<N>(dst + static_cast<int64_t>(c) * N, o);
     }
   }
 }
@@ -589,11 +619,16 @@ MB_API int mb_embed_fwd(const int64_t* ids, const int64_t* pos, const void* wte,
   if (tokens < 0 || h <= 0 || h % 8 || rows < 0 || (wpe && !pos && seq <= 0)) return -1;
   if (!aligned16(wte) || !aligned16(wpe) || !aligned16(out)) return -1;
   if (tokens == 0) return 0;
-  // whole rows once they fill the chip (48 warps on each of 148 SMs); before that a row is cut into slices of 128 vectors
-  const int per_warp = tokens >= 7104 ? h / 8 : 128;
-  embed_fwd_kernel<<<dim3((tokens + 7) / 8, (h / 8 + per_warp - 1) / per_warp), 256, 0, stream>>>(
-      ids, pos, static_cast<const __nv_bfloat16*>(wte), static_cast<const __nv_bfloat16*>(wpe),
-      static_cast<__nv_bfloat16*>(out), tokens, seq, h, v0, rows, positions, scale, per_warp);
+  // rows of whole 32-byte sectors in accesses of as many bytes
+  const bool wide = h % 16 == 0 && ((reinterpret_cast<uintptr_t>(wte) | reinterpret_cast<uintptr_t>(wpe) |
+                                     reinterpret_cast<uintptr_t>(out)) & 31) == 0;
+  const int vectors = h / (wide ? 16 : 8);
+  // whole rows once they fill the chip (48 warps on each of 148 SMs); before that a row is cut into slices of 1024 values
+  const int per_warp = tokens >= 7104 ? vectors : (wide ? 64 : 128);
+  (wide ? embed_fwd_kernel<8> : embed_fwd_kernel<4>)<<<dim3((tokens + 7) / 8, (vectors + per_warp - 1) / per_warp), 256, 0,
+                                                      stream>>>(
+      ids, pos, static_cast<const uint32_t*>(wte), static_cast<const uint32_t*>(wpe), static_cast<uint32_t*>(out), tokens, seq, h,
+      v0, rows, positions, scale, per_warp);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 

@@ -173,8 +173,8 @@ def _reference_backward(x2, weight, bias, labels, lse, gloss, v0, ignore, dx, dw
 def linear_cross_entropy(x, weight, labels, bias=None, vocab_start: int = 0, group=None, ignore_index: int = -100):
     """Loss (fp32) of every row of ``x`` ``[..., hidden]`` against ``labels`` ``[...]``: the cross entropy of the logits
     ``x @ weight.T + bias``, which are computed in fp32 and never stored as such.  For the backward pass 16 bits of each are
-    kept while that takes no more than ``Settings.xent_keep_bytes``; otherwise it computes them again.  Rows labelled ``ignore_index`` have loss 0 and
-    give no gradient.  A label outside the vocabulary counts as one whose logit is 0; no one checks for it.
+    kept while that takes no more than ``Settings.xent_keep_bytes``; otherwise it computes them again.  Rows labelled
+    ``ignore_index`` have loss 0 and give no gradient.  A label outside the vocabulary counts as one whose logit is 0; no one checks for it.
 
     ``weight`` ``[vocab, hidden]`` (and ``bias`` ``[vocab]``) may be this rank's slice of the vocabulary, starting at
     ``vocab_start``; ``group`` is then the group of the slices, and ``x`` is the same on every rank of it (its gradient is

@@ -191,3 +191,18 @@ def test_refusals(case):
         ids = ids.cpu()
     with pytest.raises(ValueError):
         F.embedding(ids, wte)
+
+
+def test_tables_on_sixteen_bytes():
+    """Tables that begin between two 32-byte sectors: another width of accesses, the same bits."""
+    torch.manual_seed(4)
+    flat = torch.randn(8 + 300 * 64, device=DEV).bfloat16()
+    off = flat[8:].view(300, 64).requires_grad_(True)
+    on = flat[8:].view(300, 64).clone().requires_grad_(True)
+    assert off.data_ptr() % 32 == 16 and on.data_ptr() % 32 == 0
+    ids = torch.randint(0, 300, (2, 90), device=DEV)
+    g = torch.randn(2, 90, 64, device=DEV).bfloat16()
+    a, b = F.embedding(ids, off, off, scale=1.5), F.embedding(ids, on, on, scale=1.5)
+    assert torch.equal(a, b)
+    assert torch.equal(a, (1.5 * on[ids].float() + on[:90].float()).bfloat16())
+    assert torch.equal(*(torch.autograd.grad(x, t, g)[0] for x, t in ((a, off), (b, on))))
