@@ -982,13 +982,10 @@ xent_kept_grad_kernel(const uint16_t* __restrict__ kept, int ldk, const float2* 
           }
         }
       }
-      const mb::bf16x8 packed = mb::pack8(f);
-      *reinterpret_cast<mb::bf16x8*>(out + static_cast<size_t>(row) * ldd + col) = packed;
-      if (SUMS) {
-        float s[8];
-        mb::unpack8(packed, s);
+      *reinterpret_cast<mb::bf16x8*>(out + static_cast<size_t>(row) * ldd + col) = mb::pack8(f);
+      if (SUMS) {      // before the rounding
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum[i] += s[i];
+        for (int i = 0; i < 8; ++i) sum[i] += f[i];
       }
     }
   }
