@@ -1070,11 +1070,11 @@ MB_API int mb_xent_linear_tiles(int V) { return (V + BN - 1) / BN; }
 // fp32, workspaces of this call.  out_stats null: loss [M] (0 where the label is `ignore`) and lse [M], natural logarithms;
 // a label outside [v0, v0 + V) has the logit 0.  out_stats [M][3]: {maximum, sum of exponentials relative to it, label's
 // logit (0 outside)} instead, which a group of vocabulary slices combines.  K and the leading dimensions multiples of 8.
-// The first form also keeps 16 bits of every logit, kept [M][ldk] (ldk >= V, a multiple of 8), for the backward pass, which then
-// needs stats, [2 * tiles][M][2] here, and target as well.
-MB_API int mb_xent_linear_fwd_keep(const void* x, const void* w, const void* bias, const int64_t* labels, float* stats,
-                                   float* target, float* loss, float* lse, float* out_stats, void* kept, int ldk, int M, int V,
-                                   int K, int ldx, int ldw, int64_t v0, int64_t ignore, int max_ctas, cudaStream_t stream) {
+// Where kept is given, 16 bits of every logit are stored there, [M][ldk] (ldk >= V, a multiple of 8), for the backward pass, which
+// then needs stats, [2 * tiles][M][2] in this case, and target as well.
+MB_API int mb_xent_linear_fwd(const void* x, const void* w, const void* bias, const int64_t* labels, float* stats,
+                              float* target, float* loss, float* lse, float* out_stats, void* kept, int ldk, int M, int V, int K,
+                              int ldx, int ldw, int64_t v0, int64_t ignore, int max_ctas, cudaStream_t stream) {
   if (!xent_args_ok(x, w, M, V, K, ldx, ldw)) return -1;
   if (kept && (ldk < V || ldk % 8 || (reinterpret_cast<uintptr_t>(kept) & 15))) return -1;
   if (M == 0) return 0;
@@ -1094,13 +1094,6 @@ MB_API int mb_xent_linear_fwd_keep(const void* x, const void* w, const void* bia
                                                          mb_xent_linear_tiles(V) * (kept ? 2 : 1), V, v0, ignore);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
-MB_API int mb_xent_linear_fwd(const void* x, const void* w, const void* bias, const int64_t* labels, float* stats,
-                              float* target, float* loss, float* lse, float* out_stats, int M, int V, int K, int ldx,
-                              int ldw, int64_t v0, int64_t ignore, int max_ctas, cudaStream_t stream) {
-  return mb_xent_linear_fwd_keep(x, w, bias, labels, stats, target, loss, lse, out_stats, nullptr, 0, M, V, K, ldx, ldw, v0, ignore,
-                                 max_ctas, stream);
-}
-
 // Bytes of workspace of mb_xent_linear_bwd, which holds the gradient of `piece` columns of logits at a time.
 MB_API size_t mb_xent_linear_bwd_workspace(int M, int V, int K, int piece, int want_x, int want_w, int want_b, int dw_fp32,
                                            int accumulate, int max_ctas) {
@@ -1112,12 +1105,12 @@ MB_API size_t mb_xent_linear_bwd_workspace(int M, int V, int K, int piece, int w
 // Gradients of the loss, gloss [M] being what it is differentiated by: with d[t,v] = (exp(logit - lse) - [label]) * gloss
 // (rows whose label is `ignore`: 0), computed again piece by piece and rounded to bf16, dx [M][K] = d w (bf16), dw [V][K]
 // (+)= d^T x (bf16 or fp32, row stride lddw), dbias [V] = column sums of d (bf16 or fp32).  dx, dw and dbias may be null.
-// piece: a multiple of 256, or V.  The first form takes what the forward pass kept instead of computing the logits again.
-MB_API int mb_xent_linear_bwd_kept(const void* x, const void* w, const void* bias, const int64_t* labels, const float* lse,
-                                   const float* gloss, void* dx, void* dw, void* dbias, const void* kept, int ldk,
-                                   const float* stats, const float* target, int M, int V, int K, int ldx, int ldw, int lddw,
-                                   int dw_fp32, int accumulate, int dbias_fp32, int64_t v0, int64_t ignore, int piece,
-                                   int max_ctas, void* workspace, cudaStream_t stream) {
+// piece: a multiple of 256, or V.  kept, stats and target: what the forward pass kept, or null to compute the logits again.
+MB_API int mb_xent_linear_bwd(const void* x, const void* w, const void* bias, const int64_t* labels, const float* lse,
+                              const float* gloss, void* dx, void* dw, void* dbias, const void* kept, int ldk, const float* stats,
+                              const float* target, int M, int V, int K, int ldx, int ldw, int lddw, int dw_fp32, int accumulate,
+                              int dbias_fp32, int64_t v0, int64_t ignore, int piece, int max_ctas, void* workspace,
+                              cudaStream_t stream) {
   if (!xent_args_ok(x, w, M, V, K, ldx, ldw) || M == 0 || piece <= 0) return -1;
   if (kept && (ldk < V || ldk % 8 || (reinterpret_cast<uintptr_t>(kept) & 15) || (M + 31) / 32 > 65535)) return -1;
   if (piece >= V) piece = V;
@@ -1175,13 +1168,6 @@ MB_API int mb_xent_linear_bwd_kept(const void* x, const void* w, const void* bia
     if (rc != 0) return rc;
   }
   return dx && piece < V ? mb_cast_f32_to_bf16(dx32, dx, static_cast<size_t>(M) * K, 1.f, stream) : 0;
-}
-MB_API int mb_xent_linear_bwd(const void* x, const void* w, const void* bias, const int64_t* labels, const float* lse,
-                              const float* gloss, void* dx, void* dw, void* dbias, int M, int V, int K, int ldx, int ldw,
-                              int lddw, int dw_fp32, int accumulate, int dbias_fp32, int64_t v0, int64_t ignore, int piece,
-                              int max_ctas, void* workspace, cudaStream_t stream) {
-  return mb_xent_linear_bwd_kept(x, w, bias, labels, lse, gloss, dx, dw, dbias, nullptr, 0, nullptr, nullptr, M, V, K, ldx, ldw, lddw,
-                                 dw_fp32, accumulate, dbias_fp32, v0, ignore, piece, max_ctas, workspace, stream);
 }
 
 MB_API int mb_gemm_pair_bf16(const void* A, const void* B, void* C, int M, int N, int K, int lda, int ldb, int ldc,

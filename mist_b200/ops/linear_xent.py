@@ -99,7 +99,7 @@ class _LinearXentFn(torch.autograd.Function):
             if keeps:
                 wide = -(-vocab // 8) * 8
                 kept = torch.empty(rows, wide, dtype=torch.int16, device=x.device), work
-            call("mb_xent_linear_fwd_keep", ptr(x2), ptr(w2), ptr(bias), ptr(labels), ptr(work), ptr(work) + 8 * entries * rows,
+            call("mb_xent_linear_fwd", ptr(x2), ptr(w2), ptr(bias), ptr(labels), ptr(work), ptr(work) + 8 * entries * rows,
                  ptr(loss), ptr(lse), ptr(out) if split else 0, ptr(kept[0]), wide if keeps else 0, rows, vocab, k, x2.stride(0),
                  w2.stride(0), v0, ignore_index, F.Settings.gemm_max_ctas, stream())
             if split:
@@ -138,7 +138,7 @@ class _LinearXentFn(torch.autograd.Function):
             area = _backward_bytes(rows, vocab, k, piece, want_x, want_w, want_b, fp32, add, ctas)
             workspace = torch.empty(area, dtype=torch.uint8, device=x2.device)
             wide, target = (0, 0) if kept is None else (kept.shape[1], ptr(stats) + 4 * (stats.numel() - rows))
-            call("mb_xent_linear_bwd_kept", ptr(x2), ptr(w2), ptr(bias), ptr(labels), ptr(lse), ptr(gloss), ptr(dx), ptr(dw),
+            call("mb_xent_linear_bwd", ptr(x2), ptr(w2), ptr(bias), ptr(labels), ptr(lse), ptr(gloss), ptr(dx), ptr(dw),
                  ptr(db), ptr(kept), wide, ptr(stats), target, rows, vocab, k, x2.stride(0), w2.stride(0), 0 if dw is None else dw.stride(0), fp32, add, 0, ctx.v0, ctx.ignore,
                  piece, ctas, ptr(workspace), stream())
         else:

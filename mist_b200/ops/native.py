@@ -66,11 +66,9 @@ _SIGNATURES = {
     "mb_xent_loss": ([_p, _p, _p, _p, _i, _i, _p], _i),
     "mb_xent_bwd": ([_p, _p, _p, _p, _f, _i, _i, _i, _i, _i, _i, _p], _i),
     "mb_xent_linear_tiles": ([_i], _i),
-    "mb_xent_linear_fwd": ([_p] * 9 + [_i] * 5 + [_l, _l, _i, _p], _i),
-    "mb_xent_linear_fwd_keep": ([_p] * 10 + [_i] * 6 + [_l, _l, _i, _p], _i),
+    "mb_xent_linear_fwd": ([_p] * 10 + [_i] * 6 + [_l, _l, _i, _p], _i),
     "mb_xent_linear_bwd_workspace": ([_i] * 10, _z),
-    "mb_xent_linear_bwd_kept": ([_p] * 10 + [_i, _p, _p] + [_i] * 9 + [_l, _l, _i, _i, _p, _p], _i),
-    "mb_xent_linear_bwd": ([_p] * 9 + [_i] * 9 + [_l, _l, _i, _i, _p, _p], _i),
+    "mb_xent_linear_bwd": ([_p] * 10 + [_i, _p, _p] + [_i] * 9 + [_l, _l, _i, _i, _p, _p], _i),
     "mb_causal_softmax_fwd": ([_p, _p, _z, _i, _i, _f, _i, _p], _i),
     "mb_causal_softmax_bwd": ([_p, _p, _p, _z, _i, _f, _p], _i),
     "mb_adam_step": ([_p, _p, _p, _p, _i, _p, _z, _f, _f, _f, _f, _f, _i, _f, _i, _p], _i),

@@ -123,7 +123,7 @@ def test_labels_outside_the_slice_and_slices_that_join():
             work, out = torch.empty(tiles, rows, 2, device=DEV), torch.full((rows, 3), float("nan"), device=DEV)
             target, bias = torch.empty(rows, device=DEV), b[a:e].contiguous()
             native.call("mb_xent_linear_fwd", native.ptr(x), native.ptr(w) + 2 * k * a, native.ptr(bias), native.ptr(labels),
-                        native.ptr(work), native.ptr(target), 0, 0, native.ptr(out), rows, e - a, k, k, k, a, -100, 0,
+                        native.ptr(work), native.ptr(target), 0, 0, native.ptr(out), 0, 0, rows, e - a, k, k, k, a, -100, 0,
                         native.stream())
             stats.append(out)
         top = torch.maximum(stats[0][:, 0], stats[1][:, 0])
@@ -138,8 +138,8 @@ def test_labels_outside_the_slice_and_slices_that_join():
             work = torch.empty(lib.mb_xent_linear_bwd_workspace(rows, e - a, k, e - a, 1, 1, 1, 0, 0, 0), dtype=torch.uint8,
                                device=DEV)
             native.call("mb_xent_linear_bwd", native.ptr(x), native.ptr(wa), native.ptr(ba), native.ptr(labels), native.ptr(lse),
-                        native.ptr(g), native.ptr(dx), native.ptr(dw), native.ptr(db), rows, e - a, k, k, k, k, 0, 0, 1, a, -100,
-                        e - a, 0, native.ptr(work), native.stream())
+                        native.ptr(g), native.ptr(dx), native.ptr(dw), native.ptr(db), 0, 0, 0, 0, rows, e - a, k, k, k, k, 0,
+                        0, 1, a, -100, e - a, 0, native.ptr(work), native.stream())
             parts.append((dx.double(), dw, db))
     exact.check(loss, (parts[0][0] + parts[1][0], torch.cat([p[1] for p in parts]), torch.cat([p[2] for p in parts])))
 
@@ -365,7 +365,7 @@ def test_slices_that_join_with_logits_kept():
         stats, target = torch.empty(2 * lib.mb_xent_linear_tiles(e - a), rows, 2, device=DEV), torch.empty(rows, device=DEV)
         kept, out = torch.empty(rows, wide, device=DEV, dtype=torch.int16), torch.full((rows, 3), float("nan"), device=DEV)
         wa, ba = w.detach()[a:e].contiguous(), b.detach()[a:e].contiguous()
-        native.call("mb_xent_linear_fwd_keep", p(x), p(wa), p(ba), p(labels), p(stats), p(target), 0, 0, p(out), p(kept), wide, rows,
+        native.call("mb_xent_linear_fwd", p(x), p(wa), p(ba), p(labels), p(stats), p(target), 0, 0, p(out), p(kept), wide, rows,
                     e - a, k, k, k, a, -100, 0, native.stream())
         held.append((a, e, wa, ba, stats, target, kept, wide))
         outs.append(out)
@@ -377,7 +377,7 @@ def test_slices_that_join_with_logits_kept():
         dw, db = torch.empty(e - a, k, device=DEV, dtype=torch.bfloat16), torch.empty(e - a, device=DEV)
         dx = torch.empty(rows, k, device=DEV, dtype=torch.bfloat16)
         work = torch.empty(lib.mb_xent_linear_bwd_workspace(rows, e - a, k, 256, 1, 1, 1, 0, 0, 0), dtype=torch.uint8, device=DEV)
-        native.call("mb_xent_linear_bwd_kept", p(x), p(wa), p(ba), p(labels), p(lse), p(g), p(dx), p(dw), p(db), p(kept), wide,
+        native.call("mb_xent_linear_bwd", p(x), p(wa), p(ba), p(labels), p(lse), p(g), p(dx), p(dw), p(db), p(kept), wide,
                     p(stats), p(target), rows, e - a, k, k, k, k, 0, 0, 1, a, -100, 256, 0, p(work), native.stream())
         parts.append((dx.double(), dw, db))
     native.check_status()
