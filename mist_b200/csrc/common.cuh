@@ -21,6 +21,7 @@ enum MbStatus : int {
   MB_ERR_TIMEOUT_TMEM = 3,     // epilogue / MMA gave up waiting for an accumulator
   MB_ERR_TIMEOUT_PEER = 4,     // a flag written by another rank never arrived
   MB_ERR_BAD_ARG = 5,
+  MB_ERR_POSITION = 6,         // a position outside the table of positions (the row got none)
 };
 
 namespace mb {

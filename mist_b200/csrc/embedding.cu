@@ -15,6 +15,8 @@
 #include <cooperative_groups.h>
 #include <string.h>
 
+MB_API int* mb_status_device_ptr();
+
 namespace cg = cooperative_groups;
 
 namespace {
@@ -49,7 +51,7 @@ template <int N>
 __global__ void __launch_bounds__(256, 4)
 embed_fwd_kernel(const int64_t* __restrict__ ids, const int64_t* __restrict__ pos, const uint32_t* __restrict__ wte,
                  const uint32_t* __restrict__ wpe, uint32_t* __restrict__ out, int tokens, int seq, int h, int64_t v0, int rows,
-                 int positions, float scale, int per_warp) {
+                 int positions, float scale, int per_warp, bool strict, int* status) {
   constexpr int kRounds = 16 / N;
   const int lane = threadIdx.x & 31;
   const int t = blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -60,7 +62,11 @@ embed_fwd_kernel(const int64_t* __restrict__ ids, const int64_t* __restrict__ po
   int64_t p = -1;
   if (wpe) {
     p = pos ? pos[t] : t % seq;
-    if (p >= positions) p = -1;
+    if (strict && p < 0) p += positions;
+    if (p < 0 || p >= positions) {
+      if (strict && status && lane == 0 && blockIdx.y == 0) atomicCAS(status, 0, MB_ERR_POSITION);
+      p = -1;
+    }
   }
   const int64_t words = h >> 1;
   const uint32_t* we = wte + (in ? row : 0) * words;
@@ -116,6 +122,7 @@ struct Sort {
   int64_t v0;
   int rows;          // keys are 0 ... rows - 1, and rows for tokens that belong to no row
   int passes;
+  bool from_end;     // negative rows count from the end
   Area area;
 };
 
@@ -192,7 +199,8 @@ __device__ __forceinline__ int sort_place(const SortSpace& z, unsigned digit, in
   return at;
 }
 __device__ __forceinline__ uint32_t row_of(const Sort& s, int i) {
-  const int64_t r = s.ids[i] - s.v0;
+  int64_t r = s.ids[i] - s.v0;
+  if (s.from_end && r < 0) r += s.rows;
   return (r >= 0 && r < s.rows) ? static_cast<uint32_t>(r) : static_cast<uint32_t>(s.rows);
 }
 
@@ -590,6 +598,7 @@ Sort make_sort(const int64_t* ids, int64_t v0, int rows, uint8_t* at, int tokens
   s.ids = ids;
   s.v0 = v0;
   s.rows = rows;
+  s.from_end = false;
   s.passes = 1;
   while (s.passes < 4 && (static_cast<uint32_t>(rows) >> (8 * s.passes))) ++s.passes;
   s.area = make_area(at, tokens, h);
@@ -613,9 +622,10 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 }  // namespace
 
 // out [tokens][h] = scale * wte[ids - v0] + wpe[pos]; wpe may be null; pos null: position t % seq.  Ids outside the rows of
-// wte and positions outside those of wpe add nothing.  h a multiple of 8, tables and out on 16 bytes.
+// wte and positions outside those of wpe add nothing; strict: negative positions count from the end of wpe, and ones outside
+// it are reported as well.  h a multiple of 8, tables and out on 16 bytes.
 MB_API int mb_embed_fwd(const int64_t* ids, const int64_t* pos, const void* wte, const void* wpe, void* out, int tokens,
-                        int seq, int h, int64_t v0, int rows, int positions, float scale, cudaStream_t stream) {
+                        int seq, int h, int64_t v0, int rows, int positions, int strict, float scale, cudaStream_t stream) {
   if (tokens < 0 || h <= 0 || h % 8 || rows < 0 || (wpe && !pos && seq <= 0)) return -1;
   if (!aligned16(wte) || !aligned16(wpe) || !aligned16(out)) return -1;
   if (tokens == 0) return 0;
@@ -628,7 +638,7 @@ MB_API int mb_embed_fwd(const int64_t* ids, const int64_t* pos, const void* wte,
   (wide ? embed_fwd_kernel<8> : embed_fwd_kernel<4>)<<<dim3((tokens + 7) / 8, (vectors + per_warp - 1) / per_warp), 256, 0,
                                                       stream>>>(
       ids, pos, static_cast<const uint32_t*>(wte), static_cast<const uint32_t*>(wpe), static_cast<uint32_t*>(out), tokens, seq, h,
-      v0, rows, positions, scale, per_warp);
+      v0, rows, positions, scale, per_warp, strict != 0, strict ? mb_status_device_ptr() : nullptr);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
@@ -639,9 +649,9 @@ MB_API size_t mb_embed_bwd_workspace(int tokens, int h, int with_positions) {
 
 // dout [tokens][h] -> dwte [rows][h] (fp32 or bf16, stored or added to) and, where dwpe is not null, dwpe [positions][h]
 // (bf16, stored).  pos null: position t % seq.  Every row of a stored table is written; rows that get no token are left
-// alone where it is added to.  The workspace is for this call alone, on 16 bytes.  dwte may be null.
+// alone where it is added to.  strict: as in the lookup.  The workspace is for this call alone, on 16 bytes.  dwte may be null.
 MB_API int mb_embed_bwd(const int64_t* ids, const int64_t* pos, const void* dout, void* dwte, void* dwpe, int tokens, int seq,
-                        int h, int64_t v0, int rows, int positions, float scale, int dwte_fp32, int accumulate,
+                        int h, int64_t v0, int rows, int positions, int strict, float scale, int dwte_fp32, int accumulate,
                         void* workspace, cudaStream_t stream) {
   if (tokens < 0 || h <= 0 || h % 8 || rows < 0 || positions < 0 || (dwpe && !pos && seq <= 0)) return -1;
   if (!aligned16(dout) || !aligned16(dwte) || !aligned16(dwpe) || !aligned16(workspace)) return -1;
@@ -658,6 +668,7 @@ MB_API int mb_embed_bwd(const int64_t* ids, const int64_t* pos, const void* dout
   }
   if (sort1) {
     s[nsort] = make_sort(pos, 0, positions, at + nsort * area_bytes(tokens, h), tokens, h);
+    s[nsort].from_end = strict != 0;
     t[1] = make_table(s[nsort++], dwpe, 1.f);
   } else if (dwpe) {
     t[1].out = dwpe;

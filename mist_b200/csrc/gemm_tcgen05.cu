@@ -502,9 +502,14 @@ MB_API int mb_status_read_and_clear() {
 }
 
 MB_API int* mb_status_device_ptr() {
-  static int* p = nullptr;  // one process drives one device
-  if (!p && cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_mb_status) != cudaSuccess)
+  static int* of_device[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  int*& p = of_device[dev];
+  if (!p && cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_mb_status) != cudaSuccess) {
+    p = nullptr;
     return nullptr;
+  }
   return p;
 }
 

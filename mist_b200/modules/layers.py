@@ -211,7 +211,7 @@ class VocabParallelEmbedding(nn.Module):
         wpe = self.position_embeddings.weight if self.position_embeddings is not None else None
         use_pos = wpe is not None and (ws == 1 or group_rank(self.process_group) == 0)
         x = F.embedding(input_ids, self.word_embeddings.weight, wpe if use_pos else None, self.vocab_start,
-                        position_ids=position_ids)
+                        position_ids=position_ids, strict_positions=True)
         if tokentype_ids is not None and self.tokentype_embeddings is not None:
             tt = self.tokentype_embeddings(tokentype_ids)
             x = x + (tt if ws == 1 or group_rank(self.process_group) == 0 else 0)

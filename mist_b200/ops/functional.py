@@ -1130,14 +1130,23 @@ def _elsewhere(t) -> bool:
     return t.is_cuda and t.get_device() != torch._C._cuda_getDevice()
 
 
-def _flat_positions(position_ids, ids):
-    """Explicit positions in the shape of ``ids``, or ``None``."""
+def _flat_positions(position_ids, ids, rows: int, strict: bool):
+    """Explicit positions in the shape of ``ids`` on their device, or ``None``.  ``strict``: those on the host are looked over
+    as indices of a table of ``rows`` rows."""
     if position_ids is None:
         return None
-    if position_ids.is_floating_point() or position_ids.device != ids.device:
-        raise ValueError("position_ids: integers on the device of the ids expected")
+    if position_ids.is_floating_point() or (position_ids.device != ids.device and position_ids.device.type != "cpu"):
+        raise ValueError("position_ids: integers on the device of the ids, or on the host, expected")
+    if strict and position_ids.device.type == "cpu" and position_ids.numel():
+        low, high = (int(x) for x in position_ids.aminmax())
+        if low < -rows or high >= rows:
+            raise IndexError(f"positions from {low} to {high}, but the table has {rows}")
+        if low < 0:
+            position_ids = torch.where(position_ids < 0, position_ids + rows, position_ids)
     if position_ids.shape != ids.shape:
         position_ids = position_ids.expand(ids.shape)
+    if position_ids.device != ids.device:
+        position_ids = position_ids.to(ids.device)
     return position_ids.long().contiguous()
 
 
@@ -1148,10 +1157,10 @@ def _embed_workspace(tokens: int, h: int, with_positions: int) -> int:
 
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ids, wte, wpe, v0, scale, pos):
+    def forward(ctx, ids, wte, wpe, v0, scale, pos, strict):
         b, s = ids.shape
         h = wte.shape[1]
-        ctx.v0, ctx.scale = v0, scale
+        ctx.v0, ctx.scale, ctx.strict = v0, scale, strict
         ctx.has_pos = wpe is not None
         ctx.param = _bucket_owner(wte)
         ctx.save_for_backward(ids, wte, wpe, pos)
@@ -1167,7 +1176,7 @@ class _EmbeddingFn(torch.autograd.Function):
             return out.to(wte.dtype)
         out = torch.empty(b, s, h, dtype=wte.dtype, device=wte.device)
         call("mb_embed_fwd", ptr(ids), ptr(pos), ptr(wte), ptr(wpe), ptr(out), b * s, max(s, 1), h, v0, wte.shape[0],
-             0 if wpe is None else wpe.shape[0], scale, stream())
+             0 if wpe is None else wpe.shape[0], strict, scale, stream())
         return out
 
     @staticmethod
@@ -1189,7 +1198,7 @@ class _EmbeddingFn(torch.autograd.Function):
             elif dwpe is not None:
                 known = ((pos >= 0) & (pos < wpe.shape[0])).reshape(-1)
                 dwpe.index_add_(0, pos.reshape(-1)[known], d2[known])
-            return None, dwte.to(wte.dtype), None if dwpe is None else dwpe.to(wpe.dtype), None, None, None
+            return None, dwte.to(wte.dtype), None if dwpe is None else dwpe.to(wpe.dtype), None, None, None, None
         bucket = getattr(ctx.param, "grad_bucket", None) if want_wte else None
         accumulate = bucket is not None and bool(getattr(ctx.param, "grad_accumulate", False))
         direct = (bucket is not None and bucket.dtype in (torch.float32, torch.bfloat16) and bucket.is_contiguous()
@@ -1205,41 +1214,43 @@ class _EmbeddingFn(torch.autograd.Function):
             dout = dout.clone()
         workspace = torch.empty(_embed_workspace(b * s, h, int(want_wpe and pos is not None)), dtype=torch.uint8, device=wte.device)
         call("mb_embed_bwd", ptr(ids), ptr(pos), ptr(dout), ptr(dwte), ptr(dwpe), b * s, max(s, 1), h, ctx.v0, wte.shape[0],
-             wpe.shape[0] if want_wpe else 0, ctx.scale, int(dwte is not None and dwte.dtype == torch.float32),
+             wpe.shape[0] if want_wpe else 0, ctx.strict, ctx.scale, int(dwte is not None and dwte.dtype == torch.float32),
              int(direct and accumulate), ptr(workspace), stream())
         if bucket is None:
-            return None, dwte, dwpe, None, None, None
+            return None, dwte, dwpe, None, None, None, None
         if not direct:
             bucket.add_(dwte) if accumulate else bucket.copy_(dwte)      # any type, order and start
         ctx.param.grad_accumulate = True
-        return None, None, dwpe, None, None, None
+        return None, None, dwpe, None, None, None, None
 
 
-def embedding(ids, wte, wpe=None, vocab_start: int = 0, scale: float = 1.0, position_ids=None):
+def embedding(ids, wte, wpe=None, vocab_start: int = 0, scale: float = 1.0, position_ids=None, strict_positions: bool = False):
     """``scale * wte[ids - vocab_start]`` (zero outside this rank's slice) ``+ wpe[position]``.
 
     ``ids``: ``[batch, seq]``; the position of a token is its place in its row, or, with ``position_ids`` (integers
     that broadcast to the shape of ``ids``), what stands there -- documents packed into one row start again at 0.
-    Positions outside ``wpe`` add nothing.  The sum is in fp32, rounded once.  The gradients of both tables are summed
+    Positions outside ``wpe`` add nothing.  With ``strict_positions`` they are indices of the table as elsewhere: negative
+    ones count from its end, and ones outside it are an error, an ``IndexError`` here where ``position_ids`` are on the host,
+    else a status that :func:`~mist_b200.ops.native.check_status` raises (and they add nothing).  The sum is in fp32, rounded once.  The gradients of both tables are summed
     over tokens sorted by row, in fp32 and always in the same order; the one of ``wte`` goes straight into its gradient
     bucket where it has one."""
     if _sym(ids):
         return _rules().embedding(ids, wte, wpe, vocab_start)
     if _elsewhere(wte):
         with torch.cuda.device(wte.device):
-            return embedding(ids, wte, wpe, vocab_start, scale, position_ids)
+            return embedding(ids, wte, wpe, vocab_start, scale, position_ids, strict_positions)
     if ids.dim() != 2 or ids.is_floating_point():
         raise ValueError(f"ids: [batch, seq] integers expected, got {tuple(ids.shape)} of {ids.dtype}")
     if wpe is not None and position_ids is None and ids.shape[1] > wpe.shape[0]:
         raise ValueError(f"{ids.shape[1]} positions, but the table has {wpe.shape[0]}")
-    pos = _flat_positions(position_ids, ids) if wpe is not None else None
+    pos = _flat_positions(position_ids, ids, wpe.shape[0], strict_positions) if wpe is not None else None
     if use_native(wte):
         for name, t in (("wte", wte),) if wpe is None else (("wte", wte), ("wpe", wpe)):
             if (t.dtype != torch.bfloat16 or not t.is_contiguous() or t.shape[1] != wte.shape[1]
                     or t.shape[1] % 8 or t.device != ids.device):
                 raise ValueError(f"{name}: contiguous bf16 rows of a multiple of 8 values on the device of the ids expected")
         ids = ids.long().contiguous()
-    return _EmbeddingFn.apply(ids, wte, wpe, int(vocab_start), float(scale), pos)
+    return _EmbeddingFn.apply(ids, wte, wpe, int(vocab_start), float(scale), pos, int(strict_positions))
 
 
 # --------------------------------------------------------------------- optimizer / casts

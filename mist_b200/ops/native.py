@@ -55,9 +55,9 @@ _SIGNATURES = {
     "mb_bias_dropout_add": ([_p, _p, _p, _p, _z, _i, _f, _u64, _p], _i),
     "mb_dropout_bwd": ([_p, _p, _z, _f, _u64, _p], _i),
     "mb_rope": ([_p, _p, _p, _z, _i, _i, _i, _i, _i, _i, _i, _p], _i),
-    "mb_embed_fwd": ([_p, _p, _p, _p, _p, _i, _i, _i, _l, _i, _i, _f, _p], _i),
+    "mb_embed_fwd": ([_p, _p, _p, _p, _p, _i, _i, _i, _l, _i, _i, _i, _f, _p], _i),
     "mb_embed_bwd_workspace": ([_i, _i, _i], _z),
-    "mb_embed_bwd": ([_p, _p, _p, _p, _p, _i, _i, _i, _l, _i, _i, _f, _i, _i, _p, _p], _i),
+    "mb_embed_bwd": ([_p, _p, _p, _p, _p, _i, _i, _i, _l, _i, _i, _i, _f, _i, _i, _p, _p], _i),
     "mb_colsum": ([_p, _p, _p, _i, _i, _i, _i, _p], _i),
     "mb_cast_f32_to_bf16": ([_p, _p, _z, _f, _p], _i),
     "mb_axpy_bf16_to_f32": ([_p, _p, _z, _f, _i, _p], _i),
@@ -169,11 +169,12 @@ def call(name: str, *args):
 
 
 _STATUS_NAMES = {1: "TMA stage wait timed out", 2: "free-stage wait timed out",
-                 3: "accumulator wait timed out", 4: "peer flag wait timed out", 5: "bad argument"}
+                 3: "accumulator wait timed out", 4: "peer flag wait timed out", 5: "bad argument",
+                 6: "a position outside the table of positions"}
 
 
 def read_and_clear_status() -> int:
-    """The device status word set by bounded waits that gave up (0 = none); clears it."""
+    """The device status word set by bounded waits that gave up, and by strict lookups (0 = none); clears it."""
     lib = kernels()
     return 0 if lib is None else int(lib.mb_status_read_and_clear())
 
@@ -183,7 +184,8 @@ def status_message(code: int) -> str:
 
 
 def check_status():
-    """Reads (and clears) the device status word and raises if a bounded wait gave up."""
+    """Reads (and clears) the device status word and raises if a bounded wait gave up, or a strict lookup met a position
+    outside its table."""
     code = read_and_clear_status()
     if code != 0:
         raise RuntimeError(status_message(code))

@@ -1,0 +1,36 @@
+"""Positions that a model's table does not have are refused, as indexing the table refuses them."""
+import pytest
+import torch
+
+from mist_b200.modules.layers import VocabParallelEmbedding
+from mist_b200.ops import functional as F
+
+
+def _module():
+    torch.manual_seed(1)
+    return VocabParallelEmbedding(11, 8, max_position_embeddings=7)
+
+
+@pytest.mark.parametrize("bad", [7, -8, 2 ** 40])
+def test_explicit_positions_outside_the_table(bad):
+    m, ids = _module(), torch.zeros(2, 3, dtype=torch.long)
+    with pytest.raises(IndexError):
+        m(ids, position_ids=torch.tensor([[0, 1, bad]]))
+    with pytest.raises(IndexError):
+        F.embedding(ids, m.word_embeddings.weight, m.position_embeddings.weight,
+                    position_ids=torch.tensor([[0, 1, bad]]), strict_positions=True)
+
+
+def test_negative_positions_count_from_the_end():
+    m, ids = _module(), torch.tensor([[1, 2, 3], [4, 5, 6]])
+    pos = torch.tensor([[-1, 0, -7], [6, -2, 3]])
+    out, want = m(ids, position_ids=pos), m.word_embeddings.weight[ids] + m.position_embeddings.weight[pos]
+    assert torch.allclose(out, want, atol=1e-6)
+    g = torch.randn_like(out)
+    leaves = (m.word_embeddings.weight, m.position_embeddings.weight)
+    for a, b in zip(torch.autograd.grad(out, leaves, g), torch.autograd.grad(want, leaves, g)):
+        assert torch.allclose(a, b, atol=1e-6)
+
+
+def test_no_tokens():
+    assert _module()(torch.zeros(2, 0, dtype=torch.long), position_ids=torch.zeros(2, 0, dtype=torch.long)).shape == (2, 0, 8)
