@@ -114,7 +114,18 @@ packed_plan_kernel(const int* cu_q, const int* cu_k, int n, int total_q, int tot
   });
 }
 
+// Reports sequences of more than `most` rows, as the plan has them.
+__global__ void __launch_bounds__(256)
+packed_limit_kernel(const int* cu, int n, int total, int most, int* status) {
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b >= n) return;
+  const int first = b ? max(0, min(cu[b], total)) : 0, end = min(cu[b + 1], total);
+  if (end - first > most) atomicCAS(status, 0, MB_ERR_POSITION);
+}
+
 }  // namespace
+
+MB_API int* mb_status_device_ptr();
 
 // Bytes of a plan for n sequences in tensors of total_q and total_k rows.
 MB_API long mb_packed_plan_bytes(int n, int total_q, int total_k) {
@@ -130,5 +141,14 @@ MB_API int mb_packed_plan(const int* cu_q, const int* cu_k, int n, int total_q, 
   if (n < 0 || total_q < 0 || total_k < 0 || (reinterpret_cast<uintptr_t>(plan) & 15)) return -1;
   packed_plan_kernel<<<4 + (total_q + kThreads - 1) / kThreads, kThreads, 0, stream>>>(
       cu_q, cu_k, n, total_q, total_k, static_cast<uint8_t*>(plan));
+  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+}
+
+// cu: n + 1 offsets in device memory.  A sequence of more than `most` of the `total` rows sets the status word.
+MB_API int mb_packed_limit(const int* cu, int n, int total, int most, cudaStream_t stream) {
+  int* status = mb_status_device_ptr();
+  if (n < 0 || total < 0 || most < 0 || !status) return -1;
+  if (n == 0) return 0;
+  packed_limit_kernel<<<(n + 255) / 256, 256, 0, stream>>>(cu, n, total, most, status);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }

@@ -98,7 +98,9 @@ class TransformerLanguageModel(nn.Module):
         token) of the encoder / decoder tokens; ``enc_dec_attn_mask``: mask of the encoder tokens as
         cross attention sees them (defaults to ``enc_attn_mask``).  Masks without padding are dropped.
         A single-stack model takes a :class:`~mist_b200.ops.packed.PackedSequences` of its ``batch * seq`` tokens as
-        ``enc_attn_mask``: documents packed back to back, which attend inside themselves and whose positions start at 0."""
+        ``enc_attn_mask``: documents packed back to back, which attend inside themselves and whose positions start at 0.
+        Documents longer than a learned position table are refused (where the offsets are on the GPU, by a status that
+        :func:`~mist_b200.ops.native.check_status` raises)."""
         bs = enc_input_ids.shape[0] if enc_input_ids is not None else None
         if enc_hidden_states is None and self.encoder is None and self.enc_hidden_input is not None:
             enc_hidden_states = self.enc_hidden_input
@@ -109,7 +111,7 @@ class TransformerLanguageModel(nn.Module):
             if self.decoder is not None or isinstance(dec_mask, F.PackedSequences):
                 raise NotImplementedError("packed sequences in an encoder-decoder model")
             if enc_position_ids is None and enc_input_ids is not None:
-                enc_position_ids = enc_mask.positions.view(enc_input_ids.shape)
+                enc_position_ids = enc_mask
         if self.pre_process and self.encoder is not None:
             hidden = self.embedding(enc_input_ids, enc_position_ids, tokentype_ids)
         else:

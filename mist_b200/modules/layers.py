@@ -207,11 +207,20 @@ class VocabParallelEmbedding(nn.Module):
                 nn.init.normal_(emb.weight, mean=0.0, std=std)
 
     def forward(self, input_ids, position_ids=None, tokentype_ids=None):
+        """``position_ids``: integers that broadcast to the shape of ``input_ids``, or the
+        :class:`~mist_b200.ops.packed.PackedSequences` that its tokens are made of."""
         ws = group_size(self.process_group)
         wpe = self.position_embeddings.weight if self.position_embeddings is not None else None
         use_pos = wpe is not None and (ws == 1 or group_rank(self.process_group) == 0)
+        strict = not isinstance(position_ids, F.PackedSequences)
+        if not strict:
+            if wpe is not None:
+                position_ids.limit_lengths(wpe.shape[0])      # rows behind the last document may go on beyond the table
+            position_ids = position_ids.positions.view(input_ids.shape)
+        elif wpe is not None and not use_pos:
+            F.check_positions(position_ids, wpe.shape[0])     # every rank refuses what the first one refuses
         x = F.embedding(input_ids, self.word_embeddings.weight, wpe if use_pos else None, self.vocab_start,
-                        position_ids=position_ids, strict_positions=True)
+                        position_ids=position_ids, strict_positions=strict)
         if tokentype_ids is not None and self.tokentype_embeddings is not None:
             tt = self.tokentype_embeddings(tokentype_ids)
             x = x + (tt if ws == 1 or group_rank(self.process_group) == 0 else 0)

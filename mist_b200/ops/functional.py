@@ -1130,19 +1130,26 @@ def _elsewhere(t) -> bool:
     return t.is_cuda and t.get_device() != torch._C._cuda_getDevice()
 
 
-def _flat_positions(position_ids, ids, rows: int, strict: bool):
-    """Explicit positions in the shape of ``ids`` on their device, or ``None``.  ``strict``: those on the host are looked over
-    as indices of a table of ``rows`` rows."""
-    if position_ids is None:
-        return None
-    if position_ids.is_floating_point() or (position_ids.device != ids.device and position_ids.device.type != "cpu"):
-        raise ValueError("position_ids: integers on the device of the ids, or on the host, expected")
-    if strict and position_ids.device.type == "cpu" and position_ids.numel():
+def check_positions(position_ids, rows: int):
+    """Positions on the host as indices of a table of ``rows`` rows: those outside raise, negative ones become what they
+    count to from the end.  ``None`` and positions on a GPU are returned as they are."""
+    if position_ids is not None and position_ids.device.type == "cpu" and position_ids.numel():
         low, high = (int(x) for x in position_ids.aminmax())
         if low < -rows or high >= rows:
             raise IndexError(f"positions from {low} to {high}, but the table has {rows}")
         if low < 0:
             position_ids = torch.where(position_ids < 0, position_ids + rows, position_ids)
+    return position_ids
+
+
+def _flat_positions(position_ids, ids, rows: int, strict: bool):
+    """Explicit positions in the shape of ``ids`` on their device, or ``None``."""
+    if position_ids is None:
+        return None
+    if position_ids.is_floating_point() or (position_ids.device != ids.device and position_ids.device.type != "cpu"):
+        raise ValueError("position_ids: integers on the device of the ids, or on the host, expected")
+    if strict:
+        position_ids = check_positions(position_ids, rows)
     if position_ids.shape != ids.shape:
         position_ids = position_ids.expand(ids.shape)
     if position_ids.device != ids.device:

@@ -99,6 +99,20 @@ class PackedSequences:
                 self._positions = rows - self.cu_q.long()[torch.searchsorted(self.cu_q, rows, right=True) - 1]
         return self._positions
 
+    def limit_lengths(self, most: int):
+        """Refuses sequences of queries longer than ``most``: here where the offsets are known on the host, else by a status
+        that :func:`~mist_b200.ops.native.check_status` raises.  Rows behind the last sequence do not count."""
+        host = self.host_q
+        if host is None and self.plan is None:
+            host = self.cu_q.tolist()
+        if host is not None:
+            longest = max((b - a for a, b in zip(host, host[1:])), default=0)
+            if longest > most:
+                raise ValueError(f"a sequence of {longest} tokens, but the table of positions has {most}")
+        else:
+            with torch.cuda.device(self.device):
+                call("mb_packed_limit", ptr(self.cu_q), self.n, self.total_q, most, stream())
+
     @staticmethod
     def _total(total, host):
         if total is None:

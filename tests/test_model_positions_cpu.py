@@ -34,3 +34,27 @@ def test_negative_positions_count_from_the_end():
 
 def test_no_tokens():
     assert _module()(torch.zeros(2, 0, dtype=torch.long), position_ids=torch.zeros(2, 0, dtype=torch.long)).shape == (2, 0, 8)
+
+
+def _gpt(**more):
+    from tests.test_packed_training_cpu import build
+    return build("gpt", **more)
+
+
+def test_documents_longer_than_the_table():
+    """A table of 32 rows: documents of 33 tokens are refused as rows of 33 are; rows behind the last document are not."""
+    model, ids = _gpt(), torch.randint(0, 250, (1, 52))
+    for offsets in ([0, 52], torch.tensor([0, 10, 43, 52])):
+        with pytest.raises(ValueError, match="32"):
+            model(ids, attention_mask=F.PackedSequences(offsets))
+    assert model(ids, attention_mask=F.PackedSequences([0, 32, 52])).shape[:2] == (1, 52)
+    packed, alone = model(ids, attention_mask=F.PackedSequences([0, 10], 52)), model(ids[:, :10])
+    assert torch.allclose(packed[:, :10], alone, atol=1e-5)
+    with pytest.raises(ValueError):
+        model(ids)
+
+
+def test_documents_of_any_length_without_a_table():
+    from tests.test_packed_training_cpu import build
+    ids = torch.randint(0, 250, (1, 52))
+    assert build("llama")(ids, attention_mask=F.PackedSequences([0, 52])).shape[:2] == (1, 52)

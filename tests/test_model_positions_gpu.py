@@ -58,3 +58,33 @@ def test_positions_on_the_host():
     with pytest.raises(IndexError):
         m(ids, position_ids=pos + 1)
     native.check_status()
+
+
+@pytest.mark.parametrize("lens,most", [([40], 40), ([41], 40), ([1] * 300 + [9], 8), ([8] * 300, 8), ([0, 0], 0), ([], 5)])
+def test_packed_documents_longer_than_a_table(lens, most):
+    """Offsets on the GPU: a status; rows behind the last sequence do not count."""
+    cu = [0] + torch.tensor(lens).cumsum(0).tolist() if lens else [0]
+    seqs = F.PackedSequences(torch.tensor(cu, device=DEV), cu[-1] + 100)
+    native.check_status()
+    seqs.limit_lengths(most)
+    assert (native.read_and_clear_status() != 0) == (max(lens, default=0) > most)
+    known = F.PackedSequences(cu, cu[-1] + 100, device=DEV)
+    if max(lens, default=0) > most:
+        with pytest.raises(ValueError):
+            known.limit_lengths(most)
+    else:
+        known.limit_lengths(most)
+    native.check_status()
+
+
+def test_a_module_takes_a_packing_as_positions():
+    m = _module()
+    ids = torch.randint(0, 50, (2, 60), device=DEV)
+    for cu, reported in (([0, 40, 80], False), ([0, 41, 80], True)):
+        seqs = F.PackedSequences(torch.tensor(cu, device=DEV), 120)
+        out = m(ids, position_ids=seqs)
+        assert (native.read_and_clear_status() != 0) == reported
+        at = torch.cat([torch.arange(cu[1]), torch.arange(80 - cu[1]), torch.arange(40)]).view(2, 60)
+        pos = m.position_embeddings.weight[at.clamp(max=39)].float() * (at < 40).to(DEV)[..., None]
+        want = m.word_embeddings.weight[ids].float() + pos
+        assert ((out.float() - want).abs() <= 1.01 * 2 ** -8 * want.abs() + 1e-6).all()
