@@ -22,7 +22,7 @@ import torch
 import torch.distributed as dist
 import torch.nn as nn
 
-from .modules.layers import ParallelMHA
+from .modules.layers import ParallelMHA, VocabParallelEmbedding
 
 
 class InferenceParams:
@@ -59,6 +59,13 @@ def kv_cache(model: nn.Module, max_batch_size: int, max_seqlen: int):
             m.inference_params = None
 
 
+def _position_rows(model: nn.Module) -> Optional[int]:
+    """Rows of the model's learned position table, ``None`` without one."""
+    tables = [m.position_embeddings for m in model.modules()
+              if isinstance(m, VocabParallelEmbedding) and m.position_embeddings is not None]
+    return min((t.num_embeddings for t in tables), default=None)
+
+
 @torch.no_grad()
 def generate(model: nn.Module, input_ids: torch.Tensor, max_new_tokens: int, eos_token_id: Optional[int] = None,
              temperature: float = 0.0, top_k: int = 0, generator: Optional[torch.Generator] = None,
@@ -68,7 +75,9 @@ def generate(model: nn.Module, input_ids: torch.Tensor, max_new_tokens: int, eos
     Returns ``[batch, prompt + generated]``; sequences that hit ``eos_token_id`` keep emitting it.
     With a tensor-parallel model pass its group as ``tp_group``: the vocabulary-parallel logits of
     the last position are gathered so every rank picks the same token (sampling then needs the
-    same ``generator`` state on every rank)."""
+    same ``generator`` state on every rank).  A model with learned positions raises an ``IndexError`` at the first token
+    behind the last row of its table."""
+    rows = _position_rows(model)
     was_training = model.training
     model.eval()
     b, s0 = input_ids.shape
@@ -79,6 +88,8 @@ def generate(model: nn.Module, input_ids: torch.Tensor, max_new_tokens: int, eos
         with kv_cache(model, b, total) as ip:
             step_ids = input_ids
             for _ in range(max_new_tokens):
+                if rows is not None and ip.seqlen_offset + step_ids.shape[1] > rows:
+                    raise IndexError(f"position {ip.seqlen_offset + step_ids.shape[1] - 1} is out of bounds: the table has {rows} rows")
                 pos = torch.arange(ip.seqlen_offset, ip.seqlen_offset + step_ids.shape[1], device=input_ids.device)
                 logits = model(step_ids, position_ids=pos.unsqueeze(0).expand(b, -1))
                 ip.seqlen_offset += step_ids.shape[1]

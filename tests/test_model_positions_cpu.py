@@ -58,3 +58,16 @@ def test_documents_of_any_length_without_a_table():
     from tests.test_packed_training_cpu import build
     ids = torch.randint(0, 250, (1, 52))
     assert build("llama")(ids, attention_mask=F.PackedSequences([0, 52])).shape[:2] == (1, 52)
+
+
+def test_generation_behind_the_table():
+    """32 rows: a prompt of 30 leaves room for three tokens (the last one is not fed back); an end before it is no error."""
+    from mist_b200.inference import generate
+    model, ids = _gpt(), torch.randint(0, 250, (1, 30), generator=torch.Generator().manual_seed(3))
+    out = generate(model, ids, 3)
+    assert out.shape == (1, 33)
+    with pytest.raises(IndexError):
+        generate(model, ids, 6)
+    with pytest.raises(IndexError):
+        generate(model, torch.cat([ids, ids], 1), 1)
+    assert generate(model, ids, 6, eos_token_id=int(out[0, 32])).shape[1] <= 33

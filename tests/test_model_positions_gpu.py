@@ -88,3 +88,14 @@ def test_a_module_takes_a_packing_as_positions():
         pos = m.position_embeddings.weight[at.clamp(max=39)].float() * (at < 40).to(DEV)[..., None]
         want = m.word_embeddings.weight[ids].float() + pos
         assert ((out.float() - want).abs() <= 1.01 * 2 ** -8 * want.abs() + 1e-6).all()
+
+
+def test_generation_behind_the_table():
+    from mist_b200.inference import generate
+    from tests.test_packed_training_cpu import build
+    model = build("gpt", device=DEV, dtype=torch.bfloat16, params_dtype="bfloat16", hidden_size=256, intermediate_size=512)
+    ids = torch.randint(0, 250, (1, 30), device=DEV)
+    assert generate(model, ids, 3).shape == (1, 33)
+    with pytest.raises(IndexError):
+        generate(model, ids, 6)
+    native.check_status()
