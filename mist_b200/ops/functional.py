@@ -871,10 +871,11 @@ def attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k=None, scale: Optional[f
     """Attention over sequences packed back to back without padding: q ``[total_q, nh, d]``, k / v
     ``[total_k, nh_kv, d]``, ``cu_seqlens_*`` the ``batch + 1`` cumulative lengths (a tensor or a list), or a
     :class:`PackedSequences` in the place of ``cu_seqlens_q``.  One launch covers all sequences, in the forward pass and
-    in the backward pass; offsets on the device are not read back.  A causal query sees the keys up to its own place, the
-    sequences aligned at their ends.  Queries without a key, and rows behind the last sequence, give zeros.
-    Returns ``[total_q, nh, d]``, or where the offsets are known on the host as many rows as they say (all, of zeros, where they say
-    none) (the interface of the
+    in the backward pass.  A causal query sees the keys up to its own place, the
+    sequences aligned at their ends.  Queries without a key give zeros.
+    Returns as many rows as the offsets say (all, of zeros, where they say none); offsets on the GPU are read back for that, once,
+    behind the launches, and refused if they do not begin with 0 or fall.  With a :class:`PackedSequences`, and while a graph is
+    captured, nothing is read back: all ``total_q`` rows are returned, zeros behind the last sequence (the interface of the
     reference's ``flash_attn_varlen`` entry points, csrc/flash_attn/flash_api.cpp ``varlen_fwd`` / ``varlen_bwd``)."""
     if _elsewhere(q):
         with torch.cuda.device(q.device):
@@ -885,6 +886,7 @@ def attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k=None, scale: Optional[f
         return packed_attention.attention(q, k, v, cu_seqlens_q, scale, causal)
     seqs = PackedSequences(cu_seqlens_q, q.shape[0], cu_seqlens_k, k.shape[0], device=q.device)
     out = packed_attention.attention(q, k, v, seqs, scale, causal)
+    seqs.read_back()
     rows = seqs.host_q[-1] if seqs.host_q is not None else 0
     return out if rows in (0, q.shape[0]) else out[:rows]
 

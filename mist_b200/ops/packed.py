@@ -44,9 +44,13 @@ def _offsets(cu, device):
                 cu = cu.to(device=device, dtype=torch.int32).contiguous()
             return cu, None
     host = [int(x) for x in (cu.tolist() if isinstance(cu, torch.Tensor) else cu)]
+    _check_offsets(host)
+    return torch.tensor(host, dtype=torch.int32, device=device), host
+
+
+def _check_offsets(host):
     if not host or host[0] != 0 or any(b < a for a, b in zip(host, host[1:])):
         raise ValueError("offsets: they begin with 0 and do not fall")
-    return torch.tensor(host, dtype=torch.int32, device=device), host
 
 
 class PackedSequences:
@@ -112,6 +116,18 @@ class PackedSequences:
         else:
             with torch.cuda.device(self.device):
                 call("mb_packed_limit", ptr(self.cu_q), self.n, self.total_q, most, stream())
+
+    def read_back(self):
+        """Offsets on the GPU come to the host, where they are checked; waits for the current stream.  Not while a graph is
+        captured."""
+        if (self.host_q is not None and self.host_k is not None) or torch.cuda.is_current_stream_capturing():
+            return
+        host_q = self.cu_q.tolist() if self.host_q is None else self.host_q
+        host_k = host_q if self.same else (self.cu_k.tolist() if self.host_k is None else self.host_k)
+        for host, total in ((host_q, self.total_q), (host_k, self.total_k)):
+            _check_offsets(host)
+            self._total(total, host)
+        self.host_q, self.host_k = host_q, host_k
 
     @staticmethod
     def _total(total, host):

@@ -1,0 +1,57 @@
+"""Offsets of packed attention, on the host and on the GPU: the same rows, the same refusals."""
+import pytest
+import torch
+
+from mist_b200.ops import functional as F
+from mist_b200.ops import native
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _tensors(rows, heads=2, d=64, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return [torch.randn(rows, heads, d, device=DEV, generator=g).bfloat16().requires_grad_(True) for _ in range(3)]
+
+
+@pytest.mark.parametrize("cu,rows", [([0, 30, 70], 70), ([0, 30, 70], 100), ([0, 1], 100), ([0, 0], 100), ([0], 100)])
+def test_rows_do_not_depend_on_where_the_offsets_are(cu, rows):
+    t = _tensors(rows)
+    outs = [F.attention_varlen(*t, c) for c in (cu, torch.tensor(cu), torch.tensor(cu, device=DEV),
+                                                torch.tensor(cu, device=DEV, dtype=torch.int32))]
+    assert outs[0].shape[0] == (cu[-1] or rows)
+    grads = [torch.autograd.grad(o, t, torch.ones_like(o)) for o in outs]
+    for o, g in zip(outs[1:], grads[1:]):
+        assert torch.equal(o, outs[0]) and all(torch.equal(a, b) for a, b in zip(g, grads[0]))
+    other = F.attention_varlen(*t, torch.tensor(cu, device=DEV), cu, causal=False)
+    assert torch.equal(other, F.attention_varlen(*t, cu, torch.tensor(cu, device=DEV), causal=False))
+    assert other.shape[0] == (cu[-1] or rows)
+    native.check_status()
+
+
+@pytest.mark.parametrize("cu", [[1, 70], [0, 50, 20, 70], [0, 71], [-5, 70]])
+def test_impossible_offsets_on_the_gpu_are_refused(cu):
+    """The kernels clamp them (which keeps them inside the tensors); the call raises."""
+    t = _tensors(70)
+    ends = [0] * (len(cu) - 1) + [70]
+    for bad, keys in ((torch.tensor(cu, device=DEV), None), (torch.tensor(cu, device=DEV), ends), (ends, torch.tensor(cu, device=DEV))):
+        with pytest.raises(ValueError):
+            F.attention_varlen(*t, bad, keys)
+    native.check_status()
+
+
+def test_a_captured_call_reads_nothing_back():
+    t, cu = _tensors(100), torch.tensor([0, 30, 70], device=DEV, dtype=torch.int32)
+    with torch.no_grad():
+        want = F.attention_varlen(*t, cu)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            F.attention_varlen(*t, cu)
+        torch.cuda.current_stream().wait_stream(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = F.attention_varlen(*t, cu)
+        graph.replay()
+    torch.cuda.synchronize()
+    assert out.shape[0] == 100 and torch.equal(out[:70], want) and not out[70:].any()
