@@ -883,6 +883,8 @@ def attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k=None, scale: Optional[f
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     if isinstance(cu_seqlens_q, PackedSequences):
+        if cu_seqlens_k is not None:
+            raise ValueError("a PackedSequences holds the offsets of the keys: none can be given beside it")
         return packed_attention.attention(q, k, v, cu_seqlens_q, scale, causal)
     seqs = PackedSequences(cu_seqlens_q, q.shape[0], cu_seqlens_k, k.shape[0], device=q.device)
     out = packed_attention.attention(q, k, v, seqs, scale, causal)
