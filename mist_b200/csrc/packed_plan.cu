@@ -2,6 +2,7 @@
 // have to be read back to the host.  A step builds them once and every layer's attention walks them.
 #include "common.cuh"
 #include "packed_plan.cuh"
+#include <string.h>
 
 namespace {
 
@@ -114,6 +115,16 @@ packed_plan_kernel(const int* cu_q, const int* cu_k, int n, int total_q, int tot
   });
 }
 
+// Offsets that the host knows, as many as the arguments of a launch take.
+constexpr int kOffsets = 992;
+struct Offsets {
+  int at[kOffsets];
+};
+__global__ void __launch_bounds__(256)
+packed_offsets_kernel(const __grid_constant__ Offsets offsets, int n, int* out) {
+  for (int i = threadIdx.x; i < n; i += 256) out[i] = offsets.at[i];
+}
+
 // Reports sequences of more than `most` rows, as the plan has them.
 __global__ void __launch_bounds__(256)
 packed_limit_kernel(const int* cu, int n, int total, int most, int* status) {
@@ -141,6 +152,18 @@ MB_API int mb_packed_plan(const int* cu_q, const int* cu_k, int n, int total_q, 
   if (n < 0 || total_q < 0 || total_k < 0 || (reinterpret_cast<uintptr_t>(plan) & 15)) return -1;
   packed_plan_kernel<<<4 + (total_q + kThreads - 1) / kThreads, kThreads, 0, stream>>>(
       cu_q, cu_k, n, total_q, total_k, static_cast<uint8_t*>(plan));
+  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+}
+
+// n offsets in host memory to device memory.
+MB_API int mb_packed_offsets(const int* host, int n, int* out, cudaStream_t stream) {
+  if (n < 0) return -1;
+  for (int first = 0; first < n; first += kOffsets) {
+    Offsets part;
+    const int count = n - first < kOffsets ? n - first : kOffsets;
+    memcpy(part.at, host + first, sizeof(int) * count);
+    packed_offsets_kernel<<<1, 256, 0, stream>>>(part, count, out + first);
+  }
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 

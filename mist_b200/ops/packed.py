@@ -6,6 +6,7 @@ nothing is read back to the host (reference: csrc/flash_attn/flash_api.cpp:427, 
 with offsets that mist/modules/mha.py:1233-1243 derives from a padding mask)."""
 from __future__ import annotations
 
+import ctypes
 import functools
 from typing import Optional
 
@@ -13,6 +14,9 @@ import torch
 
 from . import native
 from .native import call, ptr, stream, use_native
+
+
+INT32_MAX = 2 ** 31 - 1
 
 
 # what the library says of sizes alone
@@ -45,7 +49,15 @@ def _offsets(cu, device):
             return cu, None
     host = [int(x) for x in (cu.tolist() if isinstance(cu, torch.Tensor) else cu)]
     _check_offsets(host)
-    return torch.tensor(host, dtype=torch.int32, device=device), host
+    if host[-1] > INT32_MAX:
+        raise ValueError(f"offsets up to {host[-1]}: 32 bits hold them")
+    if device.type != "cuda":
+        return torch.tensor(host, dtype=torch.int32, device=device), host
+    # by the arguments of a kernel: nothing waits, and a graph that is captured holds them
+    out = torch.empty(len(host), dtype=torch.int32, device=device)
+    with torch.cuda.device(device):
+        call("mb_packed_offsets", (ctypes.c_int * len(host))(*host), len(host), ptr(out), stream())
+    return out, host
 
 
 def _check_offsets(host):

@@ -11,3 +11,8 @@ def test_offsets_of_keys_beside_a_packing():
     with pytest.raises(ValueError):
         F.attention_varlen(x, x, x, seqs, [0, 5, 7])
     F.attention_varlen(x, x, x, seqs)
+
+
+def test_offsets_that_32_bits_do_not_hold():
+    with pytest.raises(ValueError):
+        F.PackedSequences([0, 2 ** 31])

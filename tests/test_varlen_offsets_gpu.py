@@ -55,3 +55,33 @@ def test_a_captured_call_reads_nothing_back():
         graph.replay()
     torch.cuda.synchronize()
     assert out.shape[0] == 100 and torch.equal(out[:70], want) and not out[70:].any()
+
+
+@pytest.mark.parametrize("n", [1, 991, 992, 993, 2500])
+def test_offsets_of_the_host_reach_the_device(n):
+    cu = [3 * i for i in range(n)]
+    seqs = F.PackedSequences(cu, device=DEV)
+    assert seqs.cu_q.tolist() == cu and seqs.cu_q.dtype == torch.int32
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_offsets_of_the_host_in_a_captured_graph(causal):
+    """Nothing of the host's is read when the graph is replayed, and capturing waits for nothing."""
+    t, cu = _tensors(70), [0, 30, 70]
+    with torch.no_grad():
+        want = F.attention_varlen(*t, cu, causal=causal)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            F.attention_varlen(*t, cu, causal=causal)
+        torch.cuda.current_stream().wait_stream(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = F.attention_varlen(*t, torch.tensor(cu), causal=causal)
+            other = F.attention_varlen(*t, cu, [0, 10, 70], causal=causal)
+        del cu
+        for _ in range(2):
+            out.fill_(7.0)
+            graph.replay()
+        assert torch.equal(out, want)
+        assert torch.equal(other, F.attention_varlen(*t, [0, 30, 70], [0, 10, 70], causal=causal))
