@@ -1254,6 +1254,8 @@ def embedding(ids, wte, wpe=None, vocab_start: int = 0, scale: float = 1.0, posi
         raise ValueError(f"ids: [batch, seq] integers expected, got {tuple(ids.shape)} of {ids.dtype}")
     if wpe is not None and position_ids is None and ids.shape[1] > wpe.shape[0]:
         raise ValueError(f"{ids.shape[1]} positions, but the table has {wpe.shape[0]}")
+    if ids.is_cuda and max(ids.numel(), wte.shape[0]) > native.INT32_MAX:
+        raise ValueError(f"{ids.numel()} tokens and {wte.shape[0]} rows: the kernels count them in 32 bits")
     pos = _flat_positions(position_ids, ids, wpe.shape[0], strict_positions) if wpe is not None else None
     if use_native(wte):
         for name, t in (("wte", wte),) if wpe is None else (("wte", wte), ("wpe", wpe)):

@@ -16,7 +16,7 @@ import torch
 
 from . import functional as F
 from . import native
-from .native import call, ptr, stream, use_native
+from .native import INT32_MAX, call, ptr, stream, use_native
 
 # Hidden sizes from which a logit is kept and not computed again.  Both passes of 4096 tokens, vocabulary 50304 (kept, twice, us):
 # hidden 2048 2329, 2664; 1024 1448, 1552; 512 963, 978; 256 771, 717; vocabulary 8192: 1024 217, 232; 512 187, 174.
@@ -27,7 +27,7 @@ def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
     """``t`` as ``[rows, cols]`` that the kernels' copies can address: unit stride, rows on 16 bytes."""
     if t.dim() != 2:
         t = t.reshape(-1, cols)
-    if t.stride(1) != 1 or t.stride(0) % 8 or t.stride(0) < cols or ptr(t) % 16:
+    if t.stride(1) != 1 or t.stride(0) % 8 or not cols <= t.stride(0) <= INT32_MAX or ptr(t) % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -118,7 +118,7 @@ class _LinearXentFn(torch.autograd.Function):
         accumulate = bucket is not None and bool(getattr(ctx.param, "grad_accumulate", False))
         direct = bucket is not None and bucket.dtype in (torch.float32, weight.dtype) and bucket.stride(1) == 1
         if direct and use_native(x2):      # what the products' stores can address
-            direct = bucket.stride(0) % 8 == 0 and bucket.stride(0) >= k and ptr(bucket) % 16 == 0
+            direct = bucket.stride(0) % 8 == 0 and k <= bucket.stride(0) <= INT32_MAX and ptr(bucket) % 16 == 0
         dw = None
         if direct:
             dw = bucket
@@ -192,6 +192,8 @@ def linear_cross_entropy(x, weight, labels, bias=None, vocab_start: int = 0, gro
         if t is not None and t.device != x.device:
             raise ValueError("x, weight, labels and bias have to be on one device")
     if use_native(x):
+        if max(labels.numel(), *weight.shape) > INT32_MAX:
+            raise ValueError(f"{labels.numel()} rows, weight {tuple(weight.shape)}: the kernels count them in 32 bits")
         if any(t is not None and t.dtype != torch.bfloat16 for t in (x, weight, bias)) or x.shape[-1] % 8:
             raise ValueError("the kernels take bf16 of a hidden size that is a multiple of 8")
         if bias is not None and not bias.is_contiguous():

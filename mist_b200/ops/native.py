@@ -139,6 +139,10 @@ def runtime():
     return _RUNTIME
 
 
+# sizes that go to the library as C ints, whose higher bits ctypes would cut off
+INT32_MAX = 2 ** 31 - 1
+
+
 def use_native(*tensors) -> bool:
     """True when the op should run on the CUDA kernels (any tensor lives on a GPU)."""
     for t in tensors:

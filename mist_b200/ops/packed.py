@@ -13,10 +13,7 @@ from typing import Optional
 import torch
 
 from . import native
-from .native import call, ptr, stream, use_native
-
-
-INT32_MAX = 2 ** 31 - 1
+from .native import INT32_MAX, call, ptr, stream, use_native
 
 
 # what the library says of sizes alone
@@ -149,6 +146,8 @@ class PackedSequences:
             total = host[-1]
         if total < 0 or (host is not None and host[-1] > total):
             raise ValueError(f"{total} rows, but the offsets end at {host and host[-1]}")
+        if total > INT32_MAX:
+            raise ValueError(f"{total} rows: 32 bits hold their number")
         return int(total)
 
     def check(self, q, k):
