@@ -12,7 +12,7 @@ import torch.nn as nn
 
 from ..config import ModelConfig, PositionEmbeddingType
 from ..modules.layers import (ColumnParallelLinear, PaddingMask, VocabParallelEmbedding,
-                              linear_vocab_parallel_cross_entropy, vocab_parallel_cross_entropy)
+                              is_plain_projection, linear_vocab_parallel_cross_entropy, vocab_parallel_cross_entropy)
 from ..ops import functional as F
 from ..parallel import dist_ops
 from .transformer import ParallelTransformer
@@ -170,7 +170,8 @@ class TransformerLanguageModel(nn.Module):
 
 class LMHead(nn.Module):
     """Vocabulary projection (column parallel, no bias) + vocab-parallel cross entropy; with ``fused_lm_loss`` the two are
-    one operator where labels are given."""
+    one operator where labels are given.  A projection that is hooked, replaced or has a bias is called, and the loss taken from
+    its logits."""
 
     def __init__(self, cfg: ModelConfig, process_group=None, sequence_parallel=False, device=None, dtype=None):
         super().__init__()
@@ -181,7 +182,8 @@ class LMHead(nn.Module):
                                          dtype=dtype or cfg.params_dtype)
 
     def forward(self, hidden, labels=None, weight=None):
-        fused = self.fused_loss and labels is not None and not F._sym(hidden)
+        fused = (self.fused_loss and labels is not None and not F._sym(hidden)
+                 and (weight is not None or is_plain_projection(self.proj)))
         if weight is not None or fused:   # tied embeddings
             x = hidden
             if self.proj.sequence_parallel:

@@ -135,6 +135,15 @@ class ColumnParallelLinear(FusedDense):
         return F.linear(x, self.weight, self.bias, activation=self.activation, residual=residual)
 
 
+def is_plain_projection(m) -> bool:
+    """Whether calling ``m`` is nothing but the product with its weight: a :class:`ColumnParallelLinear` as it was built, with
+    no hooks of any kind on it."""
+    return (type(m) is ColumnParallelLinear and "forward" not in m.__dict__ and m.bias is None and m.activation is None
+            and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
+                     or nn_module._global_forward_hooks or nn_module._global_forward_pre_hooks
+                     or nn_module._global_backward_hooks or nn_module._global_backward_pre_hooks))
+
+
 class RowParallelLinear(FusedDense):
     """Input features split over the group; the partial outputs are summed by an
     all-reduce, or by a reduce-scatter over tokens under sequence parallelism.  The bias
