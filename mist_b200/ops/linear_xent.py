@@ -40,9 +40,15 @@ def piece_columns(rows: int, vocab: int) -> int:
     return min(vocab, -(-(-(-vocab // pieces)) // 256) * 256)
 
 
+def kept_bytes(rows: int, vocab: int) -> int:
+    """Bytes that live from the forward to the backward pass where logits are kept: of each row 16 bits per logit, a maximum
+    and a sum per 128 columns, the label's logit, the loss and the log-sum-exp."""
+    return rows * (2 * (-(-vocab // 8) * 8) + 16 * -(-vocab // 256) + 12)
+
+
 def keeps_logits(rows: int, vocab: int, k: int) -> bool:
     """Whether the forward pass keeps 16 bits of every logit for the backward pass instead of computing the logits twice."""
-    return k >= KEEP_FROM and rows <= 2 ** 20 and 2 * rows * (-(-vocab // 8) * 8) <= F.Settings.xent_keep_bytes
+    return k >= KEEP_FROM and rows <= 2 ** 20 and kept_bytes(rows, vocab) <= F.Settings.xent_keep_bytes
 
 
 @functools.lru_cache(maxsize=1024)
