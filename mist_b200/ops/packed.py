@@ -90,7 +90,8 @@ class PackedSequences:
         self._rotary = {}
         self._positions = self.plan = None
         if use_native(self.cu_q):
-            self.plan = torch.empty(_plan_bytes(self.n, self.total_q, self.total_k), dtype=torch.uint8, device=device)
+            with torch.inference_mode(False):      # autograd keeps none that were made under inference mode
+                self.plan = torch.empty(_plan_bytes(self.n, self.total_q, self.total_k), dtype=torch.uint8, device=device)
             if device.index == torch._C._cuda_getDevice():
                 self._make_plan()
             else:
@@ -104,12 +105,13 @@ class PackedSequences:
     def positions(self):
         """Every query row's place in its sequence, int64 ``[total]``."""
         if self._positions is None:
-            if self.plan is not None:
-                at = native.kernels().mb_packed_plan_positions(self.n, self.total_q, self.total_k)
-                self._positions = self.plan[at:at + 8 * self.total_q].view(torch.int64)
-            else:
-                rows = torch.arange(self.total_q)
-                self._positions = rows - self.cu_q.long()[torch.searchsorted(self.cu_q, rows, right=True) - 1]
+            with torch.inference_mode(False):
+                if self.plan is not None:
+                    at = native.kernels().mb_packed_plan_positions(self.n, self.total_q, self.total_k)
+                    self._positions = self.plan[at:at + 8 * self.total_q].view(torch.int64)
+                else:
+                    rows = torch.arange(self.total_q)
+                    self._positions = rows - self.cu_q.long()[torch.searchsorted(self.cu_q, rows, right=True) - 1]
         return self._positions
 
     def limit_lengths(self, most: int):
@@ -163,9 +165,10 @@ class PackedSequences:
         tables = self._rotary.get(key)
         if tables is None:
             # the angles of functional.rope_tables; what it keeps is by length, and packings come in every length
-            inv = 1.0 / (base ** (torch.arange(0, rot_dim, 2, dtype=torch.float32, device=self.device) / rot_dim))
-            angles = torch.outer(self.positions.float(), inv)
-            tables = (angles.cos(), angles.sin(), rot_dim)
+            with torch.inference_mode(False):
+                inv = 1.0 / (base ** (torch.arange(0, rot_dim, 2, dtype=torch.float32, device=self.device) / rot_dim))
+                angles = torch.outer(self.positions.float(), inv)
+                tables = (angles.cos(), angles.sin(), rot_dim)
             # (tables that a graph being captured computes belong to it: outside it nobody has computed them)
             if self.plan is None or not torch.cuda.is_current_stream_capturing():
                 self._rotary[key] = tables
