@@ -62,14 +62,39 @@ def _check_offsets(host):
         raise ValueError("offsets: they begin with 0 and do not fall")
 
 
+class _Made:
+    """Tensors that were made on the stream that was current then.  Others wait for that once, where they first use them; the
+    allocator learns of them.  Tensors of a graph being captured belong to it: nobody outside waits for them."""
+
+    def __init__(self, device, *tensors):
+        self.index, self.tensors, self.event = device.index, tensors, None
+        self.seen = {torch._C._cuda_getCurrentRawStream(device.index)}
+        if not torch.cuda.is_current_stream_capturing():
+            self.event = torch.cuda.Event()
+            self.event.record(torch.cuda.current_stream(device))
+
+    def here(self):
+        now = torch._C._cuda_getCurrentRawStream(self.index)
+        # (an event of outside cannot be waited for under capture; a graph is replayed after its capture, which itself begins
+        # when the device is idle)
+        if now in self.seen or self.event is None or torch.cuda.is_current_stream_capturing():
+            return
+        current = torch.cuda.current_stream(self.index)
+        current.wait_event(self.event)
+        for t in self.tensors:
+            t.record_stream(current)
+        self.seen.add(now)
+
+
 class PackedSequences:
     """``n`` sequences packed back to back: ``cu_seqlens`` holds the ``n + 1`` offsets (0 first), as a tensor or a list.
 
     ``total``: rows of the packed tensors, at least the last offset; rows behind it belong to no sequence.  It may be left
     out where the offsets are known on the host.  ``cu_seqlens_k`` / ``total_k``: offsets of the keys, where they are others
     than those of the queries.  Offsets on the GPU are not read back and not checked: ones that fall or pass ``total`` are
-    clamped, which keeps every access inside the tensors, and what comes out is unspecified.  The object's tensors are made
-    on the stream that is current then."""
+    clamped, which keeps every access inside the tensors, and what comes out is unspecified.  The object may be used on any
+    stream: its tensors are made on one and waited for on others (under capture they have to be there, as after
+    ``torch.cuda.graph`` has begun)."""
 
     def __init__(self, cu_seqlens, total: Optional[int] = None, cu_seqlens_k=None, total_k: Optional[int] = None, device=None):
         if device is None and isinstance(cu_seqlens, torch.Tensor):
@@ -88,7 +113,7 @@ class PackedSequences:
         self.total_k = self.total_q if self.same and total_k is None else self._total(total_k, self.host_k)
         self.device = device
         self._rotary = {}
-        self._positions = self.plan = None
+        self._positions = self.plan = self._made = None
         if use_native(self.cu_q):
             with torch.inference_mode(False):      # autograd keeps none that were made under inference mode
                 self.plan = torch.empty(_plan_bytes(self.n, self.total_q, self.total_k), dtype=torch.uint8, device=device)
@@ -100,10 +125,17 @@ class PackedSequences:
 
     def _make_plan(self):
         call("mb_packed_plan", ptr(self.cu_q), ptr(self.cu_k), self.n, self.total_q, self.total_k, ptr(self.plan), stream())
+        self._made = _Made(self.device, self.cu_q, self.cu_k, self.plan)
+
+    def here(self):
+        """The plan and the offsets, for kernels of the current stream."""
+        if self._made is not None:
+            self._made.here()
 
     @property
     def positions(self):
         """Every query row's place in its sequence, int64 ``[total]``."""
+        self.here()
         if self._positions is None:
             with torch.inference_mode(False):
                 if self.plan is not None:
@@ -125,6 +157,7 @@ class PackedSequences:
             if longest > most:
                 raise ValueError(f"a sequence of {longest} tokens, but the table of positions has {most}")
         else:
+            self.here()
             with torch.cuda.device(self.device):
                 call("mb_packed_limit", ptr(self.cu_q), self.n, self.total_q, most, stream())
 
@@ -133,6 +166,7 @@ class PackedSequences:
         captured."""
         if (self.host_q is not None and self.host_k is not None) or torch.cuda.is_current_stream_capturing():
             return
+        self.here()
         host_q = self.cu_q.tolist() if self.host_q is None else self.host_q
         host_k = host_q if self.same else (self.cu_k.tolist() if self.host_k is None else self.host_k)
         for host, total in ((host_q, self.total_q), (host_k, self.total_k)):
@@ -157,12 +191,15 @@ class PackedSequences:
             raise ValueError(f"{q.shape[0]} query and {k.shape[0]} key rows, but the packing is of {self.total_q} and {self.total_k}")
         if q.device != self.device:
             raise ValueError(f"tensors on {q.device}, offsets on {self.device}")
+        self.here()
 
     def rotary(self, rot_dim: int, base: float):
-        """``(cos, sin, rot_dim)`` with a row for each packed token, that of its position; made on the stream of the first call
-        and kept, or made for the graph alone while one is captured."""
+        """``(cos, sin, rot_dim)`` with a row for each packed token, that of its position; made on the stream of the first call,
+        kept, and waited for on others, or made for the graph alone while one is captured."""
         key = (rot_dim, base)
-        tables = self._rotary.get(key)
+        tables, made = self._rotary.get(key, (None, None))
+        if made is not None:
+            made.here()
         if tables is None:
             # the angles of functional.rope_tables; what it keeps is by length, and packings come in every length
             with torch.inference_mode(False):
@@ -171,7 +208,7 @@ class PackedSequences:
                 tables = (angles.cos(), angles.sin(), rot_dim)
             # (tables that a graph being captured computes belong to it: outside it nobody has computed them)
             if self.plan is None or not torch.cuda.is_current_stream_capturing():
-                self._rotary[key] = tables
+                self._rotary[key] = tables, None if self.plan is None else _Made(self.device, *tables[:2])
         return tables
 
     def _each(self):
@@ -349,6 +386,7 @@ def projected_attention(qkv, kv_heads: int, packed: PackedSequences, scale: floa
         raise ValueError(f"{tuple(qkv.shape[:2])} tokens, but the packing is of {packed.total_q}")
     if qkv.device != packed.device:
         raise ValueError(f"tensors on {qkv.device}, offsets on {packed.device}")
+    packed.here()
     if rot:
         for t in (cos, sin):
             if t.shape != (packed.total_q, rot // 2) or t.dtype != torch.float32 or not t.is_contiguous() or t.device != qkv.device:
