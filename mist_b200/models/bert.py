@@ -80,6 +80,11 @@ class BertModel(nn.Module):
 
     def forward(self, input_ids, attention_mask=None, tokentype_ids=None, lm_labels=None, labels=None,
                 sentence_order=None):
+        """Logits of the tokens and of the sentence order, or with ``lm_labels`` the loss.  With a
+        :class:`~mist_b200.ops.packed.PackedSequences` as ``attention_mask`` nothing is pooled: the logits of the sentence
+        order are ``None``, and labels for them are refused."""
+        if sentence_order is not None and isinstance(attention_mask, F.PackedSequences):
+            raise NotImplementedError("packed sequences: no pooled output, so no sentence order")
         lm_labels = lm_labels if lm_labels is not None else labels
         out = self.language_model(input_ids, enc_attn_mask=attention_mask, tokentype_ids=tokentype_ids)
         if not self.post_process:

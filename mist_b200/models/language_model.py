@@ -99,7 +99,7 @@ class TransformerLanguageModel(nn.Module):
         cross attention sees them (defaults to ``enc_attn_mask``).  Masks without padding are dropped.
         A single-stack model takes a :class:`~mist_b200.ops.packed.PackedSequences` of its ``batch * seq`` tokens as
         ``enc_attn_mask``: documents packed back to back, which attend inside themselves and whose positions start at 0.
-        Documents longer than a learned position table are refused (where the offsets are on the GPU, by a status that
+        Nothing is pooled from them.  Documents longer than a learned position table are refused (where the offsets are on the GPU, by a status that
         :func:`~mist_b200.ops.native.check_status` raises)."""
         bs = enc_input_ids.shape[0] if enc_input_ids is not None else None
         if enc_hidden_states is None and self.encoder is None and self.enc_hidden_input is not None:
@@ -128,6 +128,8 @@ class TransformerLanguageModel(nn.Module):
             enc_out = enc_hidden_states
         if self.decoder is None:
             if self.pooler is not None:
+                if isinstance(enc_mask, F.PackedSequences):
+                    return enc_out, None        # a row's first token is that of its first document only
                 full = enc_out
                 if self.sequence_parallel:
                     full = dist_ops.all_gather(enc_out, self.pre_post_process_group, replicated_consumer=True).view(
