@@ -168,13 +168,16 @@ class TrainingSession:
         """One iteration on a dictionary of model inputs (what the family's inputs provider
         returns: token ids, token types, decoder ids, labels ...), each with this rank's
         ``micro_batch * G`` samples along dimension 0; used for the encoder-only and
-        encoder-decoder families whose forward takes more than ids and labels."""
+        encoder-decoder families whose forward takes more than ids and labels.  A list or tuple holds one value for each
+        of the ``G`` micro batches, such as their :class:`~mist_b200.ops.packed.PackedSequences`."""
         self._beat()
-        # (a list or tuple holds one value per micro batch: the packings of batches of packed sequences)
         listed = {k for k, v in batch.items() if isinstance(v, (list, tuple))}
         for k in listed:
             if len(batch[k]) != self.G:
                 raise ValueError(f"{k}: {len(batch[k])} values for {self.G} micro batches")
+        for k, v in batch.items():
+            if self.G > 1 and k not in listed and not isinstance(v, torch.Tensor):
+                raise ValueError(f"{k}: a list of {self.G} values, one for each of the micro batches, expected and not one {type(v).__name__}")
         if self.G == 1:
             batches = [{k: v[0] if k in listed else v for k, v in batch.items()}]
         else:
