@@ -254,7 +254,7 @@ def analysis_cache_name(model_cfg: ModelConfig, seq_len: int, tp: int, sequence_
     change the trace here (tp is traced concretely)."""
     return (f"model_{model_cfg.name}_ori_layers_{model_cfg.num_hidden_layers}_analyzed_layers_1"
             f"_f_{int(model_cfg.use_flash_attn)}_s_{seq_len}_v_{model_cfg.vocab_size}_tp_{tp}"
-            f"_sp_{int(sequence_parallel)}.pkl")
+            f"_sp_{int(sequence_parallel)}{'_lml_1' if model_cfg.fused_lm_loss else ''}.pkl")
 
 
 def get_analysis(cfg: MistConfig, tp: int, cache_dir: Optional[str] = None, sequence_parallel: Optional[bool] = None

@@ -132,13 +132,42 @@ def cross_entropy(logits, labels, vocab_start, group, ignore_index):
     return loss
 
 
+def linear_cross_entropy(x, weight, labels, bias):
+    """Projection and loss as one operator: what it keeps and holds follows the limits that the operator itself goes by."""
+    from ..ops import functional as F
+    from ..ops import linear_xent
+    w, bz = _p(weight), _p(bias)
+    rows, k, vocab = prod(x.shape[:-1]), x.shape[-1], w.shape[0]
+    keep = linear_xent.kept_bytes(rows, vocab)
+    kept = sp.And(rows <= 2 ** 20, keep <= F.Settings.xent_keep_bytes) if k >= linear_xent.KEEP_FROM else sp.false
+    # a piece of the gradient of the logits; its sums over rows; dx in fp32 where there are several pieces
+    piece = sp.Min(2 * rows * vocab, sp.Max(F.Settings.xent_piece_bytes, 512 * rows))
+    many = sp.Piecewise((4 * rows * k, 2 * rows * vocab > F.Settings.xent_piece_bytes), (0, True))
+    fl = 2 * rows * k * vocab
+    (loss,) = record("linear_cross_entropy", [x, w, bz, labels], [(tuple(x.shape[:-1]), torch.float32)], saved=[x, w, labels],
+                     saved_extra=rows * 4 + sp.Piecewise((keep - rows * 8, kept), (0, True)),
+                     fwd_workspace=sp.Piecewise((0, kept), (rows * (8 * -(-vocab // 256) + 4), True)),
+                     bwd_workspace=piece + many + (piece / 16 if bz is not None else 0),
+                     flops_fwd=fl, flops_bwd=sp.Piecewise((2 * fl, kept), (3 * fl, True)),
+                     bytes_fwd=(rows * k + k * vocab) * 2 + sp.Piecewise((keep, kept), (0, True)),
+                     bytes_bwd=(rows * k + k * vocab) * 4 + 4 * rows * vocab + sp.Piecewise((keep, kept), (0, True)),
+                     grad_inputs=[x],
+                     spec={"op": "linear_cross_entropy", "rows": rows, "k": k, "vocab": vocab, "bias": bz is not None})
+    return loss
+
+
 def embedding(ids, wte, wpe, vocab_start):
     w, pz = _p(wte), _p(wpe)
     b_, s = ids.shape
     h = w.shape[1]
+    # The backward pass sorts the tokens (keys and tokens twice, 16 bytes each) and leaves parts of rows that lie in several
+    # tiles of 32 of them; the table's gradient goes straight to where it is wanted.
+    parts = 8 * (b_ * s / sp.Integer(32) + 1) * (h + (h + 255) // 256)
+    wpe_bytes = pz.numel() * 2 if pz is not None else 0
     (out,) = record("embedding", [ids, w, pz], [((b_, s, h), w.dtype)], saved=[ids],
-                    bytes_fwd=3 * b_ * s * h * 2, bytes_bwd=b_ * s * h * 2 + w.numel() * 6,
-                    bwd_workspace=w.numel() * 4 + (pz.numel() * 4 if pz is not None else 0),
+                    bytes_fwd=3 * b_ * s * h * 2,
+                    bytes_bwd=(2 if pz is not None else 1) * b_ * s * h * 2 + w.numel() * 2 + wpe_bytes,
+                    bwd_workspace=16 * b_ * s + parts + wpe_bytes,
                     spec={"op": "embedding", "tokens": b_ * s, "h": h, "vocab": w.shape[0]})
     return out
 

@@ -103,7 +103,7 @@ class BertModel(nn.Module):
                 input_ids.shape[0], -1, hidden.shape[-1])
         wte = (self.language_model.embedding.word_embeddings.weight if self.pre_process
                else self.word_embeddings.weight)
-        fused = self.cfg.fused_lm_loss and lm_labels is not None and not F._sym(hidden)
+        fused = self.cfg.fused_lm_loss and lm_labels is not None
         logits = None if fused else self.lm_head(hidden, wte)
         binary_logits = self.binary_head(pooled) if (self.add_binary_head and pooled is not None) else None
         if lm_labels is None:

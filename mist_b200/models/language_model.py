@@ -184,7 +184,7 @@ class LMHead(nn.Module):
                                          dtype=dtype or cfg.params_dtype)
 
     def forward(self, hidden, labels=None, weight=None):
-        fused = (self.fused_loss and labels is not None and not F._sym(hidden)
+        fused = (self.fused_loss and labels is not None
                  and (weight is not None or is_plain_projection(self.proj)))
         if weight is not None or fused:   # tied embeddings
             x = hidden

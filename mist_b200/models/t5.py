@@ -78,7 +78,7 @@ class T5Model(nn.Module):
             enc_dec_attn_mask=encoder_decoder_attn_mask)
         if not self.post_process:
             return dec_out, enc_out
-        if self.cfg.fused_lm_loss and lm_labels is not None and not F._sym(dec_out):
+        if self.cfg.fused_lm_loss and lm_labels is not None:
             return self.lm_head(dec_out, self.language_model.embedding.word_embeddings.weight, lm_labels).mean()
         logits = self.lm_head(dec_out, self.language_model.embedding.word_embeddings.weight)
         if lm_labels is None:

@@ -25,6 +25,7 @@ class DeviceModel:
     # efficiency of the compute roof per operator (forward, backward)
     eff_compute: Dict[str, Tuple[float, float]] = field(default_factory=lambda: {
         "linear": (0.85, 0.85), "bmm": (0.6, 0.6), "flash_attention": (0.28, 0.22),
+        "linear_cross_entropy": (0.95, 0.85),
     })
     # efficiency of the memory roof per operator (forward, backward); "default" for the rest
     eff_memory: Dict[str, Tuple[float, float]] = field(default_factory=lambda: {

@@ -188,6 +188,11 @@ def profile(spec: NodeSpec, dtype=torch.bfloat16) -> Optional[Tuple[float, float
                 fwd = _time(lambda: F.cross_entropy(base, labels))
             total = _time(run) - copy_t
             return fwd, max(total - fwd, 0.0)
+        if op == "linear_cross_entropy":
+            rows, k, vocab = int(g("rows")), int(g("k")), int(g("vocab"))
+            labels = torch.randint(0, vocab, (rows,), device=dev)
+            return _fwd_bwd(lambda: (rnd(rows, k), rnd(vocab, k, scale=0.02), rnd(vocab) if g("bias") else None),
+                            lambda x, w, b: F.linear_cross_entropy(x, w, labels, b))
         if op == "embedding":
             tokens, h, vocab = int(g("tokens")), int(g("h")), int(g("vocab"))
             seq = min(tokens, 2048)

@@ -185,6 +185,8 @@ def linear_cross_entropy(x, weight, labels, bias=None, vocab_start: int = 0, gro
     ``weight`` ``[vocab, hidden]`` (and ``bias`` ``[vocab]``) may be this rank's slice of the vocabulary, starting at
     ``vocab_start``; ``group`` is then the group of the slices, and ``x`` is the same on every rank of it (its gradient is
     this slice's share).  The weight's gradient goes into its bucket where it has one."""
+    if F._sym(x):
+        return F._rules().linear_cross_entropy(x, weight, labels, bias)
     if F._elsewhere(x):
         with torch.cuda.device(x.device):
             return linear_cross_entropy(x, weight, labels, bias, vocab_start, group, ignore_index)
