@@ -1166,29 +1166,33 @@ def _embed_workspace(tokens: int, h: int, with_positions: int) -> int:
     return native.kernels().mb_embed_bwd_workspace(tokens, h, with_positions)
 
 
+def _embed_lookup(ids, wte, wpe, v0, scale, pos, strict):
+    b, s = ids.shape
+    h = wte.shape[1]
+    if not use_native(wte):
+        loc = ids - v0
+        inr = (loc >= 0) & (loc < wte.shape[0])
+        out = wte[loc.clamp(0, wte.shape[0] - 1)].float() * (inr[..., None].float() * scale)
+        if wpe is not None and pos is None:
+            out = out + wpe[:s].float()[None]
+        elif wpe is not None:
+            known = (pos >= 0) & (pos < wpe.shape[0])
+            out = out + wpe[pos.clamp(0, wpe.shape[0] - 1)].float() * known[..., None].float()
+        return out.to(wte.dtype)
+    out = torch.empty(b, s, h, dtype=wte.dtype, device=wte.device)
+    call("mb_embed_fwd", ptr(ids), ptr(pos), ptr(wte), ptr(wpe), ptr(out), b * s, max(s, 1), h, v0, wte.shape[0],
+         0 if wpe is None else wpe.shape[0], strict, scale, stream())
+    return out
+
+
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, wte, wpe, v0, scale, pos, strict):
-        b, s = ids.shape
-        h = wte.shape[1]
         ctx.v0, ctx.scale, ctx.strict = v0, scale, strict
         ctx.has_pos = wpe is not None
         ctx.param = _bucket_owner(wte)
         ctx.save_for_backward(ids, wte, wpe, pos)
-        if not use_native(wte):
-            loc = ids - v0
-            inr = (loc >= 0) & (loc < wte.shape[0])
-            out = wte[loc.clamp(0, wte.shape[0] - 1)].float() * (inr[..., None].float() * scale)
-            if wpe is not None and pos is None:
-                out = out + wpe[:s].float()[None]
-            elif wpe is not None:
-                known = (pos >= 0) & (pos < wpe.shape[0])
-                out = out + wpe[pos.clamp(0, wpe.shape[0] - 1)].float() * known[..., None].float()
-            return out.to(wte.dtype)
-        out = torch.empty(b, s, h, dtype=wte.dtype, device=wte.device)
-        call("mb_embed_fwd", ptr(ids), ptr(pos), ptr(wte), ptr(wpe), ptr(out), b * s, max(s, 1), h, v0, wte.shape[0],
-             0 if wpe is None else wpe.shape[0], strict, scale, stream())
-        return out
+        return _embed_lookup(ids, wte, wpe, v0, scale, pos, strict)
 
     @staticmethod
     def backward(ctx, dout):
@@ -1263,7 +1267,10 @@ def embedding(ids, wte, wpe=None, vocab_start: int = 0, scale: float = 1.0, posi
                     or t.shape[1] % 8 or t.device != ids.device):
                 raise ValueError(f"{name}: contiguous bf16 rows of a multiple of 8 values on the device of the ids expected")
         ids = ids.long().contiguous()
-    return _EmbeddingFn.apply(ids, wte, wpe, int(vocab_start), float(scale), pos, int(strict_positions))
+    run = _embed_lookup
+    if torch.is_grad_enabled() and (wte.requires_grad or (wpe is not None and wpe.requires_grad)):
+        run = _EmbeddingFn.apply
+    return run(ids, wte, wpe, int(vocab_start), float(scale), pos, int(strict_positions))
 
 
 # --------------------------------------------------------------------- optimizer / casts
