@@ -14,7 +14,19 @@ constexpr int kCosts = 8192;       // blocks of 128 a tile walks; dearer ones co
 // queries), whose outputs are zeros.  Items of one cost come in no fixed order; no result depends on it but the order in
 // which dQ is summed.
 __global__ void __launch_bounds__(kThreads)
-packed_plan_kernel(const int* cu_q, const int* cu_k, int n, int total_q, int total_k, uint8_t* plan) {
+packed_plan_kernel(const int* cu_q, const int* cu_k, int n, int total_q, int total_k, uint8_t* plan, int* ends) {
+  if (ends && blockIdx.x == gridDim.x - 1) {      // where the offsets end, or -1 for impossible ones
+    const int* cu[2] = {cu_q, cu_k};
+    const int total[2] = {total_q, total_k};
+    for (int u = 0; u < 2; ++u) {
+      bool bad = cu[u][0] != 0 || cu[u][n] > total[u];
+      for (int i = threadIdx.x; i < n; i += kThreads) bad |= cu[u][i + 1] < cu[u][i];
+      bad = __syncthreads_or(bad);
+      if (threadIdx.x == 0) ends[u] = bad ? -1 : cu[u][n];
+    }
+    if (threadIdx.x == 0) __threadfence_system();
+    return;
+  }
   __shared__ int count[kCosts];
   __shared__ int part[32], all_costs, dearest;
   auto clamped = [](int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); };
@@ -146,24 +158,24 @@ MB_API long mb_packed_plan_bytes(int n, int total_q, int total_k) {
 // Where in a plan every query row's place in its sequence stands: total_q numbers of 64 bits.
 MB_API long mb_packed_plan_positions(int n, int total_q, int total_k) { return packed_positions_offset(total_q, total_k, n); }
 
-// cu_q, cu_k: n + 1 offsets each, in device memory.  The plan (16-byte aligned) serves causal and full attention, forward
-// and backward, with any number of heads.
-MB_API int mb_packed_plan(const int* cu_q, const int* cu_k, int n, int total_q, int total_k, void* plan, cudaStream_t stream) {
+// cu_q, cu_k: n + 1 offsets each, in device memory; host_q, host_k: null, or the offsets in host memory, which are then
+// written there first.  The plan (16-byte aligned) serves causal and full attention, forward and backward, with any number of
+// heads.  ends: null, or two numbers in pinned host memory that get the last offsets, or -1 where they are impossible.
+MB_API int mb_packed_plan(int* cu_q, int* cu_k, const int* host_q, const int* host_k, int n, int total_q, int total_k, void* plan,
+                          int* ends, cudaStream_t stream) {
   if (n < 0 || total_q < 0 || total_k < 0 || (reinterpret_cast<uintptr_t>(plan) & 15)) return -1;
-  packed_plan_kernel<<<4 + (total_q + kThreads - 1) / kThreads, kThreads, 0, stream>>>(
-      cu_q, cu_k, n, total_q, total_k, static_cast<uint8_t*>(plan));
-  return cudaGetLastError() == cudaSuccess ? 0 : -4;
-}
-
-// n offsets in host memory to device memory.
-MB_API int mb_packed_offsets(const int* host, int n, int* out, cudaStream_t stream) {
-  if (n < 0) return -1;
-  for (int first = 0; first < n; first += kOffsets) {
-    Offsets part;
-    const int count = n - first < kOffsets ? n - first : kOffsets;
-    memcpy(part.at, host + first, sizeof(int) * count);
-    packed_offsets_kernel<<<1, 256, 0, stream>>>(part, count, out + first);
+  const int* from[2] = {host_q, host_k};
+  int* to[2] = {cu_q, cu_k};
+  for (int u = 0; u < 2; ++u) {
+    for (int first = 0; from[u] && first <= n; first += kOffsets) {
+      Offsets part;
+      const int count = n + 1 - first < kOffsets ? n + 1 - first : kOffsets;
+      memcpy(part.at, from[u] + first, sizeof(int) * count);
+      packed_offsets_kernel<<<1, 256, 0, stream>>>(part, count, to[u] + first);
+    }
   }
+  packed_plan_kernel<<<4 + (total_q + kThreads - 1) / kThreads + (ends ? 1 : 0), kThreads, 0, stream>>>(
+      cu_q, cu_k, n, total_q, total_k, static_cast<uint8_t*>(plan), ends);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 

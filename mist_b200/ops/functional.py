@@ -873,8 +873,8 @@ def attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k=None, scale: Optional[f
     :class:`PackedSequences` in the place of ``cu_seqlens_q``.  One launch covers all sequences, in the forward pass and
     in the backward pass.  A causal query sees the keys up to its own place, the
     sequences aligned at their ends.  Queries without a key give zeros.
-    Returns as many rows as the offsets say (all, of zeros, where they say none); offsets on the GPU are read back for that, once,
-    behind the launches, and refused if they do not begin with 0 or fall.  With a :class:`PackedSequences`, and while a graph is
+    Returns as many rows as the offsets say (all, of zeros, where they say none); where they are on the GPU their end is read
+    back for that behind the launches, and impossible ones are refused.  With a :class:`PackedSequences`, and while a graph is
     captured, nothing is read back: all ``total_q`` rows are returned, zeros behind the last sequence (the interface of the
     reference's ``flash_attn_varlen`` entry points, csrc/flash_attn/flash_api.cpp ``varlen_fwd`` / ``varlen_bwd``)."""
     if _elsewhere(q):
@@ -886,11 +886,10 @@ def attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k=None, scale: Optional[f
         if cu_seqlens_k is not None:
             raise ValueError("a PackedSequences holds the offsets of the keys: none can be given beside it")
         return packed_attention.attention(q, k, v, cu_seqlens_q, scale, causal)
-    seqs = PackedSequences(cu_seqlens_q, q.shape[0], cu_seqlens_k, k.shape[0], device=q.device)
+    seqs = packed_attention.PackedCall(cu_seqlens_q, q.shape[0], cu_seqlens_k, k.shape[0], q.device)
     out = packed_attention.attention(q, k, v, seqs, scale, causal)
-    seqs.read_back()
-    rows = seqs.host_q[-1] if seqs.host_q is not None else 0
-    return out if rows in (0, q.shape[0]) else out[:rows]
+    rows = seqs.end()
+    return out if rows in (None, 0, q.shape[0]) else out[:rows]
 
 
 class _PackedAttnFn(torch.autograd.Function):

@@ -76,8 +76,7 @@ _SIGNATURES = {
     "mb_attn_sum_parts": ([_p] * 4 + [_i] * 5 + [_l] * 6 + [_p], _i),
     "mb_packed_plan_bytes": ([_i, _i, _i], _l),
     "mb_packed_plan_positions": ([_i, _i, _i], _l),
-    "mb_packed_plan": ([_p, _p, _i, _i, _i, _p, _p], _i),
-    "mb_packed_offsets": ([_p, _i, _p, _p], _i),
+    "mb_packed_plan": ([_p, _p, _p, _p, _i, _i, _i, _p, _p, _p], _i),
     "mb_packed_limit": ([_p, _i, _i, _i, _p], _i),
     "mb_attn_fwd_packed_counters": ([_i, _i, _i], _i),
     "mb_attn_fwd_packed": ([_p] * 7 + [_i] * 6 + [_l] * 8 + [_f, _i, _p], _i),

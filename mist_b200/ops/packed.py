@@ -48,18 +48,25 @@ def _offsets(cu, device):
     _check_offsets(host)
     if host[-1] > INT32_MAX:
         raise ValueError(f"offsets up to {host[-1]}: 32 bits hold them")
-    if device.type != "cuda":
-        return torch.tensor(host, dtype=torch.int32, device=device), host
-    # by the arguments of a kernel: nothing waits, and a graph that is captured holds them
-    out = torch.empty(len(host), dtype=torch.int32, device=device)
-    with torch.cuda.device(device):
-        call("mb_packed_offsets", (ctypes.c_int * len(host))(*host), len(host), ptr(out), stream())
-    return out, host
+    # (to a GPU they go as arguments of a kernel: nothing waits, and a graph that is captured holds them)
+    return torch.empty(len(host), dtype=torch.int32, device=device) if device.type == "cuda" else torch.tensor(host, dtype=torch.int32), host
 
 
 def _check_offsets(host):
     if not host or host[0] != 0 or any(b < a for a, b in zip(host, host[1:])):
         raise ValueError("offsets: they begin with 0 and do not fall")
+
+
+_streams = {}
+
+
+def _current_stream(index: int):
+    """The current stream of a device as an object; one for each raw handle is kept, because making it takes 3 us."""
+    handle = torch._C._cuda_getCurrentRawStream(index)
+    stream = _streams.get((index, handle))
+    if stream is None:
+        stream = _streams[index, handle] = torch.cuda.current_stream(index)
+    return stream
 
 
 class _Made:
@@ -71,7 +78,7 @@ class _Made:
         self.seen = {torch._C._cuda_getCurrentRawStream(device.index)}
         if not torch.cuda.is_current_stream_capturing():
             self.event = torch.cuda.Event()
-            self.event.record(torch.cuda.current_stream(device))
+            self.event.record(_current_stream(device.index))
 
     def here(self):
         now = torch._C._cuda_getCurrentRawStream(self.index)
@@ -79,7 +86,7 @@ class _Made:
         # when the device is idle)
         if now in self.seen or self.event is None or torch.cuda.is_current_stream_capturing():
             return
-        current = torch.cuda.current_stream(self.index)
+        current = _current_stream(self.index)
         current.wait_event(self.event)
         for t in self.tensors:
             t.record_stream(current)
@@ -97,6 +104,11 @@ class PackedSequences:
     ``torch.cuda.graph`` has begun)."""
 
     def __init__(self, cu_seqlens, total: Optional[int] = None, cu_seqlens_k=None, total_k: Optional[int] = None, device=None):
+        self._set_up(cu_seqlens, total, cu_seqlens_k, total_k, device)
+        if self.plan is not None:
+            self._made = _Made(self.device, self.cu_q, self.cu_k, self.plan)
+
+    def _set_up(self, cu_seqlens, total, cu_seqlens_k, total_k, device, ends=0):
         if device is None and isinstance(cu_seqlens, torch.Tensor):
             device = cu_seqlens.device
         else:
@@ -115,17 +127,24 @@ class PackedSequences:
         self._rotary = {}
         self._positions = self.plan = self._made = None
         if use_native(self.cu_q):
-            with torch.inference_mode(False):      # autograd keeps none that were made under inference mode
-                self.plan = torch.empty(_plan_bytes(self.n, self.total_q, self.total_k), dtype=torch.uint8, device=device)
+            size = _plan_bytes(self.n, self.total_q, self.total_k)
+            if torch.is_inference_mode_enabled():      # autograd keeps none that were made under it
+                with torch.inference_mode(False):
+                    self.plan = torch.empty(size, dtype=torch.uint8, device=device)
+            else:
+                self.plan = torch.empty(size, dtype=torch.uint8, device=device)
             if device.index == torch._C._cuda_getDevice():
-                self._make_plan()
+                self._make_plan(ends)
             else:
                 with torch.cuda.device(device):
-                    self._make_plan()
+                    self._make_plan(ends)
 
-    def _make_plan(self):
-        call("mb_packed_plan", ptr(self.cu_q), ptr(self.cu_k), self.n, self.total_q, self.total_k, ptr(self.plan), stream())
-        self._made = _Made(self.device, self.cu_q, self.cu_k, self.plan)
+    def _make_plan(self, ends):
+        def ints(host):
+            return None if host is None else (ctypes.c_int * len(host))(*host)
+
+        call("mb_packed_plan", ptr(self.cu_q), ptr(self.cu_k), ints(self.host_q), None if self.same else ints(self.host_k),
+             self.n, self.total_q, self.total_k, ptr(self.plan), ends, stream())
 
     def here(self):
         """The plan and the offsets, for kernels of the current stream."""
@@ -160,19 +179,6 @@ class PackedSequences:
             self.here()
             with torch.cuda.device(self.device):
                 call("mb_packed_limit", ptr(self.cu_q), self.n, self.total_q, most, stream())
-
-    def read_back(self):
-        """Offsets on the GPU come to the host, where they are checked; waits for the current stream.  Not while a graph is
-        captured."""
-        if (self.host_q is not None and self.host_k is not None) or torch.cuda.is_current_stream_capturing():
-            return
-        self.here()
-        host_q = self.cu_q.tolist() if self.host_q is None else self.host_q
-        host_k = host_q if self.same else (self.cu_k.tolist() if self.host_k is None else self.host_k)
-        for host, total in ((host_q, self.total_q), (host_k, self.total_k)):
-            _check_offsets(host)
-            self._total(total, host)
-        self.host_q, self.host_k = host_q, host_k
 
     @staticmethod
     def _total(total, host):
@@ -215,6 +221,37 @@ class PackedSequences:
         """``(queries, keys)`` slices of every sequence (reference path: reads the offsets)."""
         q, k = self.host_q or self.cu_q.tolist(), self.host_k or self.cu_k.tolist()
         return [(slice(q[i], q[i + 1]), slice(k[i], k[i + 1])) for i in range(self.n)]
+
+
+_ends = {}      # of each device: pinned numbers and events of calls that are over
+
+
+class PackedCall(PackedSequences):
+    """The packing of one call on one stream: nobody else waits for it, and the ends of its offsets come to the host."""
+
+    def __init__(self, cu_q, total_q, cu_k, total_k, device):
+        self._reads = None
+        if (device.type == "cuda" and any(isinstance(cu, torch.Tensor) and cu.is_cuda for cu in (cu_q, cu_k))
+                and not torch.cuda.is_current_stream_capturing()):
+            free = _ends.setdefault(device.index, [])
+            self._reads = free.pop() if free else (torch.empty(2, dtype=torch.int32, pin_memory=True), torch.cuda.Event())
+        self._set_up(cu_q, total_q, cu_k, total_k, device, 0 if self._reads is None else ptr(self._reads[0]))
+        if self._reads is not None:
+            self._reads[1].record(_current_stream(device.index))
+
+    def end(self):
+        """Where the queries' last sequence ends, or ``None`` where that is only known on the GPU and a graph is being captured.
+        Impossible offsets raise; waits for the plan, but not for what was launched behind it."""
+        if self._reads is None:
+            return None if self.host_q is None else self.host_q[-1]
+        pinned, event = self._reads
+        event.synchronize()
+        ends = pinned.tolist()
+        _ends[self.device.index].append(self._reads)
+        self._reads = None
+        if min(ends) < 0:
+            raise ValueError("offsets: they begin with 0, do not fall, and end within the tensors")
+        return ends[0]
 
 
 def _rows(t):

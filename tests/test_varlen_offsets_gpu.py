@@ -85,3 +85,21 @@ def test_offsets_of_the_host_in_a_captured_graph(causal):
             graph.replay()
         assert torch.equal(out, want)
         assert torch.equal(other, F.attention_varlen(*t, [0, 30, 70], [0, 10, 70], causal=causal))
+
+
+def test_the_ends_of_calls_on_two_streams_are_their_own():
+    """Calls on both streams at once, behind a delay on the first: each reads back its own ends."""
+    t = _tensors(100)
+    cus = [torch.tensor([0, 30, 70], device=DEV), torch.tensor([0, 10, 90], device=DEV)]
+    with torch.no_grad():
+        want = [F.attention_varlen(*t, cu) for cu in cus]
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        for _ in range(3):
+            for s, cu, w in zip(streams, cus, want):
+                with torch.cuda.stream(s):
+                    torch.cuda._sleep(1_000_000)
+                    out = F.attention_varlen(*t, cu)
+                assert out.shape == w.shape
+                s.synchronize()
+                assert torch.equal(out, w)
