@@ -69,6 +69,9 @@ def _current_stream(index: int):
     return stream
 
 
+_events = {}      # of each device: those of packings that are gone (making and destroying one takes 5 us)
+
+
 class _Made:
     """Tensors that were made on the stream that was current then.  Others wait for that once, where they first use them; the
     allocator learns of them.  Tensors of a graph being captured belong to it: nobody outside waits for them."""
@@ -77,8 +80,13 @@ class _Made:
         self.index, self.tensors, self.event = device.index, tensors, None
         self.seen = {torch._C._cuda_getCurrentRawStream(device.index)}
         if not torch.cuda.is_current_stream_capturing():
-            self.event = torch.cuda.Event()
+            free = _events.setdefault(device.index, [])
+            self.event = free.pop() if free else torch.cuda.Event()
             self.event.record(_current_stream(device.index))
+
+    def __del__(self):
+        if self.event is not None and _events is not None:      # (nothing is left of the module when the process ends)
+            _events[self.index].append(self.event)
 
     def here(self):
         now = torch._C._cuda_getCurrentRawStream(self.index)
