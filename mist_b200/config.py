@@ -123,7 +123,7 @@ class ModelConfig:
     scale_attn_by_inverse_layer_idx: bool = False
     use_flash_attn: bool = False
     bias_dropout_fusion: bool = True
-    # projection and cross entropy of the LM head as one operator without logits in between (ops/linear_xent.py)
+    # projection and cross entropy of the LM head as one operator (ops/linear_xent.py, which says what it holds in between)
     fused_lm_loss: bool = False
     tensor_parallel: Optional[bool] = None
     sequence_parallel: Optional[bool] = None

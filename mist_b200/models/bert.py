@@ -26,7 +26,7 @@ class BertLMHead(nn.Module):
             nn.init.zeros_(self.dense.bias)
 
     def forward(self, hidden, word_embeddings_weight, labels=None):
-        """Logits, or with ``labels`` the loss of every token, without logits."""
+        """Logits, or with ``labels`` the loss of every token, in one operator with the projection."""
         x = F.linear(hidden, self.dense.weight, self.dense.bias, activation="gelu")
         x = self.norm(x)
         x = dist_ops.copy_to_group(x, self.process_group)

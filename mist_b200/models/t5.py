@@ -22,7 +22,7 @@ class T5LMHead(nn.Module):
         self.bias = nn.Parameter(torch.zeros(local_vocab, device=device, dtype=dtype))
 
     def forward(self, hidden, word_embeddings_weight, labels=None):
-        """Logits, or with ``labels`` the loss of every token, without logits."""
+        """Logits, or with ``labels`` the loss of every token, in one operator with the projection."""
         if self.sequence_parallel:      # token shards -> all tokens; the backward pass reduce-scatters
             x = dist_ops.all_gather(hidden.reshape(-1, hidden.shape[-1]), self.process_group)
         else:

@@ -718,7 +718,7 @@ def vocab_parallel_cross_entropy(logits, labels, process_group=None, ignore_inde
 
 
 def linear_vocab_parallel_cross_entropy(x, weight, labels, process_group=None, bias=None, ignore_index=-100):
-    """Per-token loss of the logits ``x @ weight.T + bias`` against global labels, without logits; ``weight`` and
+    """Per-token loss of the logits ``x @ weight.T + bias`` against global labels, in one operator; ``weight`` and
     ``bias`` are this rank's slice of the vocabulary, ``x`` (``[tokens, hidden]``) is the same on every rank."""
     ws = group_size(process_group)
     group = None if (ws == 1 or isinstance(process_group, dist_ops.FakeGroup)) else process_group

@@ -1,12 +1,18 @@
-"""Vocabulary projection and cross entropy as one operator that holds neither the logits nor their gradient.
+"""Vocabulary projection and cross entropy as one operator, whose logits are never stored as numbers of their own.
 
 ``loss[t] = log sum_v exp(x_t . w_v + b_v) - (x_t . w_label + b_label)``.  The forward pass is one GEMM whose epilogue
 keeps a maximum and a sum per row and tile.  The backward pass goes over the vocabulary piece by piece, gets the gradient
 of a piece's logits and multiplies it into the gradients of ``x`` and of the weight.  It has the logits from the forward
-pass, which keeps 16 bits of each while they take no more than ``Settings.xent_keep_bytes`` and the hidden size makes it
-worth while, or computes them again (8192 tokens of 2560, vocabulary 50304, both passes: 5.1 ms with 824 MB kept, 6.4 ms
-with two numbers per row) (reference: the projection of mist/modules/fused_dense.py:221-327
-followed by mist/modules/losses.py:48-176, which hold ``[tokens, vocabulary]`` logits between the two).
+pass, which keeps 16 bits of each while all that it keeps takes no more than ``Settings.xent_keep_bytes`` and the hidden
+size makes it worth while, or computes them again.
+
+So by default this operator saves no memory: 16 bits per logit are what the two separate steps hold too, whose gradient
+overwrites their logits.  ``xent_keep_bytes = 0`` is the form that holds two numbers per row and one piece of the gradient.
+Both passes of 8192 tokens of 2560, vocabulary 50304 (time; held between the passes; at most, the gradients included):
+separate steps 5.4 ms, 786 MiB, 1072 MiB; logits kept 5.3 ms, 811, 1395; computed twice 6.4 ms, 0, 584.  What the first form
+has over the separate steps is the loss of fp32 logits instead of bf16 ones (reference: the projection of
+mist/modules/fused_dense.py:221-327 followed by mist/modules/losses.py:48-176, which hold ``[tokens, vocabulary]`` logits
+between the two).
 """
 from __future__ import annotations
 
@@ -18,8 +24,10 @@ from . import functional as F
 from . import native
 from .native import INT32_MAX, call, ptr, stream, use_native
 
-# Hidden sizes from which a logit is kept and not computed again.  Both passes of 4096 tokens, vocabulary 50304 (kept, twice, us):
-# hidden 2048 2329, 2664; 1024 1448, 1552; 512 963, 978; 256 771, 717; vocabulary 8192: 1024 217, 232; 512 187, 174.
+# Hidden sizes from which a logit is kept and not computed again.  Both passes, vocabulary 50304 (kept, twice, us): 4096 tokens of
+# 4096 3952, 5145; of 2048 2197, 2574; of 1024 1250, 1474; of 512 766, 875; 256 tokens of 4096 482, 571; of 1024 294, 309; of 512
+# 266, 270; 16384 of 1024 5033, 5758; of 512 3377, 3775.  Vocabulary 8192: 4096 tokens of 1024 209, 234; of 512 159, 163; up to 1024
+# tokens of 2048 the host decides (140, 136).  Below 1024 a tenth of the time is not worth memory of 16 bits per logit.
 KEEP_FROM = 1024
 
 
@@ -179,7 +187,8 @@ def _reference_backward(x2, weight, bias, labels, lse, gloss, v0, ignore, dx, dw
 def linear_cross_entropy(x, weight, labels, bias=None, vocab_start: int = 0, group=None, ignore_index: int = -100):
     """Loss (fp32) of every row of ``x`` ``[..., hidden]`` against ``labels`` ``[...]``: the cross entropy of the logits
     ``x @ weight.T + bias``, which are computed in fp32 and never stored as such.  For the backward pass 16 bits of each are
-    kept while that takes no more than ``Settings.xent_keep_bytes``; otherwise it computes them again.  Rows labelled
+    kept while all that is kept takes no more than ``Settings.xent_keep_bytes`` (2 GiB; 0: never); otherwise it computes them
+    again.  Rows labelled
     ``ignore_index`` have loss 0 and give no gradient.  A label outside the vocabulary counts as one whose logit is 0; no one checks for it.
 
     ``weight`` ``[vocab, hidden]`` (and ``bias`` ``[vocab]``) may be this rank's slice of the vocabulary, starting at

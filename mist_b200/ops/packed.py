@@ -2,7 +2,7 @@
 
 A :class:`PackedSequences` is made once per batch.  It holds the offsets, every token's position in its sequence, and the
 work lists that the attention kernels walk (csrc/packed_plan.cu); all layers, forward and backward, use the same one, and
-nothing is read back to the host (reference: csrc/flash_attn/flash_api.cpp:427, 814 ``varlen_fwd`` / ``varlen_bwd``, called
+nothing is read back to the host, but by ``attention_varlen`` with bare offsets on the GPU (reference: csrc/flash_attn/flash_api.cpp:427, 814 ``varlen_fwd`` / ``varlen_bwd``, called
 with offsets that mist/modules/mha.py:1233-1243 derives from a padding mask)."""
 from __future__ import annotations
 
