@@ -1245,9 +1245,9 @@ def embedding(ids, wte, wpe=None, vocab_start: int = 0, scale: float = 1.0, posi
     that broadcast to the shape of ``ids``), what stands there -- documents packed into one row start again at 0.
     Positions outside ``wpe`` add nothing.  With ``strict_positions`` they are indices of the table as elsewhere: negative
     ones count from its end, and ones outside it are an error, an ``IndexError`` here where ``position_ids`` are on the host,
-    else a status that :func:`~mist_b200.ops.native.check_status` raises (and they add nothing).  The sum is in fp32, rounded once.  The gradients of both tables are summed
-    over tokens sorted by row, in fp32 and always in the same order; the one of ``wte`` goes straight into its gradient
-    bucket where it has one."""
+    else a status that :func:`~mist_b200.ops.native.check_status` raises (and they add nothing).  The sum is in fp32,
+    rounded once.  The gradients of both tables are summed over tokens sorted by row, in fp32 and always in the same order;
+    the one of ``wte`` goes straight into its gradient bucket where it has one."""
     if _sym(ids):
         return _rules().embedding(ids, wte, wpe, vocab_start)
     if _elsewhere(wte):

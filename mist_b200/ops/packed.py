@@ -40,7 +40,7 @@ def _offsets(cu, device):
     if isinstance(cu, torch.Tensor):
         if cu.dim() != 1 or cu.numel() < 1 or cu.is_floating_point():
             raise ValueError(f"offsets: a vector of integers expected, got {tuple(cu.shape)} of {cu.dtype}")
-        if cu.is_cuda:
+        if cu.is_cuda and device.type == "cuda":
             if cu.dtype != torch.int32 or cu.device != device or not cu.is_contiguous():
                 cu = cu.to(device=device, dtype=torch.int32).contiguous()
             return cu, None
@@ -238,7 +238,7 @@ class PackedCall(PackedSequences):
     """The packing of one call on one stream: nobody else waits for it, and the ends of its offsets come to the host."""
 
     def __init__(self, cu_q, total_q, cu_k, total_k, device):
-        self._reads = None
+        self._reads, self._index = None, device.index
         if (device.type == "cuda" and any(isinstance(cu, torch.Tensor) and cu.is_cuda for cu in (cu_q, cu_k))
                 and not torch.cuda.is_current_stream_capturing()):
             free = _ends.setdefault(device.index, [])
@@ -246,6 +246,12 @@ class PackedCall(PackedSequences):
         self._set_up(cu_q, total_q, cu_k, total_k, device, 0 if self._reads is None else ptr(self._reads[0]))
         if self._reads is not None:
             self._reads[1].record(_current_stream(device.index))
+
+    def __del__(self):
+        """A call that raised: its plan may still be about to write the numbers."""
+        if self._reads is not None:
+            self._reads[1].synchronize()
+            _ends[self._index].append(self._reads)
 
     def end(self):
         """Where the queries' last sequence ends, or ``None`` where that is only known on the GPU and a graph is being captured.
@@ -255,7 +261,7 @@ class PackedCall(PackedSequences):
         pinned, event = self._reads
         event.synchronize()
         ends = pinned.tolist()
-        _ends[self.device.index].append(self._reads)
+        _ends[self._index].append(self._reads)
         self._reads = None
         if min(ends) < 0:
             raise ValueError("offsets: they begin with 0, do not fall, and end within the tensors")

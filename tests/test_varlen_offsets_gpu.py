@@ -103,3 +103,34 @@ def test_the_ends_of_calls_on_two_streams_are_their_own():
                 assert out.shape == w.shape
                 s.synchronize()
                 assert torch.equal(out, w)
+
+
+def test_a_call_that_raises_keeps_its_pinned_numbers():
+    """Tensors that do not fit are refused behind the launch of the plan, which writes them when its turn comes."""
+    from mist_b200.ops import packed
+    q, k, v = _tensors(70)
+    cu = torch.tensor([0, 30, 70], device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    free = packed._ends.setdefault(q.device.index, [])
+    kept = list(free)
+    free.clear()                                        # the call takes new ones
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(40_000_000)
+        with pytest.raises(ValueError):
+            F.attention_varlen(q, k, v[:, :1], cu)
+    others = [torch.full((2,), 7, dtype=torch.int32, pin_memory=True) for _ in range(50)]
+    torch.cuda.synchronize()
+    assert all(t.tolist() == [7, 7] for t in others)
+    import gc
+    gc.collect()
+    assert len(free) == 1 and free[0][0].tolist() == [70, 70]
+    free.extend(kept)
+
+
+def test_offsets_on_the_gpu_of_tensors_on_the_host():
+    x = torch.randn(100, 2, 16)
+    for cu in (torch.tensor([0, 30, 70]), torch.tensor([0, 30, 70], device=DEV)):
+        assert torch.equal(F.attention_varlen(x, x, x, cu), F.attention_varlen(x, x, x, [0, 30, 70]))
+    with pytest.raises(ValueError):
+        F.attention_varlen(x, x, x, torch.tensor([1, 70], device=DEV))
