@@ -174,8 +174,9 @@ def call(name: str, *args):
 
 
 _STATUS_NAMES = {1: "TMA stage wait timed out", 2: "free-stage wait timed out",
-                 3: "accumulator wait timed out", 4: "peer flag wait timed out", 5: "bad argument",
-                 6: "a position outside the table of positions"}
+                 3: "accumulator wait timed out", 4: "peer flag wait timed out", 5: "bad argument"}
+# what kernels report that ran to their end
+_REPORTS = {6: "a position outside the table of positions"}
 
 
 def read_and_clear_status() -> int:
@@ -185,7 +186,7 @@ def read_and_clear_status() -> int:
 
 
 def status_message(code: int) -> str:
-    return f"a kernel reported status {code}: {_STATUS_NAMES.get(code, 'unknown')}"
+    return f"a kernel reported status {code}: {_STATUS_NAMES.get(code) or _REPORTS.get(code, 'unknown')}"
 
 
 def check_status():

@@ -71,3 +71,9 @@ def test_generation_behind_the_table():
     with pytest.raises(IndexError):
         generate(model, torch.cat([ids, ids], 1), 1)
     assert generate(model, ids, 6, eos_token_id=int(out[0, 32])).shape[1] <= 33
+
+
+def test_the_status_of_a_position_has_a_name():
+    from mist_b200.ops import native
+    assert "position" in native.status_message(6) and "unknown" in native.status_message(7)
+    assert "peer flag" in native.status_message(4)
