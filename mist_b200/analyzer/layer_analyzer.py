@@ -32,6 +32,7 @@ import torch
 
 from ..config import MistConfig, ModelConfig
 from ..models.provider import base_model_provider, family_of
+from ..ops import functional as F
 from ..parallel.dist_ops import FakeGroup
 from ..symbols import SymbolManager
 from .symtensor import Comm, Graph, Node, SymTensor, set_scope, tracing
@@ -252,9 +253,11 @@ def trace_and_analyze(model_cfg: ModelConfig, seq_len: int, tp: int = 1, sequenc
 def analysis_cache_name(model_cfg: ModelConfig, seq_len: int, tp: int, sequence_parallel: bool) -> str:
     """Same naming scheme as the reference's analysis cache, extended by the fields that
     change the trace here (tp is traced concretely)."""
+    # (what the fused loss keeps goes by its limits)
+    loss = f"_lml_{F.Settings.xent_keep_bytes}_{F.Settings.xent_piece_bytes}" if model_cfg.fused_lm_loss else ""
     return (f"model_{model_cfg.name}_ori_layers_{model_cfg.num_hidden_layers}_analyzed_layers_1"
             f"_f_{int(model_cfg.use_flash_attn)}_s_{seq_len}_v_{model_cfg.vocab_size}_tp_{tp}"
-            f"_sp_{int(sequence_parallel)}{'_lml_1' if model_cfg.fused_lm_loss else ''}.pkl")
+            f"_sp_{int(sequence_parallel)}{loss}.pkl")
 
 
 def get_analysis(cfg: MistConfig, tp: int, cache_dir: Optional[str] = None, sequence_parallel: Optional[bool] = None

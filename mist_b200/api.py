@@ -177,7 +177,8 @@ class TrainingSession:
                 raise ValueError(f"{k}: {len(batch[k])} values for {self.G} micro batches")
         for k, v in batch.items():
             if self.G > 1 and k not in listed and not hasattr(v, "chunk"):
-                raise ValueError(f"{k}: a list of {self.G} values, one for each of the micro batches, expected and not one {type(v).__name__}")
+                raise ValueError(f"{k}: a list of {self.G} values, one for each of the micro batches, expected, "
+                                 f"not one {type(v).__name__}")
         if self.G == 1:
             batches = [{k: v[0] if k in listed else v for k, v in batch.items()}]
         else:

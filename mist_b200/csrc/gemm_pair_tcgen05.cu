@@ -72,12 +72,12 @@ __device__ __forceinline__ void report(int* status, int code) {
 // products cost the others 4 - 9 % where the epilogue is the bound (13760 x 6664 x 128: 81.7 us against 87.4).
 enum Kind : int { kPlain = 0, kAux = 1, kSplit = 2, kXentStats = 3, kXentGrad = 4, kXentKeep = 5 };
 
-// Vocabulary projection with cross entropy: C, the logits, is not stored (kXentKeep: 16 bits of each).  The statistics' epilogue hides behind the
-// products (4096 x 2048, vocabulary 50304 with bias: 496 us, 1.70 PFLOP/s, tensor pipe 97 % busy), the gradient's almost (25344
-// columns of the same: 259 us, 1.64 PFLOP/s, 88 %).  Long runs of
-// both passes are bound by the power cap: 8192 x 2560 x 50304 6.4 ms for 8 T H V operations, 5.4 where kXentKeep spares the
-// backward pass the logits (its own 1440 us against 1290: 824 MB more to write, one stage less).  A struct of its own, because a parameter
-// more changes the code of the other kinds (registers of the split one 238 -> 164).
+// Vocabulary projection with cross entropy: C, the logits, is not stored (kXentKeep: 16 bits of each).  The statistics' epilogue
+// hides behind the products (4096 x 2048, vocabulary 50304 with bias: 496 us, 1.70 PFLOP/s, tensor pipe 97 % busy), the
+// gradient's almost (25344 columns of the same: 259 us, 1.64 PFLOP/s, 88 %).  Long runs of both passes are bound by the power
+// cap: 8192 x 2560 x 50304 6.4 ms for 8 T H V operations, 5.4 where kXentKeep spares the backward pass the logits (its own 1440
+// us against 1290: 824 MB more to write, one stage less).  A struct of its own, because a parameter more changes the code of
+// the other kinds (registers of the split one 238 -> 164).
 struct XentParams : PairParams {
   const int64_t* labels;      // [M]; the label's column is labels[m] - v0
   int64_t v0, ignore;

@@ -88,8 +88,9 @@ def generate(model: nn.Module, input_ids: torch.Tensor, max_new_tokens: int, eos
         with kv_cache(model, b, total) as ip:
             step_ids = input_ids
             for _ in range(max_new_tokens):
-                if rows is not None and ip.seqlen_offset + step_ids.shape[1] > rows:
-                    raise IndexError(f"position {ip.seqlen_offset + step_ids.shape[1] - 1} is out of bounds: the table has {rows} rows")
+                end = ip.seqlen_offset + step_ids.shape[1]
+                if rows is not None and end > rows:
+                    raise IndexError(f"position {end - 1} is out of bounds: the table has {rows} rows")
                 pos = torch.arange(ip.seqlen_offset, ip.seqlen_offset + step_ids.shape[1], device=input_ids.device)
                 logits = model(step_ids, position_ids=pos.unsqueeze(0).expand(b, -1))
                 ip.seqlen_offset += step_ids.shape[1]

@@ -99,8 +99,8 @@ class TransformerLanguageModel(nn.Module):
         cross attention sees them (defaults to ``enc_attn_mask``).  Masks without padding are dropped.
         A single-stack model takes a :class:`~mist_b200.ops.packed.PackedSequences` of its ``batch * seq`` tokens as
         ``enc_attn_mask``: documents packed back to back, which attend inside themselves and whose positions start at 0.
-        Nothing is pooled from them.  Documents longer than a learned position table are refused (where the offsets are on the GPU, by a status that
-        :func:`~mist_b200.ops.native.check_status` raises)."""
+        Nothing is pooled from them.  Documents longer than a learned position table are refused (where the offsets are on
+        the GPU, by a status that :func:`~mist_b200.ops.native.check_status` raises)."""
         bs = enc_input_ids.shape[0] if enc_input_ids is not None else None
         if enc_hidden_states is None and self.encoder is None and self.enc_hidden_input is not None:
             enc_hidden_states = self.enc_hidden_input
@@ -184,8 +184,7 @@ class LMHead(nn.Module):
                                          dtype=dtype or cfg.params_dtype)
 
     def forward(self, hidden, labels=None, weight=None):
-        fused = (self.fused_loss and labels is not None
-                 and (weight is not None or is_plain_projection(self.proj)))
+        fused = self.fused_loss and labels is not None and (weight is not None or is_plain_projection(self.proj))
         if weight is not None or fused:   # tied embeddings
             x = hidden
             if self.proj.sequence_parallel:

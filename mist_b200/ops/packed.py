@@ -2,8 +2,9 @@
 
 A :class:`PackedSequences` is made once per batch.  It holds the offsets, every token's position in its sequence, and the
 work lists that the attention kernels walk (csrc/packed_plan.cu); all layers, forward and backward, use the same one, and
-nothing is read back to the host, but by ``attention_varlen`` with bare offsets on the GPU (reference: csrc/flash_attn/flash_api.cpp:427, 814 ``varlen_fwd`` / ``varlen_bwd``, called
-with offsets that mist/modules/mha.py:1233-1243 derives from a padding mask)."""
+nothing is read back to the host, but by ``attention_varlen`` with bare offsets on the GPU (reference:
+csrc/flash_attn/flash_api.cpp:427, 814 ``varlen_fwd`` / ``varlen_bwd``, called with offsets that mist/modules/mha.py:1233-1243
+derives from a padding mask)."""
 from __future__ import annotations
 
 import ctypes
@@ -48,8 +49,9 @@ def _offsets(cu, device):
     _check_offsets(host)
     if host[-1] > INT32_MAX:
         raise ValueError(f"offsets up to {host[-1]}: 32 bits hold them")
-    # (to a GPU they go as arguments of a kernel: nothing waits, and a graph that is captured holds them)
-    return torch.empty(len(host), dtype=torch.int32, device=device) if device.type == "cuda" else torch.tensor(host, dtype=torch.int32), host
+    if device.type == "cuda":      # they go there as arguments of a kernel: nothing waits, and a captured graph holds them
+        return torch.empty(len(host), dtype=torch.int32, device=device), host
+    return torch.tensor(host, dtype=torch.int32), host
 
 
 def _check_offsets(host):

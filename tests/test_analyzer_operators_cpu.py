@@ -77,3 +77,10 @@ def test_without_kept_logits_memory_falls(monkeypatch):
 def test_caches_of_the_two_are_apart():
     names = {analysis_cache_name(_cfg("gpt2-t", fused_lm_loss=f), S, 1, False) for f in (False, True)}
     assert len(names) == 2
+
+
+def test_caches_go_by_the_limits_of_the_loss(monkeypatch):
+    cfg = _cfg("gpt2-t", fused_lm_loss=True)
+    first = analysis_cache_name(cfg, S, 1, False)
+    monkeypatch.setattr(F.Settings, "xent_keep_bytes", 0)
+    assert analysis_cache_name(cfg, S, 1, False) != first
