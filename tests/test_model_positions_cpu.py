@@ -77,3 +77,15 @@ def test_the_status_of_a_position_has_a_name():
     from mist_b200.ops import native
     assert "position" in native.status_message(6) and "unknown" in native.status_message(7)
     assert "peer flag" in native.status_message(4)
+
+
+@pytest.mark.parametrize("rank", [0, 1])
+def test_every_rank_refuses_what_the_first_one_refuses(rank):
+    """Only the first rank adds positions; the others must not wait for it in the sum behind the lookup."""
+    from mist_b200.parallel.dist_ops import FakeGroup
+    m = VocabParallelEmbedding(12, 8, max_position_embeddings=7, process_group=FakeGroup(2, rank))
+    ids = torch.zeros(2, 9, dtype=torch.long)
+    with pytest.raises(IndexError):
+        m(ids[:, :3], position_ids=torch.tensor([[0, 1, 7]]))
+    with pytest.raises(ValueError, match="7"):
+        m(ids, position_ids=F.PackedSequences([0, 8, 18]))
